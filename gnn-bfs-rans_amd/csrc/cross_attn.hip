@@ -1,0 +1,633 @@
+// Cross attention of query rows to the states of another mesh
+// (mignn_cross_attn_forward, mignn_cross_attn_backward): the work plan, the
+// exact fp32 kernels and the joins of split work.
+//
+//   s_ij = scale <q_i, k_j> over the keys j of the row's sequence that the mask keeps
+//   P_ij = 2^(c <q_i, k_j> - lse_i),  c = scale log2 e,  lse_i = log2 sum_j 2^(c <q_i, k_j>)
+//   o_i  = sum_j P_ij v_j
+//   delta_i = <do_i, o_i>;  dS_ij = P_ij (<do_i, v_j> - delta_i)
+//   dq_i = scale sum_j dS_ij k_j;  dk_j = scale sum_i dS_ij q_i;  dv_j = sum_i P_ij do_i
+//
+// One pass over the keys with the running maximum and sum of the softmax;
+// scores and P stay in registers: S^T = K Q^T puts a query in a lane's column,
+// so the maximum and the sum are in-lane but for one exchange between the
+// wave's halves, and the result registers of S^T are, as they stand, the B
+// operand of O^T = V^T P^T (the product over keys takes them in the order in
+// which the accumulator holds them).  dq runs like the forward; dk and dv
+// swap the roles (a wave owns 32 keys, rows go by), so nothing is added
+// atomically and results do not depend on the order of workgroups.  The query
+// heads that share a kv head are rows of one tile: their keys are read once,
+// and dk, dv sum over them in place.
+#include "cross_attn.hpp"
+
+#include <cstdlib>
+
+namespace mignn {
+namespace {
+
+// A tile of 32 rows of q or do, or of k or v, into LDS as fp32, columns >= d
+// and rows that `keep` leaves out as zeros.
+template <typename T, int DP, int NT, typename Row>
+__device__ __forceinline__ void stage_tile(float* lds, int d, Row row_ptr) {
+    constexpr int C4 = DP / 4;
+    for (int i = threadIdx.x; i < 32 * C4; i += NT) {
+        const int r = i / C4, c = (i % C4) * 4;
+        const T* p = row_ptr(r);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p && c < d) v = load4(p + c);
+        st4(lds + r * (DP + 4) + c, v);
+    }
+}
+
+// 32 values a lane of one row: columns 8 i + 4 (lane / 32) + 0..3, the k order
+// of the products over columns
+template <typename T, int DP>
+__device__ __forceinline__ void load_frag(float4 (&f)[DP / 8], const T* p, int d, int half) {
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+        const int c = 8 * i + 4 * half;
+        f[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p && c < d) f[i] = load4(p + c);
+    }
+}
+
+__device__ __forceinline__ f32x16 mfma32(float a, float b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
+// acc += (LDS tile row l % 32) . (fragment), over the columns
+template <int DP>
+__device__ __forceinline__ f32x16 dot_tile(const float* tile, const float4 (&f)[DP / 8], int col,
+                                           int half) {
+    f32x16 acc = {};
+    const float* p = tile + col * (DP + 4) + 4 * half;
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+        const float4 a = ld4(p + 8 * i);
+        acc = mfma32(a.x, f[i].x, acc);
+        acc = mfma32(a.y, f[i].y, acc);
+        acc = mfma32(a.z, f[i].z, acc);
+        acc = mfma32(a.w, f[i].w, acc);
+    }
+    return acc;
+}
+
+// acc[b] += tile^T (columns 32 b + l % 32) . w, over the tile's 32 rows in the
+// order in which w's registers hold them
+template <int DP>
+__device__ __forceinline__ void add_tile(const float* tile, const f32x16& w, f32x16 (&acc)[DP / 32],
+                                         int col, int half) {
+    const float* p = tile + 4 * half * (DP + 4) + col;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b)
+            acc[b] = mfma32(p[acc_row(r) * (DP + 4) + 32 * b], w[r], acc[b]);
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_acc(T* p, const f32x16 (&acc)[DP / 32], float f, int d,
+                                          int half) {
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * b + 8 * g + 4 * half;
+            if (c < d) {
+                const float o[4] = {acc[b][4 * g] * f, acc[b][4 * g + 1] * f, acc[b][4 * g + 2] * f,
+                                    acc[b][4 * g + 3] * f};
+                store_row(p + c, o);
+            }
+        }
+}
+
+struct RowRef {
+    int64_t token;
+    int head;
+};
+__device__ __forceinline__ RowRef row_ref(const CrossArgs& a, const CrossItem& it, int row, int kvh) {
+    const int t = row / a.group;
+    return {it.q_begin + static_cast<int64_t>(t), kvh * a.group + (row - t * a.group)};
+}
+
+// partial results: [slot][kv head][rows of the tile][d + 2] (forward: o
+// unnormalised, maximum, sum; dq: dq; dk / dv: dk and dv, 2 d)
+__device__ __forceinline__ float* part_row(const CrossArgs& a, int slot, int kvh, int r, int rows,
+                                           int width) {
+    return a.part + ((static_cast<int64_t>(slot) * a.kv_heads + kvh) * rows + r) * width;
+}
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void cross_fwd_kernel(CrossArgs a) {
+    __shared__ __attribute__((aligned(16))) float ks[32 * (DP + 4)], vs[32 * (DP + 4)];
+    int item, kvh;
+    if (!cross_work(a, a.n_items, item, kvh)) return;
+    const CrossItem it = a.items[item];
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int row = it.r0 + wave * 32 + col;
+    const bool live = row < it.r1;
+    const RowRef ref = row_ref(a, it, row, kvh);
+    float4 qf[DP / 8];
+    load_frag<T, DP>(qf, live ? static_cast<const T*>(a.q) + ref.token * a.ldq + ref.head * a.ldqh
+                              : nullptr, a.d, half);
+    f32x16 o[DP / 32] = {};
+    float m = -INFINITY, l = 0.f;
+    for (int k0 = it.c0; k0 < it.c1; k0 += 32) {
+        const int64_t key0 = it.k_begin + static_cast<int64_t>(k0);
+        const int left = it.c1 - k0;
+        const bool ok = lane < 32 && lane < left && (!a.mask || a.mask[key0 + lane]);
+        const uint32_t bits = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok));
+        __syncthreads();
+        stage_tile<T, DP, NW * 64>(ks, a.d, [&](int r) {
+            return (bits >> r) & 1u ? static_cast<const T*>(a.k) + (key0 + r) * a.ldk + kvh * a.ldkh
+                                    : nullptr;
+        });
+        stage_tile<T, DP, NW * 64>(vs, a.d, [&](int r) {
+            return (bits >> r) & 1u ? static_cast<const T*>(a.v) + (key0 + r) * a.ldv + kvh * a.ldvh
+                                    : nullptr;
+        });
+        __syncthreads();
+        f32x16 s = dot_tile<DP>(ks, qf, col, half);
+        if (bits != 0xffffffffu) {
+            const uint32_t mine = bits >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!((mine >> acc_row(r)) & 1u)) s[r] = -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float mn = fmaxf(m, mx);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f((m - base) * a.c);
+        m = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -base * a.c));
+            sum += s[r];
+        }
+        l = fmaf(l, alpha, sum);
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) o[b] *= alpha;
+        add_tile<DP>(vs, s, o, col, half);
+    }
+    l += __shfl_xor(l, 32);
+    if (!live) return;
+    const float m2 = (m == -INFINITY ? 0.f : m) * a.c;
+    if (it.slot >= 0) {
+        float* p = part_row(a, it.slot, kvh, wave * 32 + col, NW * 32, a.d + 2);
+        store_acc<float, DP>(p, o, 1.f, a.d, half);
+        if (half == 0) p[a.d] = m == -INFINITY ? -INFINITY : m2;
+        else p[a.d + 1] = l;
+        return;
+    }
+    // a row without keys: o = 0, and lse = inf makes every P of the backward 0
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t at = ref.token * a.heads + ref.head;
+    store_acc<T, DP>(static_cast<T*>(a.out) + at * a.d, o, inv, a.d, half);
+    if (a.o32) store_acc<float, DP>(a.o32 + at * a.d, o, inv, a.d, half);
+    if (a.lse && half == 0) a.lse[at] = l == 0.f ? INFINITY : m2 + log2f(l);
+}
+
+// Joins the parts of split rows: one wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void cross_join_fwd_kernel(CrossArgs a, int tile_rows) {
+    const CrossJoin jn = a.joins[blockIdx.x];
+    const int kvh = blockIdx.y, lane = threadIdx.x & 63;
+    for (int r = threadIdx.x >> 6; r < jn.r1 - jn.r0; r += 4) {
+        const int row = jn.r0 + r, t = row / a.group;
+        const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group +
+                           (row - t * a.group);
+        float m = -INFINITY;
+        for (int p = 0; p < jn.parts; ++p)
+            m = fmaxf(m, part_row(a, jn.slot + p, kvh, r, tile_rows, a.d + 2)[a.d]);
+        const float base = m == -INFINITY ? 0.f : m;
+        float l = 0.f, o[2] = {0.f, 0.f};
+        for (int p = 0; p < jn.parts; ++p) {
+            const float* src = part_row(a, jn.slot + p, kvh, r, tile_rows, a.d + 2);
+            const float f = __builtin_amdgcn_exp2f(src[a.d] - base);
+            l = fmaf(src[a.d + 1], f, l);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (lane + 64 * i < a.d) o[i] = fmaf(src[lane + 64 * i], f, o[i]);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = lane + 64 * i;
+            if (c >= a.d) continue;
+            static_cast<T*>(a.out)[at * a.d + c] = static_cast<T>(o[i] * inv);
+            if (a.o32) a.o32[at * a.d + c] = o[i] * inv;
+        }
+        if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : base + log2f(l);
+    }
+}
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void cross_dq_kernel(CrossArgs a) {
+    __shared__ __attribute__((aligned(16))) float ks[32 * (DP + 4)], vs[32 * (DP + 4)];
+    int item, kvh;
+    if (!cross_work(a, a.n_items, item, kvh)) return;
+    const CrossItem it = a.items[item];
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int row = it.r0 + wave * 32 + col;
+    const bool live = row < it.r1;
+    const RowRef ref = row_ref(a, it, row, kvh);
+    const int64_t at = ref.token * a.heads + ref.head;
+    float4 qf[DP / 8], gf[DP / 8];
+    load_frag<T, DP>(qf, live ? static_cast<const T*>(a.q) + ref.token * a.ldq + ref.head * a.ldqh
+                              : nullptr, a.d, half);
+    load_frag<T, DP>(gf, live ? static_cast<const T*>(a.dout) + ref.token * a.lddo +
+                                    ref.head * a.lddoh : nullptr, a.d, half);
+    float delta = 0.f;
+    {
+        const float* o = live ? a.out32 + at * a.d : nullptr;
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+            const int c = 8 * i + 4 * half;
+            if (!o || c >= a.d) continue;
+            const float4 v = ld4(o + c);
+            delta = fmaf(v.x, gf[i].x, fmaf(v.y, gf[i].y, fmaf(v.z, gf[i].z, fmaf(v.w, gf[i].w, delta))));
+        }
+        delta += __shfl_xor(delta, 32);
+        // the dk / dv kernel's: written by the item of the row's first keys
+        if (live && half == 0 && it.c0 == 0) a.delta[at] = delta;
+    }
+    const float lse = live ? a.lse[at] : INFINITY;
+    f32x16 acc[DP / 32] = {};
+    for (int k0 = it.c0; k0 < it.c1; k0 += 32) {
+        const int64_t key0 = it.k_begin + static_cast<int64_t>(k0);
+        const int left = it.c1 - k0;
+        const bool ok = lane < 32 && lane < left && (!a.mask || a.mask[key0 + lane]);
+        const uint32_t bits = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok));
+        __syncthreads();
+        stage_tile<T, DP, NW * 64>(ks, a.d, [&](int r) {
+            return (bits >> r) & 1u ? static_cast<const T*>(a.k) + (key0 + r) * a.ldk + kvh * a.ldkh
+                                    : nullptr;
+        });
+        stage_tile<T, DP, NW * 64>(vs, a.d, [&](int r) {
+            return (bits >> r) & 1u ? static_cast<const T*>(a.v) + (key0 + r) * a.ldv + kvh * a.ldvh
+                                    : nullptr;
+        });
+        __syncthreads();
+        f32x16 s = dot_tile<DP>(ks, qf, col, half);
+        const f32x16 dp = dot_tile<DP>(vs, gf, col, half);
+        const uint32_t mine = bits >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse));
+            s[r] = (mine >> acc_row(r)) & 1u ? p * (dp[r] - delta) : 0.f;
+        }
+        add_tile<DP>(ks, s, acc, col, half);
+    }
+    if (!live) return;
+    if (it.slot >= 0)
+        store_acc<float, DP>(part_row(a, it.slot, kvh, wave * 32 + col, NW * 32, a.d), acc, a.scale,
+                             a.d, half);
+    else
+        store_acc<T, DP>(static_cast<T*>(a.out) + at * a.d, acc, a.scale, a.d, half);
+}
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void cross_dkv_kernel(CrossArgs a) {
+    __shared__ __attribute__((aligned(16))) float qs[32 * (DP + 4)], gs[32 * (DP + 4)];
+    __shared__ __attribute__((aligned(16))) float ls[32], ds[32];
+    int item, kvh;
+    if (!cross_work(a, a.n_items, item, kvh)) return;
+    const CrossItem it = a.items[item];
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int key = it.r0 + wave * 32 + col;
+    const int64_t kt = it.k_begin + static_cast<int64_t>(key);
+    const bool live = key < it.r1;
+    const bool keep = live && (!a.mask || a.mask[kt]);
+    float4 kf[DP / 8], vf[DP / 8];
+    load_frag<T, DP>(kf, keep ? static_cast<const T*>(a.k) + kt * a.ldk + kvh * a.ldkh : nullptr,
+                     a.d, half);
+    load_frag<T, DP>(vf, keep ? static_cast<const T*>(a.v) + kt * a.ldv + kvh * a.ldvh : nullptr,
+                     a.d, half);
+    f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+    for (int r0 = it.c0; r0 < it.c1; r0 += 32) {
+        __syncthreads();
+        stage_tile<T, DP, NW * 64>(qs, a.d, [&](int r) -> const T* {
+            if (r0 + r >= it.c1) return nullptr;
+            const RowRef ref = row_ref(a, it, r0 + r, kvh);
+            return static_cast<const T*>(a.q) + ref.token * a.ldq + ref.head * a.ldqh;
+        });
+        stage_tile<T, DP, NW * 64>(gs, a.d, [&](int r) -> const T* {
+            if (r0 + r >= it.c1) return nullptr;
+            const RowRef ref = row_ref(a, it, r0 + r, kvh);
+            return static_cast<const T*>(a.dout) + ref.token * a.lddo + ref.head * a.lddoh;
+        });
+        if (threadIdx.x < 32) {
+            const bool in = r0 + static_cast<int>(threadIdx.x) < it.c1;
+            const RowRef ref = row_ref(a, it, r0 + threadIdx.x, kvh);
+            ls[threadIdx.x] = in ? a.lse[ref.token * a.heads + ref.head] : INFINITY;
+            ds[threadIdx.x] = in ? a.delta[ref.token * a.heads + ref.head] : 0.f;
+        }
+        __syncthreads();
+        f32x16 s = dot_tile<DP>(qs, kf, col, half);
+        f32x16 dp = dot_tile<DP>(gs, vf, col, half);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 lse = ld4(ls + 8 * g + 4 * half), del = ld4(ds + 8 * g + 4 * half);
+            const float lv[4] = {lse.x, lse.y, lse.z, lse.w}, ev[4] = {del.x, del.y, del.z, del.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * g + e;
+                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lv[e]));
+                dp[r] = s[r] * (dp[r] - ev[e]);
+            }
+        }
+        add_tile<DP>(gs, s, dv, col, half);
+        add_tile<DP>(qs, dp, dk, col, half);
+    }
+    if (!live) return;
+    // a key that the mask leaves out has no gradient, whatever its rows hold
+    if (!keep) {
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) dk[b] = dv[b] = f32x16{};
+    }
+    if (it.slot >= 0) {
+        float* p = part_row(a, it.slot, kvh, wave * 32 + col, NW * 32, 2 * a.d);
+        store_acc<float, DP>(p, dk, a.scale, a.d, half);
+        store_acc<float, DP>(p + a.d, dv, 1.f, a.d, half);
+    } else {
+        const int64_t at = (kt * a.kv_heads + kvh) * a.d;
+        store_acc<T, DP>(static_cast<T*>(a.dk) + at, dk, a.scale, a.d, half);
+        store_acc<T, DP>(static_cast<T*>(a.dv) + at, dv, 1.f, a.d, half);
+    }
+}
+
+// Sums the parts of split gradients in slot order: `width` floats a row, one
+// wave a row; dq (dkv = false) or dk | dv.
+template <typename T>
+__global__ __launch_bounds__(256) void cross_join_grad_kernel(CrossArgs a, int tile_rows, bool dkv) {
+    const CrossJoin jn = a.joins[blockIdx.x];
+    const int kvh = blockIdx.y, lane = threadIdx.x & 63;
+    const int width = dkv ? 2 * a.d : a.d;
+    for (int r = threadIdx.x >> 6; r < jn.r1 - jn.r0; r += 4) {
+        const int row = jn.r0 + r;
+        for (int c = lane; c < width; c += 64) {
+            float v = 0.f;
+            for (int p = 0; p < jn.parts; ++p)
+                v += part_row(a, jn.slot + p, kvh, r, tile_rows, width)[c];
+            if (dkv) {
+                const int64_t at = ((jn.begin + static_cast<int64_t>(row)) * a.kv_heads + kvh) * a.d;
+                T* dst = static_cast<T*>(c < a.d ? a.dk : a.dv);
+                dst[at + (c < a.d ? c : c - a.d)] = static_cast<T>(v);
+            } else {
+                const int t = row / a.group;
+                const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group +
+                                   (row - t * a.group);
+                static_cast<T*>(a.out)[at * a.d + c] = static_cast<T>(v);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Plan
+
+constexpr int CROSS_WAVES = 4;
+constexpr int CROSS_TILE = CROSS_WAVES * CROSS_ROWS;
+
+// Tiles of the "r" side (rows or keys) times chunks of the "c" side.  The
+// chunk is chosen so that the pass has about two workgroups for each of the
+// 256 CUs when the tiles alone are fewer; it stays a multiple of 32 and not
+// under 256, where a part's join would cost what the split gains.
+struct PassPlan {
+    int64_t items = 0, joins = 0, slots = 0;
+};
+
+int64_t pass_chunk(const int64_t* rows, const int64_t* keys, int64_t batch, bool dkv, int heads) {
+    double work = 0.0;
+    for (int64_t b = 0; b < batch; ++b) {
+        const int64_t r = dkv ? keys[b] : rows[b], c = dkv ? rows[b] : keys[b];
+        work += static_cast<double>((r + CROSS_TILE - 1) / CROSS_TILE) * static_cast<double>(c);
+    }
+    const double share = work * heads / 512.0;
+    int64_t chunk = static_cast<int64_t>(share);
+    if (chunk < 256) chunk = 256;
+    return (chunk + 31) / 32 * 32;
+}
+
+PassPlan plan_pass(const int64_t* rows, const int64_t* queries, const int64_t* keys, int64_t batch,
+                   bool dkv, int heads, CrossItem* items, CrossJoin* joins) {
+    const int64_t chunk = pass_chunk(rows, keys, batch, dkv, heads);
+    PassPlan p;
+    int64_t qb = 0, kb = 0;
+    for (int64_t b = 0; b < batch; ++b) {
+        const int64_t rn = dkv ? keys[b] : rows[b], cn = dkv ? rows[b] : keys[b];
+        int64_t parts = (cn + chunk - 1) / chunk;
+        if (parts < 1) parts = 1;
+        // equal parts, each a multiple of 32 but the last
+        const int64_t len = cn == 0 ? 0 : ((cn + parts - 1) / parts + 31) / 32 * 32;
+        if (len > 0) parts = (cn + len - 1) / len;
+        for (int64_t r0 = 0; r0 < rn; r0 += CROSS_TILE) {
+            const int64_t r1 = r0 + CROSS_TILE < rn ? r0 + CROSS_TILE : rn;
+            if (joins && parts > 1)
+                joins[p.joins] = {static_cast<int32_t>(dkv ? kb : qb), static_cast<int32_t>(r0),
+                                  static_cast<int32_t>(r1), static_cast<int32_t>(p.slots),
+                                  static_cast<int32_t>(parts), {0, 0, 0}};
+            for (int64_t s = 0; s < parts; ++s) {
+                if (items) {
+                    const int64_t c0 = s * len, c1 = c0 + len < cn ? c0 + len : cn;
+                    items[p.items] = {static_cast<int32_t>(qb), static_cast<int32_t>(kb),
+                                      static_cast<int32_t>(r0), static_cast<int32_t>(r1),
+                                      static_cast<int32_t>(c0), static_cast<int32_t>(c1),
+                                      parts > 1 ? static_cast<int32_t>(p.slots + s) : -1, 0};
+                }
+                ++p.items;
+            }
+            if (parts > 1) {
+                ++p.joins;
+                p.slots += parts;
+            }
+        }
+        qb += queries[b];
+        kb += keys[b];
+    }
+    return p;
+}
+
+int64_t part_width(int pass, int d) {
+    return pass == MIGNN_CROSS_FORWARD ? d + 2 : pass == MIGNN_CROSS_DQ ? d : 2 * d;
+}
+
+template <typename K>
+void launch_cross(K kernel, const CrossArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL(kernel, dim3(cross_grid(a.n_items, a.kv_heads)), dim3(CROSS_WAVES * 64), 0,
+                       st, a);
+}
+
+template <typename T, int DP>
+int run_pass_d(const CrossArgs& a, int pass, hipStream_t st) {
+    if (a.n_items > 0) {
+        if (pass == MIGNN_CROSS_FORWARD) launch_cross(cross_fwd_kernel<T, DP, CROSS_WAVES>, a, st);
+        else if (pass == MIGNN_CROSS_DQ) launch_cross(cross_dq_kernel<T, DP, CROSS_WAVES>, a, st);
+        else launch_cross(cross_dkv_kernel<T, DP, CROSS_WAVES>, a, st);
+        if (int rc = launch_status("cross attention kernel")) return rc;
+    }
+    if (a.n_joins == 0) return MIGNN_OK;
+    const dim3 grid(a.n_joins, a.kv_heads);
+    if (pass == MIGNN_CROSS_FORWARD)
+        hipLaunchKernelGGL(cross_join_fwd_kernel<T>, grid, dim3(256), 0, st, a, CROSS_TILE);
+    else
+        hipLaunchKernelGGL(cross_join_grad_kernel<T>, grid, dim3(256), 0, st, a, CROSS_TILE,
+                           pass == MIGNN_CROSS_DKV);
+    return launch_status("cross attention join");
+}
+
+template <typename T>
+int run_pass_t(const CrossArgs& a, int pass, hipStream_t st) {
+    if (a.d <= 32) return run_pass_d<T, 32>(a, pass, st);
+    if (a.d <= 64) return run_pass_d<T, 64>(a, pass, st);
+    if (a.d <= 96) return run_pass_d<T, 96>(a, pass, st);
+    return run_pass_d<T, 128>(a, pass, st);
+}
+
+int run_pass(const CrossArgs& a, int pass, int dtype, hipStream_t st) {
+    switch (dtype) {
+        case MIGNN_ROW_F32: return run_pass_t<float>(a, pass, st);
+        case MIGNN_ROW_BF16: return run_pass_t<bf16_t>(a, pass, st);
+        default: return run_pass_t<f16_t>(a, pass, st);
+    }
+}
+
+// dims of a plan's pass (mignn_cross_plan): items, joins, slots, scratch bytes
+int check_dims(const char* who, int heads, int kv_heads, int d, int dtype) {
+    MIGNN_REQUIRE(row_type_ok(dtype), "%s: unknown row type %d", who, dtype);
+    MIGNN_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads <= 65535,
+                  "%s: %d query heads over %d key heads", who, heads, kv_heads);
+    MIGNN_REQUIRE(d > 0 && d % 8 == 0 && d <= MIGNN_CROSS_MAX_D, "%s: head width %d (a multiple of 8, <= %d)",
+                  who, d, MIGNN_CROSS_MAX_D);
+    return MIGNN_OK;
+}
+
+int check_rows(const char* who, const char* what, const void* p, int64_t ldt, int64_t ldh,
+               int dtype) {
+    const int64_t es = row_type_size(dtype);
+    MIGNN_REQUIRE(p && aligned16(p) && ldt >= 0 && ldh >= 0 && ldt * es % 16 == 0 &&
+                      ldh * es % 16 == 0,
+                  "%s: %s needs a 16-byte aligned pointer and strides", who, what);
+    return MIGNN_OK;
+}
+
+}  // namespace
+}  // namespace mignn
+
+using namespace mignn;
+
+extern "C" int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, int64_t batch,
+                                int heads, int kv_heads, int d, int dtype, int pass, void* items,
+                                void* joins, int64_t* info) {
+    if (int rc = check_dims("cross_plan", heads, kv_heads, d, dtype)) return rc;
+    MIGNN_REQUIRE(pass >= MIGNN_CROSS_FORWARD && pass <= MIGNN_CROSS_DKV, "cross_plan: unknown pass %d",
+                  pass);
+    MIGNN_REQUIRE(batch >= 0 && (batch == 0 || (q_lens && k_lens)) && info,
+                  "cross_plan: null pointer or negative batch");
+    const int64_t group = heads / kv_heads;
+    int64_t queries = 0, keys = 0;
+    for (int64_t b = 0; b < batch; ++b) {
+        MIGNN_REQUIRE(q_lens[b] >= 0 && k_lens[b] >= 0, "cross_plan: negative length in sequence %lld",
+                      static_cast<long long>(b));
+        MIGNN_REQUIRE(q_lens[b] <= INT32_MAX / group - CROSS_TILE && k_lens[b] <= INT32_MAX - CROSS_TILE,
+                      "cross_plan: sequence %lld too long", static_cast<long long>(b));
+        queries += q_lens[b];
+        keys += k_lens[b];
+        MIGNN_REQUIRE(queries <= INT32_MAX && keys <= INT32_MAX, "cross_plan: more than 2^31 - 1 rows");
+    }
+    int64_t* rows = static_cast<int64_t*>(malloc(sizeof(int64_t) * (batch > 0 ? batch : 1)));
+    MIGNN_REQUIRE(rows, "cross_plan: out of host memory");
+    for (int64_t b = 0; b < batch; ++b) rows[b] = q_lens[b] * group;
+    const PassPlan p = plan_pass(rows, q_lens, k_lens, batch, pass == MIGNN_CROSS_DKV, kv_heads,
+                                 static_cast<CrossItem*>(items), static_cast<CrossJoin*>(joins));
+    free(rows);
+    MIGNN_REQUIRE(p.items * kv_heads <= INT32_MAX / 2 && p.joins <= INT32_MAX,
+                  "cross_plan: too many tiles");
+    info[0] = p.items;
+    info[1] = p.joins;
+    info[2] = p.slots * kv_heads * CROSS_TILE * part_width(pass, d) * static_cast<int64_t>(sizeof(float));
+    info[3] = queries;
+    info[4] = keys;
+    return MIGNN_OK;
+}
+
+extern "C" int mignn_cross_attn_forward(const mignn_cross_call* c, void* out, float* out32, float* lse,
+                                        void* stream) {
+    MIGNN_REQUIRE(c, "cross_attn_forward: null call");
+    const char* who = "cross_attn_forward";
+    if (int rc = check_dims(who, c->heads, c->kv_heads, c->d, c->dtype)) return rc;
+    const mignn_cross_pass& ps = c->pass[MIGNN_CROSS_FORWARD];
+    if (ps.n_items == 0) return MIGNN_OK;
+    MIGNN_REQUIRE(c->scale > 0.f && c->scale <= 3.0e38f, "%s: scale must be positive", who);
+    if (int rc = check_rows(who, "q", c->q, c->ldq, c->ldqh, c->dtype)) return rc;
+    if (c->n_keys > 0) {
+        if (int rc = check_rows(who, "k", c->k, c->ldk, c->ldkh, c->dtype)) return rc;
+        if (int rc = check_rows(who, "v", c->v, c->ldv, c->ldvh, c->dtype)) return rc;
+    }
+    MIGNN_REQUIRE(out && aligned16(out) && (!out32 || aligned16(out32)), "%s: output pointer", who);
+    MIGNN_REQUIRE(ps.items && (ps.n_joins == 0 || ps.joins), "%s: no plan", who);
+    if (ps.part_bytes > 0 && (!c->scratch || c->scratch_bytes < static_cast<size_t>(ps.part_bytes))) {
+        set_error("%s: scratch %zu bytes, need %lld", who, c->scratch_bytes,
+                  static_cast<long long>(ps.part_bytes));
+        return MIGNN_ERR_SCRATCH;
+    }
+    CrossArgs a{};
+    a.q = c->q, a.k = c->k, a.v = c->v, a.mask = c->key_mask;
+    a.out = out, a.o32 = out32, a.lse = lse, a.part = static_cast<float*>(c->scratch);
+    a.items = static_cast<const CrossItem*>(ps.items);
+    a.joins = static_cast<const CrossJoin*>(ps.joins);
+    a.ldq = c->ldq, a.ldqh = c->ldqh, a.ldk = c->ldk, a.ldkh = c->ldkh, a.ldv = c->ldv, a.ldvh = c->ldvh;
+    a.n_items = ps.n_items, a.n_joins = ps.n_joins;
+    a.heads = c->heads, a.kv_heads = c->kv_heads, a.group = c->heads / c->kv_heads, a.d = c->d;
+    a.scale = c->scale, a.c = c->scale * LOG2E;
+    return run_pass(a, MIGNN_CROSS_FORWARD, c->dtype, as_stream(stream));
+}
+
+extern "C" int mignn_cross_attn_backward(const mignn_cross_call* c, const void* dout, int64_t lddo,
+                                         int64_t lddoh, const float* out32, const float* lse,
+                                         float* delta, void* dq, void* dk, void* dv, void* stream) {
+    MIGNN_REQUIRE(c, "cross_attn_backward: null call");
+    const char* who = "cross_attn_backward";
+    if (int rc = check_dims(who, c->heads, c->kv_heads, c->d, c->dtype)) return rc;
+    const mignn_cross_pass &pq = c->pass[MIGNN_CROSS_DQ], &pk = c->pass[MIGNN_CROSS_DKV];
+    MIGNN_REQUIRE(c->scale > 0.f && c->scale <= 3.0e38f, "%s: scale must be positive", who);
+    if (pq.n_items > 0) {
+        if (int rc = check_rows(who, "q", c->q, c->ldq, c->ldqh, c->dtype)) return rc;
+        if (int rc = check_rows(who, "dout", dout, lddo, lddoh, c->dtype)) return rc;
+        MIGNN_REQUIRE(out32 && aligned16(out32) && lse && delta && dq && aligned16(dq) && pq.items,
+                      "%s: null or unaligned pointer", who);
+    }
+    const bool keys = dk || dv;
+    if (c->n_keys > 0) {
+        if (int rc = check_rows(who, "k", c->k, c->ldk, c->ldkh, c->dtype)) return rc;
+        if (int rc = check_rows(who, "v", c->v, c->ldv, c->ldvh, c->dtype)) return rc;
+        MIGNN_REQUIRE(!keys || (dk && dv && aligned16(dk) && aligned16(dv) && pk.items),
+                      "%s: null or unaligned pointer", who);
+    }
+    const int64_t need = pq.part_bytes > pk.part_bytes ? pq.part_bytes : pk.part_bytes;
+    if (need > 0 && (!c->scratch || c->scratch_bytes < static_cast<size_t>(need))) {
+        set_error("%s: scratch %zu bytes, need %lld", who, c->scratch_bytes, static_cast<long long>(need));
+        return MIGNN_ERR_SCRATCH;
+    }
+    CrossArgs a{};
+    a.q = c->q, a.k = c->k, a.v = c->v, a.mask = c->key_mask;
+    a.dout = dout, a.out32 = out32, a.lse = const_cast<float*>(lse), a.delta = delta;
+    a.out = dq, a.dk = dk, a.dv = dv, a.part = static_cast<float*>(c->scratch);
+    a.ldq = c->ldq, a.ldqh = c->ldqh, a.ldk = c->ldk, a.ldkh = c->ldkh, a.ldv = c->ldv, a.ldvh = c->ldvh;
+    a.lddo = lddo, a.lddoh = lddoh;
+    a.heads = c->heads, a.kv_heads = c->kv_heads, a.group = c->heads / c->kv_heads, a.d = c->d;
+    a.scale = c->scale, a.c = c->scale * LOG2E;
+    for (int pass : {MIGNN_CROSS_DQ, MIGNN_CROSS_DKV}) {   // dq first: it writes delta
+        if (pass == MIGNN_CROSS_DKV && !keys) break;
+        const mignn_cross_pass& ps = c->pass[pass];
+        a.items = static_cast<const CrossItem*>(ps.items);
+        a.joins = static_cast<const CrossJoin*>(ps.joins);
+        a.n_items = ps.n_items, a.n_joins = ps.n_joins;
+        if (int rc = run_pass(a, pass, c->dtype, as_stream(stream))) return rc;
+    }
+    return MIGNN_OK;
+}

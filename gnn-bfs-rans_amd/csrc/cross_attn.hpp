@@ -1,0 +1,77 @@
+// Shared by the cross-attention sources (cross_attn.hip: plan, exact fp32
+// kernels, joins).
+#pragma once
+
+#include "row_types.hpp"
+
+namespace mignn {
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+
+constexpr int CROSS_ROWS = 32;    // rows (or keys) a wave owns: one MFMA tile edge
+constexpr float LOG2E = 1.44269504088896340736f;
+
+// One workgroup's share of a pass, per kv head.  "Rows" are the (query, head
+// of the group) pairs of one sequence: row r is query r / G, head kvh G + r % G.
+// Forward and dq: r0..r1 rows of the tile, c0..c1 keys to go through;
+// dk / dv:        r0..r1 keys of the tile, c0..c1 rows to go through.
+struct CrossItem {
+    int32_t q_begin, k_begin;   // first query / key of the sequence
+    int32_t r0, r1, c0, c1;
+    int32_t slot;               // partial results' slot, -1: the item is its tile's only one
+    int32_t reserved;
+};
+static_assert(sizeof(CrossItem) == MIGNN_CROSS_ITEM_BYTES, "plan item layout");
+
+// The items of one tile that several workgroups share: slots slot .. slot + parts - 1.
+struct CrossJoin {
+    int32_t begin;              // first query (forward, dq) or key (dk / dv) of the sequence
+    int32_t r0, r1;
+    int32_t slot, parts;
+    int32_t reserved[3];
+};
+static_assert(sizeof(CrossJoin) == MIGNN_CROSS_ITEM_BYTES, "plan join layout");
+
+struct CrossArgs {
+    const void *q, *k, *v;
+    const uint8_t* mask;
+    const void* dout;
+    const float* out32;          // fp32 outputs of the forward (training)
+    void *out, *dk, *dv;         // out: the forward's output or dq
+    float *o32, *lse, *delta;
+    float* part;                 // partial results
+    const CrossItem* items;
+    const CrossJoin* joins;
+    int64_t ldq, ldqh, ldk, ldkh, ldv, ldvh, lddo, lddoh;
+    int32_t n_items, n_joins, heads, kv_heads, group, d;
+    float scale, c;              // c = scale log2(e)
+};
+
+// Block -> (item, kv head).  Consecutive blocks go to the 8 XCDs in turn; each
+// XCD gets one run of the (head-major) work, so that the tiles that read one
+// head's keys and values share an L2.
+__device__ __forceinline__ bool cross_work(const CrossArgs& a, int n_items, int& item, int& kvh) {
+    const int64_t total = static_cast<int64_t>(n_items) * a.kv_heads;
+    const int64_t per = (total + 7) / 8;
+    const int64_t w = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= per || w >= total) return false;
+    kvh = static_cast<int>(w / n_items);
+    item = static_cast<int>(w - static_cast<int64_t>(kvh) * n_items);
+    return true;
+}
+inline unsigned cross_grid(int64_t n_items, int kv_heads) {
+    return static_cast<unsigned>((n_items * kv_heads + 7) / 8 * 8);
+}
+
+// Position in the sequence of an accumulator's element: MFMA 32x32 results
+// hold D[8 (r / 4) + 4 (lane / 32) + r % 4][lane % 32] in register r.
+__device__ __forceinline__ constexpr int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+    float o[4];
+    load_row(p, o);
+    return make_float4(o[0], o[1], o[2], o[3]);
+}
+
+}  // namespace mignn

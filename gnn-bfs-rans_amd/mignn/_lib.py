@@ -22,10 +22,32 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 # the same ABI-version check.  The product path never sets it.
 VARIANT_ENV = "MIGNN_LIB_VARIANT"
 
+ROW_F32, ROW_BF16, ROW_F16 = 0, 1, 2
+POS_F32, POS_F64, POS_I32, POS_I64 = 0, 1, 2, 3
+CROSS_FORWARD, CROSS_DQ, CROSS_DKV = 0, 1, 2
+CROSS_MAX_D, CROSS_ITEM_BYTES, RMS_NORM_MAX_H = 128, 32, 2048
 EPI_BIAS, EPI_RESIDUAL, EPI_AFFINE, EPI_RELU = 1, 2, 4, 8
 CSR_VERBATIM, CSR_ONE_SELF_LOOP, CSR_TRANSPOSE = 0, 1, 4
 
 _P = c_void_p
+
+
+class CrossPass(ctypes.Structure):
+    """mignn_cross_pass"""
+    _fields_ = [("items", c_void_p), ("joins", c_void_p), ("part_bytes", c_int64),
+                ("n_items", ctypes.c_int32), ("n_joins", ctypes.c_int32)]
+
+
+class CrossCall(ctypes.Structure):
+    """mignn_cross_call"""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("key_mask", c_void_p),
+                ("ldq", c_int64), ("ldqh", c_int64), ("ldk", c_int64), ("ldkh", c_int64),
+                ("ldv", c_int64), ("ldvh", c_int64), ("n_keys", c_int64),
+                ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("d", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("scale", c_float), ("reserved", ctypes.c_int32),
+                ("scratch", c_void_p), ("scratch_bytes", c_size_t), ("passes", CrossPass * 3)]
+
+
 # name -> (restype, argtypes); mirrors include/mignn.h
 SIGNATURES = {
     "mignn_abi_version": (c_int, []),
@@ -172,6 +194,17 @@ SIGNATURES = {
     "mignn_gcn_norm": (c_int, [_P, _P, _P, c_int64, c_int64, _P, _P]),
     "mignn_rows_gather": (c_int, [_P, c_int64, _P, c_int64, c_int, _P, c_int64, _P]),
     "mignn_grid_graph": (c_int, [c_int, c_int, c_int, c_int, c_int, _P, _P, _P]),
+    "mignn_rms_norm": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, c_int64, c_int, c_float, c_int,
+                               _P, c_int64, _P, c_int64, _P]),
+    "mignn_rms_norm_backward_scratch_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "mignn_rms_norm_backward": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, c_int64, c_int,
+                                        c_float, c_int, _P, c_int64, _P, c_int64, _P, c_int64, _P,
+                                        _P, c_size_t, _P]),
+    "mignn_rotary": (c_int, [_P, c_int64, c_int64, c_int64, c_int, c_int, _P, c_int, c_int64, _P,
+                             _P, c_int, c_int, c_int, c_int, _P, c_int64, c_int64, _P]),
+    "mignn_cross_plan": (c_int, [_P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, _P, _P, _P]),
+    "mignn_cross_attn_forward": (c_int, [_P, _P, _P, _P, _P]),
+    "mignn_cross_attn_backward": (c_int, [_P, _P, c_int64, c_int64, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 # diagnostic entry points (include/mignn_diag.h; timing studies only)

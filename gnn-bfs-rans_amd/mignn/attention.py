@@ -1,0 +1,452 @@
+"""Operators on activation rows for attention between two meshes: rows of one
+graph (cells, or single probe points) read the states of an encoder that ran
+over another graph of another size.
+
+  rms_norm         root-mean-square norm with the residual's addition
+  rotary           rotary positions over several axes (cell coordinates)
+  cross_attention  softmax attention of query rows to another sequence's keys
+
+Rows are fp32, bf16 or fp16; sums, softmax statistics and norms are fp32 and
+each output is rounded once.  All three run and differentiate in HIP kernels
+of libmignn.so on the tensors' device and its current stream; there is no CPU
+path.  Outputs and scratch come from PyTorch's allocator at every call, so
+calls on several streams, or captured into several graphs, share nothing but
+the read-only `RotaryAxes` / `CrossPlan`.  Gradients are first order only.
+
+A graph batch is a list of lengths (one sequence a graph), rows back to back.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+import torch.nn as nn
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from . import train_ops as T
+
+P = _lib.ptr
+
+_ROW = {torch.float32: _lib.ROW_F32, torch.bfloat16: _lib.ROW_BF16, torch.float16: _lib.ROW_F16}
+_POS = {torch.float32: _lib.POS_F32, torch.float64: _lib.POS_F64, torch.int32: _lib.POS_I32,
+        torch.int64: _lib.POS_I64}
+
+
+def _row_type(what: str, t: torch.Tensor) -> int:
+    code = _ROW.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: rows must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _on_device(what: str, ref: torch.Tensor, **others):
+    if ref.device.type != "cuda":
+        raise RuntimeError(f"mignn {what} runs on ROCm devices only (no CPU path)")
+    for name, t in others.items():
+        if t is not None and t.device != ref.device:
+            raise RuntimeError(f"mignn {what}: {name} is on {t.device}, not on {ref.device}")
+
+
+class _device_of:
+    """Makes a tensor's device current around a launch (nothing to do when it
+    is)."""
+    __slots__ = ("index", "prev")
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+def _grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+# ---------------------------------------------------------------------------
+# Root-mean-square norm
+
+def _matrix(t: torch.Tensor) -> torch.Tensor:
+    """Rows with contiguous columns that do not overlap (a copy if need be)."""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        return t.contiguous()
+    return t
+
+
+def _norm_forward(x, weight, residual, eps: float, code: int):
+    x = _matrix(x)
+    residual = None if residual is None else _matrix(residual)
+    weight = weight.contiguous()
+    n, h = x.shape
+    y = torch.empty((n, h), dtype=x.dtype, device=x.device)
+    s = None if residual is None else torch.empty_like(y)
+    with _device_of(x):
+        _lib.check(_lib.lib().mignn_rms_norm(
+            P(x), x.stride(0), P(residual), 0 if residual is None else residual.stride(0),
+            P(weight), weight.dtype == torch.float32, n, h, eps, code, P(y), h, P(s), h,
+            _lib.stream(x.device)), "mignn_rms_norm")
+    return y, s
+
+
+class _RMSNorm(Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps: float, code: int):
+        y, s = _norm_forward(x, weight, residual, eps, code)
+        ctx.eps, ctx.code, ctx.residual = eps, code, residual is not None
+        ctx.set_materialize_grads(False)
+        # fp32 rows: the stored s is the s that was normed; 16-bit rows: it is
+        # rounded, so the gradient adds x and the residual again
+        if s is not None and x.dtype == torch.float32:
+            ctx.save_for_backward(s, weight, None)
+        else:
+            ctx.save_for_backward(x, weight, residual)
+        return y if s is None else (y, s)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds=None):
+        x, weight, residual = ctx.saved_tensors
+        if dy is None:
+            dx = ds
+            dw = torch.zeros_like(weight) if ctx.needs_input_grad[1] else None
+            return dx, dw, dx if ctx.residual else None, None, None
+        x, dy = _matrix(x), _matrix(dy)
+        residual = None if residual is None else _matrix(residual)
+        ds = None if ds is None else _matrix(ds)
+        weight = weight.contiguous()
+        n, h = x.shape
+        dx = torch.empty((n, h), dtype=x.dtype, device=x.device)
+        dw = scratch = None
+        nbytes = 0
+        L = _lib.lib()
+        if ctx.needs_input_grad[1]:
+            dw = torch.empty_like(weight)
+            nbytes = L.mignn_rms_norm_backward_scratch_bytes(n, h, ctx.code)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        with _device_of(x):
+            _lib.check(L.mignn_rms_norm_backward(
+                P(x), x.stride(0), P(residual), 0 if residual is None else residual.stride(0),
+                P(weight), weight.dtype == torch.float32, n, h, ctx.eps, ctx.code, P(dy),
+                dy.stride(0), P(ds), 0 if ds is None else ds.stride(0), P(dx), h, P(dw),
+                P(scratch), nbytes, _lib.stream(x.device)), "mignn_rms_norm_backward")
+        return dx, dw, dx if ctx.residual else None, None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
+             eps: float = 1e-6):
+    """y = s / sqrt(mean(s^2) + eps) * weight over the columns of x [N, H].
+
+    Without `residual`, s = x and y is returned; with it (x's shape and type)
+    s = x + residual and (y, s) is returned, s being the stream that the next
+    residual adds to.  y is formed from the unrounded s.  weight: [H], float32
+    or x's type.  H <= 2048."""
+    if x.dim() != 2:
+        raise ValueError(f"rms_norm: x must be [N, H], got {tuple(x.shape)}")
+    code = _row_type("rms_norm", x)
+    h = x.shape[1]
+    if not 1 <= h <= _lib.RMS_NORM_MAX_H:
+        raise ValueError(f"rms_norm: width {h} is not in 1..{_lib.RMS_NORM_MAX_H}")
+    if weight.dim() != 1 or weight.shape[0] != h:
+        raise ValueError(f"rms_norm: weight must be [{h}], got {tuple(weight.shape)}")
+    if weight.dtype != torch.float32 and weight.dtype != x.dtype:
+        raise TypeError(f"rms_norm: weight must be float32 or {x.dtype}, got {weight.dtype}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"rms_norm: residual must be {tuple(x.shape)} {x.dtype}, got "
+                         f"{tuple(residual.shape)} {residual.dtype}")
+    if not eps >= 0.0:
+        raise ValueError(f"rms_norm: eps must not be negative, got {eps}")
+    _on_device("rms_norm", x, weight=weight, residual=residual)
+    if _grad(x, weight, residual):
+        return _RMSNorm.apply(x, weight, residual, float(eps), code)
+    y, s = _norm_forward(x, weight, residual, float(eps), code)
+    return y if s is None else (y, s)
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions
+
+class RotaryAxes:
+    """The rotated pairs of each position axis and their frequencies.
+
+    pairs[a] column pairs of a head belong to axis a, in order; pair i of axis
+    a turns by pos[a] * scales[a] * base^(-i / pairs[a]) radians.  Pair j of
+    all is columns (j, j + sum(pairs)), or (2j, 2j + 1) when `interleaved`;
+    further columns of a head pass through.  Immutable; one device."""
+
+    __slots__ = ("pairs", "base", "scales", "interleaved", "device", "freq", "axis", "total")
+
+    def __init__(self, pairs: Sequence[int], base: float = 10000.0,
+                 scales: Optional[Sequence[float]] = None, interleaved: bool = False,
+                 device="cuda"):
+        self.pairs = tuple(int(m) for m in pairs)
+        if not self.pairs or any(m < 0 for m in self.pairs) or sum(self.pairs) == 0:
+            raise ValueError(f"RotaryAxes: pairs must be counts with a positive sum, got {pairs}")
+        if not (base > 0.0 and math.isfinite(base)):
+            raise ValueError(f"RotaryAxes: base must be positive and finite, got {base}")
+        self.scales = tuple(float(s) for s in scales) if scales is not None \
+            else (1.0,) * len(self.pairs)
+        if len(self.scales) != len(self.pairs) or not all(math.isfinite(s) for s in self.scales):
+            raise ValueError(f"RotaryAxes: {len(self.pairs)} finite scales expected, got {scales}")
+        self.base, self.interleaved = float(base), bool(interleaved)
+        self.total = sum(self.pairs)
+        freq = [s * self.base ** (-i / m) / (2.0 * math.pi)
+                for m, s in zip(self.pairs, self.scales) for i in range(m)]
+        axis = [a for a, m in enumerate(self.pairs) for _ in range(m)]
+        self.freq = torch.tensor(freq, dtype=torch.float64).to(device)
+        self.axis = torch.tensor(axis, dtype=torch.int32).to(device)
+        self.device = self.freq.device
+
+
+def _heads(t: torch.Tensor, align: int = 1) -> torch.Tensor:
+    """[rows, heads, d] with contiguous columns; align: bytes that the pointer
+    and the strides are multiples of (a copy if need be)."""
+    es = t.element_size()
+    if (t.shape[2] > 1 and t.stride(2) != 1) or t.data_ptr() % align or \
+            t.stride(0) * es % align or t.stride(1) * es % align:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _turn(x, pos, axes: RotaryAxes, code: int, inverse: bool):
+    x = _heads(x)
+    n, heads, d = x.shape
+    if pos.shape[1] > 1 and pos.stride(1) != 1:
+        pos = pos.contiguous()
+    y = torch.empty((n, heads, d), dtype=x.dtype, device=x.device)
+    with _device_of(x):
+        _lib.check(_lib.lib().mignn_rotary(
+            P(x), x.stride(0), x.stride(1), n, heads, d, P(pos), _POS[pos.dtype], pos.stride(0),
+            P(axes.freq), P(axes.axis), axes.total, axes.interleaved, inverse, code, P(y),
+            heads * d, d, _lib.stream(x.device)), "mignn_rotary")
+    return y
+
+
+class _Rotary(Function):
+    @staticmethod
+    def forward(ctx, x, pos, axes, code: int):
+        ctx.axes, ctx.code = axes, code
+        ctx.save_for_backward(pos)
+        return _turn(x, pos, axes, code, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (pos,) = ctx.saved_tensors
+        return _turn(dy, pos, ctx.axes, ctx.code, True), None, None, None
+
+
+def rotary(x: torch.Tensor, pos: torch.Tensor, axes: RotaryAxes) -> torch.Tensor:
+    """x [N, heads, d] with the pairs of every head turned by the row's
+    position pos [N, len(axes.pairs)] (float32 / float64 coordinates or int32 /
+    int64 indices; angles are formed in float64).  Positions get no gradient."""
+    if x.dim() != 3:
+        raise ValueError(f"rotary: x must be [N, heads, d], got {tuple(x.shape)}")
+    code = _row_type("rotary", x)
+    if pos.dim() != 2 or pos.shape[0] != x.shape[0] or pos.shape[1] != len(axes.pairs):
+        raise ValueError(f"rotary: pos must be [{x.shape[0]}, {len(axes.pairs)}], got "
+                         f"{tuple(pos.shape)}")
+    if pos.dtype not in _POS:
+        raise TypeError("rotary: pos must be float32, float64, int32 or int64, got "
+                        f"{pos.dtype}")
+    if 2 * axes.total > x.shape[2]:
+        raise ValueError(f"rotary: {axes.total} pairs do not fit heads of width {x.shape[2]}")
+    if torch.is_grad_enabled() and pos.requires_grad:
+        raise NotImplementedError("rotary: positions get no gradient (pass pos.detach())")
+    _on_device("rotary", x, pos=pos, axes=axes.freq)
+    if _grad(x):
+        return _Rotary.apply(x, pos, axes, code)
+    return _turn(x, pos, axes, code, False)
+
+
+# ---------------------------------------------------------------------------
+# Cross attention
+
+def _lengths(what: str, lens) -> np.ndarray:
+    if torch.is_tensor(lens):
+        if lens.device.type != "cpu":
+            raise ValueError(f"CrossPlan: {what} must be on the host (they size the launches)")
+        lens = lens.tolist()
+    if isinstance(lens, (int, np.integer)):
+        lens = [lens]
+    a = np.asarray(lens)
+    if a.size and (a.dtype.kind not in "iu"):
+        raise ValueError(f"CrossPlan: {what} must be whole numbers")
+    a = np.ascontiguousarray(a.reshape(-1), dtype=np.int64)
+    if a.size and a.min() < 0:
+        raise ValueError(f"CrossPlan: negative length in {what}")
+    return a
+
+
+class CrossPlan:
+    """The work of cross attention for given lengths: q_lens[b] queries read
+    k_lens[b] keys, the sequences' rows back to back (one int: a single
+    sequence).  Lengths of 0 are allowed.  Holds the launches' work lists on
+    `device`; immutable, so it may serve any number of calls, streams and
+    captured graphs.  train=False leaves the backward's lists out."""
+
+    __slots__ = ("q_lens", "k_lens", "queries", "keys", "heads", "kv_heads", "head_dim", "dtype",
+                 "device", "train", "_call", "_lists", "_scratch")
+
+    def __init__(self, q_lens, k_lens, *, heads: int, kv_heads: Optional[int] = None,
+                 head_dim: int, dtype: torch.dtype = torch.float32, device="cuda",
+                 train: bool = True):
+        ql, kl = _lengths("q_lens", q_lens), _lengths("k_lens", k_lens)
+        if ql.size != kl.size:
+            raise ValueError(f"CrossPlan: {ql.size} query sequences but {kl.size} key sequences")
+        kv_heads = heads if kv_heads is None else kv_heads
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise ValueError(f"CrossPlan: {heads} query heads over {kv_heads} key heads")
+        if head_dim < 8 or head_dim % 8 or head_dim > _lib.CROSS_MAX_D:
+            raise ValueError(f"CrossPlan: head_dim must be a multiple of 8 up to "
+                             f"{_lib.CROSS_MAX_D}, got {head_dim}")
+        if dtype not in _ROW:
+            raise TypeError(f"CrossPlan: rows must be float32, bfloat16 or float16, got {dtype}")
+        self.q_lens, self.k_lens = tuple(ql.tolist()), tuple(kl.tolist())
+        self.heads, self.kv_heads, self.head_dim = int(heads), int(kv_heads), int(head_dim)
+        self.dtype, self.train = dtype, bool(train)
+        self.queries, self.keys = int(ql.sum()), int(kl.sum())
+        L = _lib.lib()
+        info = np.zeros(5, np.int64)
+        lists, spans, at = [], [], 0
+        size = _lib.CROSS_ITEM_BYTES
+        for kind in range(3 if train else 1):
+            def plan(items, joins):
+                _lib.check(L.mignn_cross_plan(
+                    ql.ctypes.data, kl.ctypes.data, ql.size, self.heads, self.kv_heads,
+                    self.head_dim, _ROW[dtype], kind, items, joins, info.ctypes.data),
+                    "mignn_cross_plan")
+            plan(None, None)
+            n_items, n_joins, part = (int(v) for v in info[:3])
+            buf = np.zeros((n_items + n_joins) * size, np.uint8)
+            plan(buf.ctypes.data, buf.ctypes.data + n_items * size)
+            spans.append((at, at + n_items * size, part, n_items, n_joins))
+            lists.append(buf)
+            at += buf.size
+        host = torch.from_numpy(np.concatenate(lists))
+        self._lists = host.to(device)
+        self.device = self._lists.device
+        base = self._lists.data_ptr()
+        call = _lib.CrossCall()
+        call.heads, call.kv_heads, call.d = self.heads, self.kv_heads, self.head_dim
+        call.dtype, call.n_keys = _ROW[dtype], self.keys
+        for kind, (items, joins, part, n_items, n_joins) in enumerate(spans):
+            ps = call.passes[kind]
+            ps.items, ps.joins, ps.part_bytes = base + items, base + joins, part
+            ps.n_items, ps.n_joins = n_items, n_joins
+        self._call = call
+        parts = [s[2] for s in spans]
+        self._scratch = (parts[0], max(parts[1:]) if train else 0)
+
+
+def _cross_call(q, k, v, plan: CrossPlan, mask, scale: float, scratch):
+    c = _lib.CrossCall.from_buffer_copy(plan._call)
+    c.q, c.k, c.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    c.key_mask = None if mask is None else mask.data_ptr()
+    c.ldq, c.ldqh = q.stride(0), q.stride(1)
+    c.ldk, c.ldkh = k.stride(0), k.stride(1)
+    c.ldv, c.ldvh = v.stride(0), v.stride(1)
+    c.scale = scale
+    if scratch is not None:
+        c.scratch, c.scratch_bytes = scratch.data_ptr(), scratch.numel()
+    return c
+
+
+def _scratch(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _cross_forward(q, k, v, plan: CrossPlan, mask, scale: float, train: bool):
+    q, k, v = _heads(q, 16), _heads(k, 16), _heads(v, 16)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out32 = lse = None
+    if train:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        if q.dtype != torch.float32:
+            out32 = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    with _device_of(q):
+        scratch = _scratch(plan._scratch[0], q.device)
+        c = _cross_call(q, k, v, plan, mask, scale, scratch)
+        _lib.check(_lib.lib().mignn_cross_attn_forward(
+            ctypes.addressof(c), P(out), P(out32), P(lse), _lib.stream(q.device)),
+            "mignn_cross_attn_forward")
+    return out, (out if out32 is None else out32), lse
+
+
+class _CrossAttention(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, plan: CrossPlan, mask, scale: float):
+        out, out32, lse = _cross_forward(q, k, v, plan, mask, scale, True)
+        ctx.plan, ctx.scale = plan, scale
+        # out32 (the fp32 output): <do, o> from the rounded output would leave
+        # the rounding of o in every dS
+        ctx.save_for_backward(q, k, v, mask, out32, lse)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, mask, out32, lse = ctx.saved_tensors
+        plan = ctx.plan
+        q, k, v, dout = _heads(q, 16), _heads(k, 16), _heads(v, 16), _heads(dout, 16)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = dv = None
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        delta = torch.empty_like(lse)
+        with _device_of(q):
+            scratch = _scratch(plan._scratch[1], q.device)
+            c = _cross_call(q, k, v, plan, mask, ctx.scale, scratch)
+            _lib.check(_lib.lib().mignn_cross_attn_backward(
+                ctypes.addressof(c), P(dout), dout.stride(0), dout.stride(1), P(out32), P(lse),
+                P(delta), P(dq), P(dk), P(dv), _lib.stream(q.device)),
+                "mignn_cross_attn_backward")
+        need = ctx.needs_input_grad
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None,
+                None, None)
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: CrossPlan,
+                    key_mask: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of q [queries, heads, d] to k, v [keys, kv_heads, d], each
+    sequence of `plan` to its own keys; query head h reads key head
+    h // (heads // kv_heads).  key_mask: bool [keys], False leaves a key out,
+    whatever its rows hold.  scale: > 0, default 1 / sqrt(d).  Returns
+    [queries, heads, d]; a query without keys gets 0, and no gradient flows
+    through it."""
+    want_q = (plan.queries, plan.heads, plan.head_dim)
+    want_k = (plan.keys, plan.kv_heads, plan.head_dim)
+    for name, t, want in (("q", q, want_q), ("k", k, want_k), ("v", v, want_k)):
+        if tuple(t.shape) != want:
+            raise ValueError(f"cross_attention: the plan's {name} is {want}, got {tuple(t.shape)}")
+        if t.dtype != plan.dtype:
+            raise TypeError(f"cross_attention: the plan's rows are {plan.dtype}, {name} is "
+                            f"{t.dtype}")
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (plan.keys,):
+            raise ValueError(f"cross_attention: key_mask must be bool [{plan.keys}], got "
+                             f"{key_mask.dtype} {tuple(key_mask.shape)}")
+    scale = 1.0 / math.sqrt(plan.head_dim) if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"cross_attention: scale must be positive and finite, got {scale}")
+    _on_device("cross_attention", q, k=k, v=v, key_mask=key_mask, plan=plan._lists)
+    if key_mask is not None:
+        key_mask = key_mask.contiguous()
+    if _grad(q, k, v):
+        if not plan.train:
+            raise ValueError("cross_attention: gradients need a plan built with train=True")
+        return _CrossAttention.apply(q, k, v, plan, key_mask, scale)
+    return _cross_forward(q, k, v, plan, key_mask, scale, False)[0]

@@ -725,6 +725,83 @@ int mignn_transformer_train_backward(const int32_t* row_ptr, const int32_t* col,
                                      uint64_t seed, float* stats, float* dqkv, int64_t ldd,
                                      void* stream);
 
+/* ------------------------------------------------------------------------
+ * Operators on activation rows (mignn.attention): rows of fp32, bf16 or fp16,
+ * sums in fp32, one rounding at the store.  No reference counterpart.
+ * ------------------------------------------------------------------------ */
+enum { MIGNN_ROW_F32 = 0, MIGNN_ROW_BF16 = 1, MIGNN_ROW_F16 = 2 };
+enum { MIGNN_POS_F32 = 0, MIGNN_POS_F64 = 1, MIGNN_POS_I32 = 2, MIGNN_POS_I64 = 3 };
+
+/* y = s / sqrt(mean_h s^2 + eps) * weight, s = x + residual (residual NULL:
+ * s = x); s is written when the pointer is given.  weight: fp32 (weight_f32)
+ * or the rows' type.  h <= MIGNN_RMS_NORM_MAX_H.  Outputs must not overlap the
+ * inputs. */
+#define MIGNN_RMS_NORM_MAX_H 2048
+int mignn_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                   const void* weight, int weight_f32, int64_t n, int h, float eps, int dtype,
+                   void* y, int64_t ldy, void* s, int64_t lds, void* stream);
+/* Gradients: dx (the residual's is the same) from dy and, when given, ds (the
+ * gradient of s); dw in the weight's type, or NULL.  Scratch is needed for dw. */
+size_t mignn_rms_norm_backward_scratch_bytes(int64_t n, int h, int dtype);
+int mignn_rms_norm_backward(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                            const void* weight, int weight_f32, int64_t n, int h, float eps,
+                            int dtype, const void* dy, int64_t lddy, const void* ds, int64_t ldds,
+                            void* dx, int64_t lddx, void* dw, void* scratch, size_t scratch_bytes,
+                            void* stream);
+
+/* Rotary positions: pair j of every head of row i turned by
+ * 2 pi pos[i, axis[j]] freq[j] (freq fp64, in turns), the other way round when
+ * `inverse`.  Pairs are columns (j, j + pairs), or (2j, 2j + 1) when
+ * `interleaved`; columns from 2 pairs on are copied.  ldt / ldh, ldyt / ldyh:
+ * strides of rows and heads in elements, columns contiguous; y must not
+ * overlap x.  Every axis[j] indexes a column of pos. */
+int mignn_rotary(const void* x, int64_t ldt, int64_t ldh, int64_t n, int heads, int d,
+                 const void* pos, int pos_type, int64_t ldp, const double* freq,
+                 const int32_t* axis, int pairs, int interleaved, int inverse, int dtype, void* y,
+                 int64_t ldyt, int64_t ldyh, void* stream);
+
+/* Cross attention over a batch of sequences: query i of sequence b attends to
+ * the keys of sequence b that key_mask keeps.  q [queries, heads, d], k and v
+ * [keys, kv_heads, d], query head h reads kv head h / (heads / kv_heads).
+ * mignn_cross_plan runs on the HOST: given the lengths it fills the work items
+ * and joins of one pass (host memory, MIGNN_CROSS_ITEM_BYTES each; either may
+ * be NULL to count) and info[5] = {items, joins, scratch bytes, queries, keys}.
+ * The caller copies them to the device. */
+#define MIGNN_CROSS_MAX_D 128
+#define MIGNN_CROSS_ITEM_BYTES 32
+enum { MIGNN_CROSS_FORWARD = 0, MIGNN_CROSS_DQ = 1, MIGNN_CROSS_DKV = 2 };
+int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, int64_t batch, int heads,
+                     int kv_heads, int d, int dtype, int pass, void* items, void* joins,
+                     int64_t* info);
+typedef struct {
+    const void* items;      /* device */
+    const void* joins;      /* device */
+    int64_t part_bytes;
+    int32_t n_items, n_joins;
+} mignn_cross_pass;
+typedef struct {
+    const void *q, *k, *v;
+    const uint8_t* key_mask;     /* [keys], 0 leaves a key out; NULL: all kept */
+    int64_t ldq, ldqh, ldk, ldkh, ldv, ldvh;   /* strides of rows and heads, elements */
+    int64_t n_keys;
+    int32_t heads, kv_heads, d, dtype;
+    float scale;
+    int32_t reserved;
+    void* scratch;
+    size_t scratch_bytes;
+    mignn_cross_pass pass[3];
+} mignn_cross_call;
+/* out [queries, heads, d] contiguous, in the rows' type; for the backward also
+ * out32 (the same in fp32; fp32 rows: pass out itself there and NULL here) and lse [queries,
+ * heads] (log2 of the softmax's sum).  A query without keys: out = 0. */
+int mignn_cross_attn_forward(const mignn_cross_call* call, void* out, float* out32, float* lse,
+                             void* stream);
+/* dq, dk, dv contiguous, shaped as q, k, v (dk and dv both NULL: dq alone); delta: scratch [queries, heads].
+ * Gradients of left-out keys are 0. */
+int mignn_cross_attn_backward(const mignn_cross_call* call, const void* dout, int64_t lddo,
+                              int64_t lddoh, const float* out32, const float* lse, float* delta,
+                              void* dq, void* dk, void* dv, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
