@@ -390,8 +390,7 @@ __global__ __launch_bounds__(256) void cross_join_grad_kernel(CrossArgs a, int t
 // ---------------------------------------------------------------------------
 // Plan
 
-constexpr int CROSS_WAVES = 4;
-constexpr int CROSS_TILE = CROSS_WAVES * CROSS_ROWS;
+constexpr int CROSS_WAVES = CROSS_TILE / CROSS_ROWS;
 
 // Tiles of the "r" side (rows or keys) times chunks of the "c" side.  The
 // chunk is chosen so that the pass has about two workgroups for each of the
@@ -462,38 +461,44 @@ void launch_cross(K kernel, const CrossArgs& a, hipStream_t st) {
                        st, a);
 }
 
-template <typename T, int DP>
-int run_pass_d(const CrossArgs& a, int pass, hipStream_t st) {
-    if (a.n_items > 0) {
-        if (pass == MIGNN_CROSS_FORWARD) launch_cross(cross_fwd_kernel<T, DP, CROSS_WAVES>, a, st);
-        else if (pass == MIGNN_CROSS_DQ) launch_cross(cross_dq_kernel<T, DP, CROSS_WAVES>, a, st);
-        else launch_cross(cross_dkv_kernel<T, DP, CROSS_WAVES>, a, st);
-        if (int rc = launch_status("cross attention kernel")) return rc;
-    }
-    if (a.n_joins == 0) return MIGNN_OK;
+template <int DP>
+void launch_exact(const CrossArgs& a, int pass, hipStream_t st) {
+    if (pass == MIGNN_CROSS_FORWARD) launch_cross(cross_fwd_kernel<float, DP, CROSS_WAVES>, a, st);
+    else if (pass == MIGNN_CROSS_DQ) launch_cross(cross_dq_kernel<float, DP, CROSS_WAVES>, a, st);
+    else launch_cross(cross_dkv_kernel<float, DP, CROSS_WAVES>, a, st);
+}
+
+int cross_pass_exact(const CrossArgs& a, int pass, hipStream_t st) {
+    if (a.d <= 32) launch_exact<32>(a, pass, st);
+    else if (a.d <= 64) launch_exact<64>(a, pass, st);
+    else if (a.d <= 96) launch_exact<96>(a, pass, st);
+    else launch_exact<128>(a, pass, st);
+    return launch_status("cross attention kernel");
+}
+
+template <typename T>
+void launch_join(const CrossArgs& a, int pass, hipStream_t st) {
     const dim3 grid(a.n_joins, a.kv_heads);
     if (pass == MIGNN_CROSS_FORWARD)
         hipLaunchKernelGGL(cross_join_fwd_kernel<T>, grid, dim3(256), 0, st, a, CROSS_TILE);
     else
         hipLaunchKernelGGL(cross_join_grad_kernel<T>, grid, dim3(256), 0, st, a, CROSS_TILE,
                            pass == MIGNN_CROSS_DKV);
-    return launch_status("cross attention join");
-}
-
-template <typename T>
-int run_pass_t(const CrossArgs& a, int pass, hipStream_t st) {
-    if (a.d <= 32) return run_pass_d<T, 32>(a, pass, st);
-    if (a.d <= 64) return run_pass_d<T, 64>(a, pass, st);
-    if (a.d <= 96) return run_pass_d<T, 96>(a, pass, st);
-    return run_pass_d<T, 128>(a, pass, st);
 }
 
 int run_pass(const CrossArgs& a, int pass, int dtype, hipStream_t st) {
-    switch (dtype) {
-        case MIGNN_ROW_F32: return run_pass_t<float>(a, pass, st);
-        case MIGNN_ROW_BF16: return run_pass_t<bf16_t>(a, pass, st);
-        default: return run_pass_t<f16_t>(a, pass, st);
+    if (a.n_items > 0) {
+        const int rc = dtype == MIGNN_ROW_F32 ? cross_pass_exact(a, pass, st)
+                                              : cross_pass16(a, pass, dtype, st);
+        if (rc) return rc;
     }
+    if (a.n_joins == 0) return MIGNN_OK;
+    switch (dtype) {
+        case MIGNN_ROW_F32: launch_join<float>(a, pass, st); break;
+        case MIGNN_ROW_BF16: launch_join<bf16_t>(a, pass, st); break;
+        default: launch_join<f16_t>(a, pass, st); break;
+    }
+    return launch_status("cross attention join");
 }
 
 // dims of a plan's pass (mignn_cross_plan): items, joins, slots, scratch bytes

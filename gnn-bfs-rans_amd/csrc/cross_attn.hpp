@@ -1,5 +1,5 @@
 // Shared by the cross-attention sources (cross_attn.hip: plan, exact fp32
-// kernels, joins).
+// kernels, joins; cross_attn16.hip: 16-bit kernels).
 #pragma once
 
 #include "row_types.hpp"
@@ -9,6 +9,7 @@ namespace mignn {
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 
 constexpr int CROSS_ROWS = 32;    // rows (or keys) a wave owns: one MFMA tile edge
+constexpr int CROSS_TILE = 4 * CROSS_ROWS;   // of a workgroup
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // One workgroup's share of a pass, per kv head.  "Rows" are the (query, head
@@ -73,5 +74,8 @@ __device__ __forceinline__ float4 load4(const T* p) {
     load_row(p, o);
     return make_float4(o[0], o[1], o[2], o[3]);
 }
+
+// the 16-bit rows' kernels of a pass (cross_attn16.hip)
+int cross_pass16(const CrossArgs& a, int pass, int dtype, hipStream_t st);
 
 }  // namespace mignn

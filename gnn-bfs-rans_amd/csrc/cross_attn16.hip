@@ -1,0 +1,658 @@
+// Cross attention of bf16 and fp16 rows on the 16-bit matrix instructions
+// (formulas and pass structure: cross_attn.hip).
+//
+// A wave owns CB blocks of 32 rows (forward, dq) or keys (dk / dv) as MFMA
+// columns.  The other side comes in LDS tiles of 64, double buffered through
+// registers: while a tile is worked on, the next one's rows are in flight.
+//   S^T (keys x rows)   A = key rows, 16 bytes a lane;  B = q, in registers
+//   O^T (d x rows)      A = V^T, read transposed from the row-major tile
+//                       (ds_read_b64_tr_b16: 4 rows x 16 columns a 16-lane
+//                       group);  B = P^T, the accumulator of S^T rounded in
+//                       place: the product over keys takes them in the order
+//                       in which its registers hold them
+// dq and dk / dv are made of the same two forms.  Row pitch: the tile's width
+// plus 32 bytes, so that neither 8 rows' 16-byte reads nor 4 rows' transposed
+// reads meet in a bank.
+//
+// P and dS are rounded to the rows' type ahead of their second product (the
+// matrix instruction takes both operands in one type); statistics, sums and
+// accumulators are fp32.  bf16 has fp32's range.  fp16 has not: a weight of
+// 1 / 5000 is already subnormal there, so P is carried up by a constant power
+// of two and dS by one that each row (dq) or key (dk) lowers when its values
+// would not fit (DsScale); the results are brought back in fp32.
+#include "cross_attn.hpp"
+
+namespace mignn {
+namespace {
+
+template <typename T>
+using vec8 = T __attribute__((ext_vector_type(8)));
+template <typename T>
+using vec2 = T __attribute__((ext_vector_type(2)));
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using lds_s16x4 = __attribute__((address_space(3))) s16x4;
+
+__device__ __forceinline__ f32x16 mfma16(vec8<bf16_t> a, vec8<bf16_t> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma16(vec8<f16_t> a, vec8<f16_t> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr int KT = 64;   // rows of an LDS tile
+
+template <int DP>
+constexpr int pitch() { return DP * 2 + 32; }
+
+// the transposed read's share of a lane: row 4 half + (l % 16) / 4, columns
+// 16 ((l / 16) % 2) + 4 (l % 4) ..+3
+template <int DP>
+__device__ __forceinline__ int tr_lane(int lane) {
+    return (4 * (lane >> 5) + ((lane & 15) >> 2)) * pitch<DP>() + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+}
+
+// A operand of a product over rows 16 t + (the accumulator's order) of a tile:
+// columns 32 b + l % 32
+template <typename T, int DP>
+__device__ __forceinline__ vec8<T> tr_frag(const char* tile, int trl, int row, int b) {
+    const char* p = tile + trl + row * pitch<DP>() + 64 * b;
+    union {
+        s16x4 h[2];
+        vec8<T> v;
+    } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * pitch<DP>()));
+    return u.v;
+}
+
+// A operand of a product over columns: row r + l % 32, columns 16 i + 8 half ..+7
+template <typename T, int DP>
+__device__ __forceinline__ vec8<T> row_frag(const char* tile, int r, int i, int col, int half) {
+    return *reinterpret_cast<const vec8<T>*>(tile + (r + col) * pitch<DP>() + 32 * i + 16 * half);
+}
+
+// B operand rows held in registers
+template <typename T, int DP>
+__device__ __forceinline__ void load_frag16(vec8<T> (&f)[DP / 16], const T* p, int d, int half) {
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+        const int c = 16 * i + 8 * half;
+        f[i] = vec8<T>{};
+        if (p && c < d) f[i] = *reinterpret_cast<const vec8<T>*>(p + c);
+    }
+}
+
+// registers 8 t ..+7 of a 32 x 32 accumulator as the B operand of 16 rows
+template <typename T>
+__device__ __forceinline__ vec8<T> pack8(const f32x16& w, int t) {
+    vec8<T> v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(w[8 * t + i]);
+    return v;
+}
+
+// One thread's share of a 64-row tile on its way from memory to LDS
+template <typename T, int DP, int NT>
+struct Stage {
+    static constexpr int C8 = DP / 8, N = KT * C8 / NT;
+    static_assert(KT * C8 % NT == 0, "tile share");
+    u32x4 v[N];
+    __device__ __forceinline__ static int row(int j) { return (threadIdx.x + j * NT) / C8; }
+    __device__ __forceinline__ static int chunk(int j) { return (threadIdx.x + j * NT) % C8; }
+    // rows from..to - 1 of a matrix of row stride ld; rows past the end repeat the last
+    __device__ __forceinline__ void load(const T* base, int64_t ld, int left, int d) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = row(j) < left ? row(j) : left - 1;
+            v[j] = u32x4{};
+            if (chunk(j) * 8 < d)
+                v[j] = *reinterpret_cast<const u32x4*>(base + r * ld + chunk(j) * 8);
+        }
+    }
+    __device__ __forceinline__ void write(char* tile, uint64_t keep) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const u32x4 x = (keep >> row(j)) & 1u ? v[j] : u32x4{};
+            *reinterpret_cast<u32x4*>(tile + row(j) * pitch<DP>() + chunk(j) * 16) = x;
+        }
+    }
+};
+
+// Which of the 64 keys from k0 on take part (bit = key), for every lane
+__device__ __forceinline__ uint64_t key_bits(const CrossArgs& a, int64_t key0, int left, int lane) {
+    const bool ok = lane < left && (!a.mask || a.mask[key0 + lane]);
+    return __builtin_amdgcn_ballot_w64(ok);
+}
+
+__device__ __forceinline__ float swap_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float swap_add(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_acc16(T* p, const f32x16 (&acc)[DP / 32], float f, int d, int half) {
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * b + 8 * g + 4 * half;
+            if (c < d) {
+                const float o[4] = {acc[b][4 * g] * f, acc[b][4 * g + 1] * f, acc[b][4 * g + 2] * f,
+                                    acc[b][4 * g + 3] * f};
+                store_row(p + c, o);
+            }
+        }
+}
+
+// fp16's P is kept 2^8 up: a weight down to 2^-22 of the largest keeps its
+// full precision, and 2^(8 + 6) stays below fp16's largest.  bf16 has fp32's
+// range.
+template <typename T>
+constexpr float P_UP = 0.f;
+template <>
+constexpr float P_UP<f16_t> = 8.f;
+// the running maximum is raised when a score passes it by this power of two
+constexpr float MAX_SLACK = 6.f;
+
+template <typename T>
+constexpr bool NARROW = sizeof(T) == 2 && !__is_same(T, bf16_t);
+// P's power of two in the dk / dv kernel, where it is at most 1
+template <typename T>
+constexpr float PB_UP = NARROW<T> ? 14.f : 0.f;
+
+// dS of one row (or key) as fp16: 2^up dS.  When a value passes 2^15, `up` is
+// lowered so that the largest comes to 2^8 and what is summed so far is
+// brought along, in the same way as a softmax's maximum.
+template <typename T>
+struct DsScale {
+    float up = NARROW<T> ? 12.f : 0.f;
+    template <int NB>
+    __device__ __forceinline__ bool fit(f32x16& ds, f32x16 (&acc)[NB]) {
+        if constexpr (!NARROW<T>) return false;
+        float mx = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(ds[r]));
+        if (!__any(mx > 32768.f)) return false;
+        mx = swap_max(mx);
+        const int e = static_cast<int>((__float_as_uint(mx) >> 23) & 255u) - 127 - 7;
+        const float down = mx > 32768.f ? static_cast<float>(e) : 0.f;
+        const float f = __builtin_amdgcn_exp2f(-down);
+        up -= down;
+        ds *= f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b] *= f;
+        return true;
+    }
+    __device__ __forceinline__ float back() const { return NARROW<T> ? __builtin_amdgcn_exp2f(-up) : 1.f; }
+};
+
+template <typename T, int DP, int NW, int CB>
+__global__ __launch_bounds__(NW * 64) void cross_fwd16_kernel(CrossArgs a) {
+    constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
+    __shared__ __attribute__((aligned(16))) char lds[4 * TILE];   // K, V; twice
+    int item, kvh;
+    if (!cross_work(a, a.n_items, item, kvh)) return;
+    const CrossItem it = a.items[item];
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int trl = tr_lane<DP>(lane);
+    vec8<T> qf[CB][DP / 16];
+    int row[CB];
+    int64_t at[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        row[cb] = it.r0 + (wave * CB + cb) * 32 + col;
+        const int t = row[cb] / a.group, h = kvh * a.group + row[cb] - t * a.group;
+        const int64_t token = it.q_begin + static_cast<int64_t>(t);
+        at[cb] = token * a.heads + h;
+        load_frag16<T, DP>(qf[cb], row[cb] < it.r1 ? static_cast<const T*>(a.q) + token * a.ldq + h * a.ldqh
+                                                   : nullptr, a.d, half);
+    }
+    f32x16 o[CB][DP / 32] = {};
+    float m[CB], l[CB];   // m: the maximum in use, raw scores
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) m[cb] = -INFINITY, l[cb] = 0.f;
+    const T* kbase = static_cast<const T*>(a.k) + kvh * a.ldkh;
+    const T* vbase = static_cast<const T*>(a.v) + kvh * a.ldvh;
+    Stage<T, DP, NT> sk, sv;
+    uint64_t bits = 0, next = 0;
+    if (it.c0 < it.c1) {
+        const int64_t key0 = it.k_begin + static_cast<int64_t>(it.c0);
+        const int left = it.c1 - it.c0;
+        sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
+        sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
+        bits = key_bits(a, key0, left, lane);
+        sk.write(lds, ~0ull);
+        sv.write(lds + TILE, bits);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int k0 = it.c0; k0 < it.c1; k0 += KT) {
+        const char* kt = lds + buf * 2 * TILE;
+        const char* vt = kt + TILE;
+        const bool more = k0 + KT < it.c1;
+        if (more) {
+            const int64_t key0 = it.k_begin + static_cast<int64_t>(k0 + KT);
+            const int left = it.c1 - k0 - KT;
+            sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
+            sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
+            next = key_bits(a, key0, left, lane);
+        }
+        f32x16 s[CB][2] = {};
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const vec8<T> f = row_frag<T, DP>(kt, 32 * kb, i, col, half);
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) s[cb][kb] = mfma16(f, qf[cb][i], s[cb][kb]);
+            }
+        if (bits != ~0ull) {
+            const uint64_t mine = bits >> (4 * half);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!((mine >> (32 * kb + acc_row(r))) & 1u)) {
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb) s[cb][kb][r] = -INFINITY;
+                    }
+        }
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            float mx = s[cb][0][0];
+#pragma unroll
+            for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[cb][r >> 4][r & 15]);
+            mx = swap_max(mx);
+            // (m = -inf: any score raises it)
+            if (__any((mx - m[cb]) * a.c > MAX_SLACK)) {
+                const float mn = fmaxf(m[cb], mx);
+                const float alpha = m[cb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[cb] - mn) * a.c);
+                m[cb] = mn;
+                l[cb] *= alpha;
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b) o[cb][b] *= alpha;
+            }
+            const float shift = P_UP<T> - (m[cb] == -INFINITY ? 0.f : m[cb]) * a.c;
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 32; ++r) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[cb][r >> 4][r & 15], a.c, shift));
+                s[cb][r >> 4][r & 15] = p;
+                sum += p;
+            }
+            l[cb] += sum;
+        }
+#pragma unroll
+        for (int t = 0; t < KT / 16; ++t) {
+            vec8<T> p[CB];
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) p[cb] = pack8<T>(s[cb][t >> 1], t & 1);
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b) {
+                const vec8<T> f = tr_frag<T, DP>(vt, trl, 16 * t, b);
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) o[cb][b] = mfma16(f, p[cb], o[cb][b]);
+            }
+        }
+        if (more) {
+            char* dst = lds + (buf ^ 1) * 2 * TILE;
+            sk.write(dst, ~0ull);
+            sv.write(dst + TILE, next);
+        }
+        __syncthreads();
+        buf ^= 1;
+        bits = next;
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        const float sum = swap_add(l[cb]);
+        if (row[cb] >= it.r1) continue;
+        const float m2 = (m[cb] == -INFINITY ? 0.f : m[cb]) * a.c - P_UP<T>;
+        if (it.slot >= 0) {
+            float* p = a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
+                                 row[cb] - it.r0) * (a.d + 2);
+            store_acc16<float, DP>(p, o[cb], 1.f, a.d, half);
+            if (half == 0) p[a.d] = m[cb] == -INFINITY ? -INFINITY : m2;
+            else p[a.d + 1] = sum;
+            continue;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        store_acc16<T, DP>(static_cast<T*>(a.out) + at[cb] * a.d, o[cb], inv, a.d, half);
+        if (a.o32) store_acc16<float, DP>(a.o32 + at[cb] * a.d, o[cb], inv, a.d, half);
+        if (a.lse && half == 0) a.lse[at[cb]] = sum == 0.f ? INFINITY : m2 + log2f(sum);
+    }
+}
+
+template <typename T, int DP, int NW, int CB>
+__global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
+    constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
+    __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+    int item, kvh;
+    if (!cross_work(a, a.n_items, item, kvh)) return;
+    const CrossItem it = a.items[item];
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int trl = tr_lane<DP>(lane);
+    vec8<T> qf[CB][DP / 16], gf[CB][DP / 16];
+    int row[CB];
+    int64_t at[CB];
+    float lse[CB], delta[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        row[cb] = it.r0 + (wave * CB + cb) * 32 + col;
+        const bool live = row[cb] < it.r1;
+        const int t = row[cb] / a.group, h = kvh * a.group + row[cb] - t * a.group;
+        const int64_t token = it.q_begin + static_cast<int64_t>(t);
+        at[cb] = token * a.heads + h;
+        load_frag16<T, DP>(qf[cb], live ? static_cast<const T*>(a.q) + token * a.ldq + h * a.ldqh : nullptr,
+                           a.d, half);
+        load_frag16<T, DP>(gf[cb], live ? static_cast<const T*>(a.dout) + token * a.lddo + h * a.lddoh
+                                        : nullptr, a.d, half);
+        float del = 0.f;
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const int c = 16 * i + 8 * half;
+                if (c >= a.d) continue;
+                const float4 x = ld4(a.out32 + at[cb] * a.d + c), y = ld4(a.out32 + at[cb] * a.d + c + 4);
+                const float ov[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) del = fmaf(ov[e], static_cast<float>(gf[cb][i][e]), del);
+            }
+        }
+        delta[cb] = swap_add(del);
+        // the dk / dv kernel's: written by the item of the row's first keys
+        if (live && half == 0 && it.c0 == 0) a.delta[at[cb]] = delta[cb];
+        lse[cb] = live ? a.lse[at[cb]] : INFINITY;
+    }
+    f32x16 acc[CB][DP / 32] = {};
+    DsScale<T> sc[CB];
+    const T* kbase = static_cast<const T*>(a.k) + kvh * a.ldkh;
+    const T* vbase = static_cast<const T*>(a.v) + kvh * a.ldvh;
+    Stage<T, DP, NT> sk, sv;
+    uint64_t bits = 0, next = 0;
+    if (it.c0 < it.c1) {
+        const int64_t key0 = it.k_begin + static_cast<int64_t>(it.c0);
+        const int left = it.c1 - it.c0;
+        sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
+        sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
+        bits = key_bits(a, key0, left, lane);
+        sk.write(lds, bits);
+        sv.write(lds + TILE, bits);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int k0 = it.c0; k0 < it.c1; k0 += KT) {
+        const char* kt = lds + buf * 2 * TILE;
+        const char* vt = kt + TILE;
+        const bool more = k0 + KT < it.c1;
+        if (more) {
+            const int64_t key0 = it.k_begin + static_cast<int64_t>(k0 + KT);
+            const int left = it.c1 - k0 - KT;
+            sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
+            sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
+            next = key_bits(a, key0, left, lane);
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            f32x16 s[CB] = {}, dp[CB] = {};
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const vec8<T> fk = row_frag<T, DP>(kt, 32 * kb, i, col, half);
+                const vec8<T> fv = row_frag<T, DP>(vt, 32 * kb, i, col, half);
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) {
+                    s[cb] = mfma16(fk, qf[cb][i], s[cb]);
+                    dp[cb] = mfma16(fv, gf[cb][i], dp[cb]);
+                }
+            }
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[cb][r] = __builtin_amdgcn_exp2f(fmaf(s[cb][r], a.c, sc[cb].up - lse[cb])) *
+                               (dp[cb][r] - delta[cb]);
+            if (bits != ~0ull) {
+                const uint32_t mine = static_cast<uint32_t>(bits >> (32 * kb + 4 * half));
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!((mine >> acc_row(r)) & 1u)) {
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb) s[cb][r] = 0.f;
+                    }
+            }
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) sc[cb].fit(s[cb], acc[cb]);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                vec8<T> p[CB];
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) p[cb] = pack8<T>(s[cb], t);
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b) {
+                    const vec8<T> f = tr_frag<T, DP>(kt, trl, 32 * kb + 16 * t, b);
+#pragma unroll
+                    for (int cb = 0; cb < CB; ++cb) acc[cb][b] = mfma16(f, p[cb], acc[cb][b]);
+                }
+            }
+        }
+        if (more) {
+            char* dst = lds + (buf ^ 1) * 2 * TILE;
+            sk.write(dst, next);
+            sv.write(dst + TILE, next);
+        }
+        __syncthreads();
+        buf ^= 1;
+        bits = next;
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        if (row[cb] >= it.r1) continue;
+        const float f = a.scale * sc[cb].back();
+        if (it.slot >= 0)
+            store_acc16<float, DP>(a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
+                                             row[cb] - it.r0) * a.d, acc[cb], f, a.d, half);
+        else
+            store_acc16<T, DP>(static_cast<T*>(a.out) + at[cb] * a.d, acc[cb], f, a.d, half);
+    }
+}
+
+// One thread's share of a tile of 64 (query, head) rows
+template <typename T, int DP, int NT>
+struct RowStage {
+    static constexpr int C8 = DP / 8, N = KT * C8 / NT;
+    u32x4 v[N];
+    __device__ __forceinline__ void load(const T* base, int64_t ldt, int64_t ldh, int r0, int r1, int group,
+                                         int d) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = r0 + (threadIdx.x + j * NT) / C8, c = (threadIdx.x + j * NT) % C8 * 8;
+            v[j] = u32x4{};
+            if (r < r1 && c < d) {
+                const int t = r / group;
+                v[j] = *reinterpret_cast<const u32x4*>(base + t * ldt + (r - t * group) * ldh + c);
+            }
+        }
+    }
+    __device__ __forceinline__ void write(char* tile) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = threadIdx.x + j * NT;
+            *reinterpret_cast<u32x4*>(tile + i / C8 * pitch<DP>() + i % C8 * 16) = v[j];
+        }
+    }
+};
+
+template <typename T, int DP, int NW, int CB>
+__global__ __launch_bounds__(NW * 64) void cross_dkv16_kernel(CrossArgs a) {
+    constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
+    __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+    __shared__ __attribute__((aligned(16))) float st[2][2][KT];   // lse, delta
+    int item, kvh;
+    if (!cross_work(a, a.n_items, item, kvh)) return;
+    const CrossItem it = a.items[item];
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int trl = tr_lane<DP>(lane);
+    vec8<T> kf[CB][DP / 16], vf[CB][DP / 16];
+    int key[CB];
+    bool keep[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        key[cb] = it.r0 + (wave * CB + cb) * 32 + col;
+        const int64_t kt = it.k_begin + static_cast<int64_t>(key[cb]);
+        keep[cb] = key[cb] < it.r1 && (!a.mask || a.mask[kt]);
+        load_frag16<T, DP>(kf[cb], keep[cb] ? static_cast<const T*>(a.k) + kt * a.ldk + kvh * a.ldkh : nullptr,
+                           a.d, half);
+        load_frag16<T, DP>(vf[cb], keep[cb] ? static_cast<const T*>(a.v) + kt * a.ldv + kvh * a.ldvh : nullptr,
+                           a.d, half);
+    }
+    f32x16 dk[CB][DP / 32] = {}, dv[CB][DP / 32] = {};
+    DsScale<T> sc[CB];
+    float gain[CB];   // dS's power of two over P's
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) gain[cb] = __builtin_amdgcn_exp2f(sc[cb].up - PB_UP<T>);
+    const T* qbase = static_cast<const T*>(a.q) + it.q_begin * a.ldq + kvh * a.group * a.ldqh;
+    const T* gbase = static_cast<const T*>(a.dout) + it.q_begin * a.lddo + kvh * a.group * a.lddoh;
+    RowStage<T, DP, NT> sq, sg;
+    float stat = 0.f;
+    auto load = [&](int r0) {
+        sq.load(qbase, a.ldq, a.ldqh, r0, it.c1, a.group, a.d);
+        sg.load(gbase, a.lddo, a.lddoh, r0, it.c1, a.group, a.d);
+        if (threadIdx.x < 2 * KT) {   // rows past the end: lse = inf, P = 0
+            const int r = r0 + (threadIdx.x & (KT - 1)), t = r / a.group;
+            const bool is_lse = threadIdx.x < KT;
+            stat = is_lse ? INFINITY : 0.f;
+            if (r < it.c1)
+                stat = (is_lse ? a.lse : a.delta)[(it.q_begin + static_cast<int64_t>(t)) * a.heads +
+                                                  kvh * a.group + r - t * a.group] -
+                       (is_lse ? PB_UP<T> : 0.f);
+        }
+    };
+    auto write = [&](int buf) {
+        sq.write(lds + buf * 2 * TILE);
+        sg.write(lds + buf * 2 * TILE + TILE);
+        if (threadIdx.x < 2 * KT) st[buf][threadIdx.x / KT][threadIdx.x & (KT - 1)] = stat;
+    };
+    if (it.c0 < it.c1) {
+        load(it.c0);
+        write(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int r0 = it.c0; r0 < it.c1; r0 += KT) {
+        const char* qt = lds + buf * 2 * TILE;
+        const char* gt = qt + TILE;
+        const bool more = r0 + KT < it.c1;
+        if (more) load(r0 + KT);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            f32x16 s[CB] = {}, dp[CB] = {};
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const vec8<T> fq = row_frag<T, DP>(qt, 32 * rb, i, col, half);
+                const vec8<T> fg = row_frag<T, DP>(gt, 32 * rb, i, col, half);
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) {
+                    s[cb] = mfma16(fq, kf[cb][i], s[cb]);
+                    dp[cb] = mfma16(fg, vf[cb][i], dp[cb]);
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 x = ld4(&st[buf][0][32 * rb + 8 * g + 4 * half]);
+                const float4 y = ld4(&st[buf][1][32 * rb + 8 * g + 4 * half]);
+                const float lv[4] = {x.x, x.y, x.z, x.w}, ev[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * g + e;
+#pragma unroll
+                    for (int cb = 0; cb < CB; ++cb) {
+                        s[cb][r] = __builtin_amdgcn_exp2f(fmaf(s[cb][r], a.c, -lv[e]));
+                        dp[cb][r] = s[cb][r] * (dp[cb][r] - ev[e]);
+                        if constexpr (NARROW<T>) dp[cb][r] *= gain[cb];
+                    }
+                }
+            }
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+                if (sc[cb].fit(dp[cb], dk[cb])) gain[cb] = __builtin_amdgcn_exp2f(sc[cb].up - PB_UP<T>);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                vec8<T> p[CB], ds[CB];
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) {
+                    p[cb] = pack8<T>(s[cb], t);
+                    ds[cb] = pack8<T>(dp[cb], t);
+                }
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b) {
+                    const vec8<T> fg = tr_frag<T, DP>(gt, trl, 32 * rb + 16 * t, b);
+                    const vec8<T> fq = tr_frag<T, DP>(qt, trl, 32 * rb + 16 * t, b);
+#pragma unroll
+                    for (int cb = 0; cb < CB; ++cb) {
+                        dv[cb][b] = mfma16(fg, p[cb], dv[cb][b]);
+                        dk[cb][b] = mfma16(fq, ds[cb], dk[cb][b]);
+                    }
+                }
+            }
+        }
+        if (more) write(buf ^ 1);
+        __syncthreads();
+        buf ^= 1;
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        if (key[cb] >= it.r1) continue;
+        // a key that the mask leaves out has no gradient, whatever its rows hold
+        if (!keep[cb]) {
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b) dk[cb][b] = dv[cb][b] = f32x16{};
+        }
+        const float fk = a.scale * sc[cb].back(), fv = __builtin_amdgcn_exp2f(-PB_UP<T>);
+        if (it.slot >= 0) {
+            float* p = a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
+                                 key[cb] - it.r0) * (2 * a.d);
+            store_acc16<float, DP>(p, dk[cb], fk, a.d, half);
+            store_acc16<float, DP>(p + a.d, dv[cb], fv, a.d, half);
+        } else {
+            const int64_t at = ((it.k_begin + static_cast<int64_t>(key[cb])) * a.kv_heads + kvh) * a.d;
+            store_acc16<T, DP>(static_cast<T*>(a.dk) + at, dk[cb], fk, a.d, half);
+            store_acc16<T, DP>(static_cast<T*>(a.dv) + at, dv[cb], fv, a.d, half);
+        }
+    }
+}
+
+constexpr int NW = CROSS_TILE / 32;
+
+template <typename T, int DP>
+void launch16(const CrossArgs& a, int pass, hipStream_t st) {
+    const dim3 grid(cross_grid(a.n_items, a.kv_heads)), block(NW * 64);
+    if (pass == MIGNN_CROSS_FORWARD)
+        hipLaunchKernelGGL((cross_fwd16_kernel<T, DP, NW, 1>), grid, block, 0, st, a);
+    else if (pass == MIGNN_CROSS_DQ)
+        hipLaunchKernelGGL((cross_dq16_kernel<T, DP, NW, 1>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((cross_dkv16_kernel<T, DP, NW, 1>), grid, block, 0, st, a);
+}
+
+template <typename T>
+void launch16_d(const CrossArgs& a, int pass, hipStream_t st) {
+    if (a.d <= 32) launch16<T, 32>(a, pass, st);
+    else if (a.d <= 64) launch16<T, 64>(a, pass, st);
+    else if (a.d <= 96) launch16<T, 96>(a, pass, st);
+    else launch16<T, 128>(a, pass, st);
+}
+
+}  // namespace
+
+int cross_pass16(const CrossArgs& a, int pass, int dtype, hipStream_t st) {
+    if (dtype == MIGNN_ROW_BF16) launch16_d<bf16_t>(a, pass, st);
+    else launch16_d<f16_t>(a, pass, st);
+    return launch_status("cross attention kernel (16 bit)");
+}
+
+}  // namespace mignn

@@ -357,6 +357,28 @@ def test_cross_attention_is_deterministic_and_stream_safe(ql, kl, dt):
         assert torch.equal(torch.autograd.grad(out, t, do)[0], first[1 + i])
 
 
+@pytest.mark.parametrize("up", [2.0 ** -9, 1.0, 2.0 ** 9])
+@pytest.mark.parametrize("ql,kl", [([2], [5000]), ([130], [300]), ([900], [9])])
+def test_cross_attention_fp16_range(ql, kl, up):
+    """fp16 rows with output gradients and values far from 1: P and dS leave
+    fp16's range (dS up to 2^9 2^6 sqrt(d) and more, down to 2^-9 / 5000), the
+    gradients do not."""
+    dt, d = torch.float16, 64
+    q, k, v, _ = cross_inputs(ql, kl, 2, 1, d, dt, seed=3)
+    v = (v.float() * (8.0 if up > 1 else 1.0)).to(dt)
+    do = rnd(*q.shape, seed=8, dt=dt, scale=up)
+    # rows of very unlike gradients in one tile
+    do[::3] = do[::3] * 2.0 ** -7
+    plan = A.CrossPlan(ql, kl, heads=2, kv_heads=1, head_dim=d, dtype=dt)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(A.cross_attention(*leaves, plan, scale=0.03), leaves, do)
+    ref = orc.cross_attention(q, k, v, ql, kl, None, 0.03, do)
+    assert max(ref[n].abs().max().item() for n in ("dq", "dk", "dv")) < 65504
+    bound = cross_bounds(ref, dt, d, kl, ql, 2)
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        close(g, ref[name], bound[name], dt, name)
+
+
 def test_cross_attention_nan_in_a_query_stays_in_its_row():
     ql, kl = [100], [300]
     q, k, v, _ = cross_inputs(ql, kl, 2, 2, 32, torch.float32)
