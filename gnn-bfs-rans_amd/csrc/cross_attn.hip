@@ -191,38 +191,58 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd_kernel(CrossArgs a) {
     if (a.lse && half == 0) a.lse[at] = l == 0.f ? INFINITY : m2 + log2f(l);
 }
 
-// Joins the parts of split rows: one wave a row.
-template <typename T>
-__global__ __launch_bounds__(256) void cross_join_fwd_kernel(CrossArgs a, int tile_rows) {
+// Joins the parts of split rows onto their largest maximum.  WPR waves a row
+// share its parts (1 where parts are few, 4 where a row has many).
+template <typename T, int WPR>
+__global__ __launch_bounds__(256) void cross_join_fwd_kernel(CrossArgs a) {
     const CrossJoin jn = a.joins[blockIdx.x];
-    const int kvh = blockIdx.y, lane = threadIdx.x & 63;
-    for (int r = threadIdx.x >> 6; r < jn.r1 - jn.r0; r += 4) {
-        const int row = jn.r0 + r, t = row / a.group;
-        const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group +
-                           (row - t * a.group);
-        float m = -INFINITY;
-        for (int p = 0; p < jn.parts; ++p)
-            m = fmaxf(m, part_row(a, jn.slot + p, kvh, r, tile_rows, a.d + 2)[a.d]);
-        const float base = m == -INFINITY ? 0.f : m;
-        float l = 0.f, o[2] = {0.f, 0.f};
-        for (int p = 0; p < jn.parts; ++p) {
-            const float* src = part_row(a, jn.slot + p, kvh, r, tile_rows, a.d + 2);
-            const float f = __builtin_amdgcn_exp2f(src[a.d] - base);
-            l = fmaf(src[a.d + 1], f, l);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (lane + 64 * i < a.d) o[i] = fmaf(src[lane + 64 * i], f, o[i]);
+    const int kvh = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = blockIdx.z * (4 / WPR) + wave / WPR;
+    const bool live = r < jn.r1 - jn.r0;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.tile * (a.d + 2);   // part to part
+    const float* src = part_row(a, jn.slot, kvh, live ? r : 0, a.tile, a.d + 2);
+    float m = -INFINITY;
+    for (int p = lane; p < jn.parts; p += 64) m = fmaxf(m, src[p * step + a.d]);
+    for (int b = 1; b < 64; b <<= 1) m = fmaxf(m, __shfl_xor(m, b));
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[2] = {0.f, 0.f};
+    const bool two = lane + 64 < a.d, one = lane < a.d;
+    for (int p0 = 0; p0 < jn.parts; p0 += 64) {
+        float f = 0.f;
+        if (p0 + lane < jn.parts) {
+            f = __builtin_amdgcn_exp2f(src[(p0 + lane) * step + a.d] - base);
+            l = fmaf(src[(p0 + lane) * step + a.d + 1], f, l);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int c = lane + 64 * i;
-            if (c >= a.d) continue;
-            static_cast<T*>(a.out)[at * a.d + c] = static_cast<T>(o[i] * inv);
-            if (a.o32) a.o32[at * a.d + c] = o[i] * inv;
+        const int n = jn.parts - p0 < 64 ? jn.parts - p0 : 64;
+#pragma unroll 4
+        for (int p = wave % WPR; p < n; p += WPR) {
+            const float fp = __shfl(f, p);
+            const float* row = src + (p0 + p) * step + lane;
+            if (one) o[0] = fmaf(row[0], fp, o[0]);
+            if (two) o[1] = fmaf(row[64], fp, o[1]);
         }
-        if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : base + log2f(l);
     }
+    for (int b = 1; b < 64; b <<= 1) l += __shfl_xor(l, b);
+    if constexpr (WPR > 1) {
+        __shared__ float os[4][128];
+        os[wave][lane] = o[0], os[wave][lane + 64] = o[1];
+        __syncthreads();
+        if (wave % WPR) return;
+#pragma unroll
+        for (int w = 1; w < WPR; ++w) o[0] += os[wave + w][lane], o[1] += os[wave + w][lane + 64];
+    }
+    if (!live) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int row = jn.r0 + r, t = row / a.group;
+    const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group + (row - t * a.group);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = lane + 64 * i;
+        if (c >= a.d) continue;
+        static_cast<T*>(a.out)[at * a.d + c] = static_cast<T>(o[i] * inv);
+        if (a.o32) a.o32[at * a.d + c] = o[i] * inv;
+    }
+    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : base + log2f(l);
 }
 
 template <typename T, int DP, int NW>
@@ -360,29 +380,31 @@ __global__ __launch_bounds__(NW * 64) void cross_dkv_kernel(CrossArgs a) {
     }
 }
 
-// Sums the parts of split gradients in slot order: `width` floats a row, one
-// wave a row; dq (dkv = false) or dk | dv.
+// Sums the parts of split gradients in slot order, one wave a row: dq, or dk
+// and dv side by side.
 template <typename T>
-__global__ __launch_bounds__(256) void cross_join_grad_kernel(CrossArgs a, int tile_rows, bool dkv) {
+__global__ __launch_bounds__(256) void cross_join_grad_kernel(CrossArgs a, bool dkv) {
     const CrossJoin jn = a.joins[blockIdx.x];
     const int kvh = blockIdx.y, lane = threadIdx.x & 63;
     const int width = dkv ? 2 * a.d : a.d;
-    for (int r = threadIdx.x >> 6; r < jn.r1 - jn.r0; r += 4) {
-        const int row = jn.r0 + r;
-        for (int c = lane; c < width; c += 64) {
-            float v = 0.f;
-            for (int p = 0; p < jn.parts; ++p)
-                v += part_row(a, jn.slot + p, kvh, r, tile_rows, width)[c];
-            if (dkv) {
-                const int64_t at = ((jn.begin + static_cast<int64_t>(row)) * a.kv_heads + kvh) * a.d;
-                T* dst = static_cast<T*>(c < a.d ? a.dk : a.dv);
-                dst[at + (c < a.d ? c : c - a.d)] = static_cast<T>(v);
-            } else {
-                const int t = row / a.group;
-                const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group +
-                                   (row - t * a.group);
-                static_cast<T*>(a.out)[at * a.d + c] = static_cast<T>(v);
-            }
+    const int r = blockIdx.z * 4 + (threadIdx.x >> 6);
+    if (r >= jn.r1 - jn.r0) return;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.tile * width;
+    const float* src = part_row(a, jn.slot, kvh, r, a.tile, width);
+    const int row = jn.r0 + r;
+    for (int c = lane; c < width; c += 64) {
+        float v = 0.f;
+#pragma unroll 8
+        for (int p = 0; p < jn.parts; ++p) v += src[p * step + c];
+        if (dkv) {
+            const int64_t at = ((jn.begin + static_cast<int64_t>(row)) * a.kv_heads + kvh) * a.d;
+            T* dst = static_cast<T*>(c < a.d ? a.dk : a.dv);
+            dst[at + (c < a.d ? c : c - a.d)] = static_cast<T>(v);
+        } else {
+            const int t = row / a.group;
+            const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group +
+                               (row - t * a.group);
+            static_cast<T*>(a.out)[at * a.d + c] = static_cast<T>(v);
         }
     }
 }
@@ -390,42 +412,58 @@ __global__ __launch_bounds__(256) void cross_join_grad_kernel(CrossArgs a, int t
 // ---------------------------------------------------------------------------
 // Plan
 
-constexpr int CROSS_WAVES = CROSS_TILE / CROSS_ROWS;
-
-// Tiles of the "r" side (rows or keys) times chunks of the "c" side.  The
-// chunk is chosen so that the pass has about two workgroups for each of the
-// 256 CUs when the tiles alone are fewer; it stays a multiple of 32 and not
-// under 256, where a part's join would cost what the split gains.
+// Tiles of the "r" side (rows or keys) times chunks of the "c" side.
+struct PassShape {
+    int tile;        // rows of a tile
+    int64_t longest; // of the r side
+    int64_t chunk;
+};
 struct PassPlan {
     int64_t items = 0, joins = 0, slots = 0;
 };
 
-int64_t pass_chunk(const int64_t* rows, const int64_t* keys, int64_t batch, bool dkv, int heads) {
+// Tile: 8 rows where no sequence has more (forward: cross_few), 32 where none
+// has more than 32 (one wave: more workgroups, and three waves of four would
+// idle), else 128.
+// Chunk: the pass should have `target` workgroups (two for each of the 256
+// CUs, eight small ones) when its tiles alone are fewer; not under `least`,
+// where the parts' join would cost what the split gains.
+PassShape pass_shape(const int64_t* rows, const int64_t* keys, int64_t batch, int pass, int kv_heads,
+                     int dtype) {
+    const bool dkv = pass == MIGNN_CROSS_DKV;
+    PassShape s{128, 0, 0};
+    for (int64_t b = 0; b < batch; ++b) {
+        const int64_t r = dkv ? keys[b] : rows[b];
+        if (r > s.longest) s.longest = r;
+    }
+    if (pass == MIGNN_CROSS_FORWARD && s.longest <= CROSS_FEW) s.tile = CROSS_FEW;
+    else if (s.longest <= CROSS_ROWS) s.tile = CROSS_ROWS;
     double work = 0.0;
     for (int64_t b = 0; b < batch; ++b) {
         const int64_t r = dkv ? keys[b] : rows[b], c = dkv ? rows[b] : keys[b];
-        work += static_cast<double>((r + CROSS_TILE - 1) / CROSS_TILE) * static_cast<double>(c);
+        work += static_cast<double>((r + s.tile - 1) / s.tile) * static_cast<double>(c);
     }
-    const double share = work * heads / 512.0;
-    int64_t chunk = static_cast<int64_t>(share);
-    if (chunk < 256) chunk = 256;
-    return (chunk + 31) / 32 * 32;
+    const int64_t target = s.tile == 128 ? 512 : 2048, least = s.tile == 128 ? 256 : 128;
+    s.chunk = static_cast<int64_t>(work * kv_heads / static_cast<double>(target));
+    if (s.chunk < least) s.chunk = least;
+    s.chunk = (s.chunk + 63) / 64 * 64;
+    return s;
 }
 
-PassPlan plan_pass(const int64_t* rows, const int64_t* queries, const int64_t* keys, int64_t batch,
-                   bool dkv, int heads, CrossItem* items, CrossJoin* joins) {
-    const int64_t chunk = pass_chunk(rows, keys, batch, dkv, heads);
+PassPlan plan_pass(const PassShape& shape, const int64_t* rows, const int64_t* queries, const int64_t* keys,
+                   int64_t batch, bool dkv, CrossItem* items, CrossJoin* joins) {
+    const int64_t chunk = shape.chunk, tile = shape.tile;
     PassPlan p;
     int64_t qb = 0, kb = 0;
     for (int64_t b = 0; b < batch; ++b) {
         const int64_t rn = dkv ? keys[b] : rows[b], cn = dkv ? rows[b] : keys[b];
         int64_t parts = (cn + chunk - 1) / chunk;
         if (parts < 1) parts = 1;
-        // equal parts, each a multiple of 32 but the last
-        const int64_t len = cn == 0 ? 0 : ((cn + parts - 1) / parts + 31) / 32 * 32;
+        // equal parts, each a multiple of 64 but the last
+        const int64_t len = cn == 0 ? 0 : ((cn + parts - 1) / parts + 63) / 64 * 64;
         if (len > 0) parts = (cn + len - 1) / len;
-        for (int64_t r0 = 0; r0 < rn; r0 += CROSS_TILE) {
-            const int64_t r1 = r0 + CROSS_TILE < rn ? r0 + CROSS_TILE : rn;
+        for (int64_t r0 = 0; r0 < rn; r0 += tile) {
+            const int64_t r1 = r0 + tile < rn ? r0 + tile : rn;
             if (joins && parts > 1)
                 joins[p.joins] = {static_cast<int32_t>(dkv ? kb : qb), static_cast<int32_t>(r0),
                                   static_cast<int32_t>(r1), static_cast<int32_t>(p.slots),
@@ -455,41 +493,53 @@ int64_t part_width(int pass, int d) {
     return pass == MIGNN_CROSS_FORWARD ? d + 2 : pass == MIGNN_CROSS_DQ ? d : 2 * d;
 }
 
-template <typename K>
-void launch_cross(K kernel, const CrossArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(kernel, dim3(cross_grid(a.n_items, a.kv_heads)), dim3(CROSS_WAVES * 64), 0,
-                       st, a);
+template <int DP, int NW>
+void launch_exact(const CrossArgs& a, int pass, hipStream_t st) {
+    const dim3 grid(cross_grid(a.n_items, a.kv_heads)), block(NW * 64);
+    if (pass == MIGNN_CROSS_FORWARD)
+        hipLaunchKernelGGL((cross_fwd_kernel<float, DP, NW>), grid, block, 0, st, a);
+    else if (pass == MIGNN_CROSS_DQ)
+        hipLaunchKernelGGL((cross_dq_kernel<float, DP, NW>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((cross_dkv_kernel<float, DP, NW>), grid, block, 0, st, a);
 }
 
 template <int DP>
-void launch_exact(const CrossArgs& a, int pass, hipStream_t st) {
-    if (pass == MIGNN_CROSS_FORWARD) launch_cross(cross_fwd_kernel<float, DP, CROSS_WAVES>, a, st);
-    else if (pass == MIGNN_CROSS_DQ) launch_cross(cross_dq_kernel<float, DP, CROSS_WAVES>, a, st);
-    else launch_cross(cross_dkv_kernel<float, DP, CROSS_WAVES>, a, st);
+void launch_exact_d(const CrossArgs& a, int pass, hipStream_t st) {
+    if (a.tile == CROSS_ROWS) launch_exact<DP, 1>(a, pass, st);
+    else launch_exact<DP, 4>(a, pass, st);
 }
 
 int cross_pass_exact(const CrossArgs& a, int pass, hipStream_t st) {
-    if (a.d <= 32) launch_exact<32>(a, pass, st);
-    else if (a.d <= 64) launch_exact<64>(a, pass, st);
-    else if (a.d <= 96) launch_exact<96>(a, pass, st);
-    else launch_exact<128>(a, pass, st);
+    if (a.d <= 32) launch_exact_d<32>(a, pass, st);
+    else if (a.d <= 64) launch_exact_d<64>(a, pass, st);
+    else if (a.d <= 96) launch_exact_d<96>(a, pass, st);
+    else launch_exact_d<128>(a, pass, st);
     return launch_status("cross attention kernel");
 }
 
 template <typename T>
 void launch_join(const CrossArgs& a, int pass, hipStream_t st) {
-    const dim3 grid(a.n_joins, a.kv_heads);
-    if (pass == MIGNN_CROSS_FORWARD)
-        hipLaunchKernelGGL(cross_join_fwd_kernel<T>, grid, dim3(256), 0, st, a, CROSS_TILE);
-    else
-        hipLaunchKernelGGL(cross_join_grad_kernel<T>, grid, dim3(256), 0, st, a, CROSS_TILE,
-                           pass == MIGNN_CROSS_DKV);
+    const unsigned rows = a.rows < a.tile ? a.rows : a.tile;
+    const dim3 grid(a.n_joins, a.kv_heads, (rows + 3) / 4);
+    if (pass != MIGNN_CROSS_FORWARD)
+        hipLaunchKernelGGL(cross_join_grad_kernel<T>, grid, dim3(256), 0, st, a, pass == MIGNN_CROSS_DKV);
+    else if (a.tile == 128)
+        hipLaunchKernelGGL((cross_join_fwd_kernel<T, 1>), grid, dim3(256), 0, st, a);
+    else   // few rows in many parts
+        hipLaunchKernelGGL((cross_join_fwd_kernel<T, 4>), dim3(a.n_joins, a.kv_heads, rows), dim3(256), 0,
+                           st, a);
 }
 
-int run_pass(const CrossArgs& a, int pass, int dtype, hipStream_t st) {
+int run_pass(CrossArgs a, const mignn_cross_pass& ps, int pass, int dtype, hipStream_t st) {
+    a.items = static_cast<const CrossItem*>(ps.items);
+    a.joins = static_cast<const CrossJoin*>(ps.joins);
+    a.n_items = ps.n_items, a.n_joins = ps.n_joins, a.tile = ps.tile, a.rows = ps.rows;
     if (a.n_items > 0) {
-        const int rc = dtype == MIGNN_ROW_F32 ? cross_pass_exact(a, pass, st)
-                                              : cross_pass16(a, pass, dtype, st);
+        int rc;
+        if (a.tile == CROSS_FEW) rc = cross_few(a, dtype, st);
+        else if (dtype == MIGNN_ROW_F32) rc = cross_pass_exact(a, pass, st);
+        else rc = cross_pass16(a, pass, dtype, st);
         if (rc) return rc;
     }
     if (a.n_joins == 0) return MIGNN_OK;
@@ -538,7 +588,7 @@ extern "C" int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, in
     for (int64_t b = 0; b < batch; ++b) {
         MIGNN_REQUIRE(q_lens[b] >= 0 && k_lens[b] >= 0, "cross_plan: negative length in sequence %lld",
                       static_cast<long long>(b));
-        MIGNN_REQUIRE(q_lens[b] <= INT32_MAX / group - CROSS_TILE && k_lens[b] <= INT32_MAX - CROSS_TILE,
+        MIGNN_REQUIRE(q_lens[b] <= INT32_MAX / group - 1024 && k_lens[b] <= INT32_MAX - 1024,
                       "cross_plan: sequence %lld too long", static_cast<long long>(b));
         queries += q_lens[b];
         keys += k_lens[b];
@@ -547,16 +597,19 @@ extern "C" int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, in
     int64_t* rows = static_cast<int64_t*>(malloc(sizeof(int64_t) * (batch > 0 ? batch : 1)));
     MIGNN_REQUIRE(rows, "cross_plan: out of host memory");
     for (int64_t b = 0; b < batch; ++b) rows[b] = q_lens[b] * group;
-    const PassPlan p = plan_pass(rows, q_lens, k_lens, batch, pass == MIGNN_CROSS_DKV, kv_heads,
+    const PassShape sh = pass_shape(rows, k_lens, batch, pass, kv_heads, dtype);
+    const PassPlan p = plan_pass(sh, rows, q_lens, k_lens, batch, pass == MIGNN_CROSS_DKV,
                                  static_cast<CrossItem*>(items), static_cast<CrossJoin*>(joins));
     free(rows);
     MIGNN_REQUIRE(p.items * kv_heads <= INT32_MAX / 2 && p.joins <= INT32_MAX,
                   "cross_plan: too many tiles");
     info[0] = p.items;
     info[1] = p.joins;
-    info[2] = p.slots * kv_heads * CROSS_TILE * part_width(pass, d) * static_cast<int64_t>(sizeof(float));
+    info[2] = p.slots * kv_heads * sh.tile * part_width(pass, d) * static_cast<int64_t>(sizeof(float));
     info[3] = queries;
     info[4] = keys;
+    info[5] = sh.tile;
+    info[6] = sh.longest;
     return MIGNN_OK;
 }
 
@@ -583,13 +636,10 @@ extern "C" int mignn_cross_attn_forward(const mignn_cross_call* c, void* out, fl
     CrossArgs a{};
     a.q = c->q, a.k = c->k, a.v = c->v, a.mask = c->key_mask;
     a.out = out, a.o32 = out32, a.lse = lse, a.part = static_cast<float*>(c->scratch);
-    a.items = static_cast<const CrossItem*>(ps.items);
-    a.joins = static_cast<const CrossJoin*>(ps.joins);
     a.ldq = c->ldq, a.ldqh = c->ldqh, a.ldk = c->ldk, a.ldkh = c->ldkh, a.ldv = c->ldv, a.ldvh = c->ldvh;
-    a.n_items = ps.n_items, a.n_joins = ps.n_joins;
     a.heads = c->heads, a.kv_heads = c->kv_heads, a.group = c->heads / c->kv_heads, a.d = c->d;
     a.scale = c->scale, a.c = c->scale * LOG2E;
-    return run_pass(a, MIGNN_CROSS_FORWARD, c->dtype, as_stream(stream));
+    return run_pass(a, ps, MIGNN_CROSS_FORWARD, c->dtype, as_stream(stream));
 }
 
 extern "C" int mignn_cross_attn_backward(const mignn_cross_call* c, const void* dout, int64_t lddo,
@@ -628,11 +678,7 @@ extern "C" int mignn_cross_attn_backward(const mignn_cross_call* c, const void* 
     a.scale = c->scale, a.c = c->scale * LOG2E;
     for (int pass : {MIGNN_CROSS_DQ, MIGNN_CROSS_DKV}) {   // dq first: it writes delta
         if (pass == MIGNN_CROSS_DKV && !keys) break;
-        const mignn_cross_pass& ps = c->pass[pass];
-        a.items = static_cast<const CrossItem*>(ps.items);
-        a.joins = static_cast<const CrossJoin*>(ps.joins);
-        a.n_items = ps.n_items, a.n_joins = ps.n_joins;
-        if (int rc = run_pass(a, pass, c->dtype, as_stream(stream))) return rc;
+        if (int rc = run_pass(a, c->pass[pass], pass, c->dtype, as_stream(stream))) return rc;
     }
     return MIGNN_OK;
 }

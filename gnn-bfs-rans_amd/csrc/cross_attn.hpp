@@ -1,5 +1,6 @@
 // Shared by the cross-attention sources (cross_attn.hip: plan, exact fp32
-// kernels, joins; cross_attn16.hip: 16-bit kernels).
+// kernels, joins; cross_attn16.hip: 16-bit kernels;
+// cross_decode.hip: few rows).
 #pragma once
 
 #include "row_types.hpp"
@@ -9,7 +10,7 @@ namespace mignn {
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 
 constexpr int CROSS_ROWS = 32;    // rows (or keys) a wave owns: one MFMA tile edge
-constexpr int CROSS_TILE = 4 * CROSS_ROWS;   // of a workgroup
+constexpr int CROSS_FEW = 8;      // rows that cross_few takes
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // One workgroup's share of a pass, per kv head.  "Rows" are the (query, head
@@ -45,6 +46,7 @@ struct CrossArgs {
     const CrossJoin* joins;
     int64_t ldq, ldqh, ldk, ldkh, ldv, ldvh, lddo, lddoh;
     int32_t n_items, n_joins, heads, kv_heads, group, d;
+    int32_t tile, rows;          // of the pass: rows (keys) of a tile, of the longest sequence
     float scale, c;              // c = scale log2(e)
 };
 
@@ -77,5 +79,7 @@ __device__ __forceinline__ float4 load4(const T* p) {
 
 // the 16-bit rows' kernels of a pass (cross_attn16.hip)
 int cross_pass16(const CrossArgs& a, int pass, int dtype, hipStream_t st);
+// the forward of up to CROSS_FEW rows a sequence (cross_decode.hip)
+int cross_few(const CrossArgs& a, int dtype, hipStream_t st);
 
 }  // namespace mignn

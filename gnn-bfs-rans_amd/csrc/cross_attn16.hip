@@ -518,24 +518,24 @@ __global__ __launch_bounds__(NW * 64) void cross_dkv16_kernel(CrossArgs a) {
     const T* qbase = static_cast<const T*>(a.q) + it.q_begin * a.ldq + kvh * a.group * a.ldqh;
     const T* gbase = static_cast<const T*>(a.dout) + it.q_begin * a.lddo + kvh * a.group * a.lddoh;
     RowStage<T, DP, NT> sq, sg;
-    float stat = 0.f;
+    float lse = INFINITY, delta = 0.f;
     auto load = [&](int r0) {
         sq.load(qbase, a.ldq, a.ldqh, r0, it.c1, a.group, a.d);
         sg.load(gbase, a.lddo, a.lddoh, r0, it.c1, a.group, a.d);
-        if (threadIdx.x < 2 * KT) {   // rows past the end: lse = inf, P = 0
-            const int r = r0 + (threadIdx.x & (KT - 1)), t = r / a.group;
-            const bool is_lse = threadIdx.x < KT;
-            stat = is_lse ? INFINITY : 0.f;
-            if (r < it.c1)
-                stat = (is_lse ? a.lse : a.delta)[(it.q_begin + static_cast<int64_t>(t)) * a.heads +
-                                                  kvh * a.group + r - t * a.group] -
-                       (is_lse ? PB_UP<T> : 0.f);
+        if (threadIdx.x < KT) {   // rows past the end: lse = inf, P = 0
+            const int r = r0 + threadIdx.x, t = r / a.group;
+            lse = INFINITY, delta = 0.f;
+            if (r < it.c1) {
+                const int64_t at = (it.q_begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group + r - t * a.group;
+                lse = a.lse[at] - PB_UP<T>;
+                delta = a.delta[at];
+            }
         }
     };
     auto write = [&](int buf) {
         sq.write(lds + buf * 2 * TILE);
         sg.write(lds + buf * 2 * TILE + TILE);
-        if (threadIdx.x < 2 * KT) st[buf][threadIdx.x / KT][threadIdx.x & (KT - 1)] = stat;
+        if (threadIdx.x < KT) st[buf][0][threadIdx.x] = lse, st[buf][1][threadIdx.x] = delta;
     };
     if (it.c0 < it.c1) {
         load(it.c0);
@@ -626,17 +626,21 @@ __global__ __launch_bounds__(NW * 64) void cross_dkv16_kernel(CrossArgs a) {
     }
 }
 
-constexpr int NW = CROSS_TILE / 32;
+template <typename T, int DP, int NW, int CB>
+void launch16_tile(const CrossArgs& a, int pass, hipStream_t st) {
+    const dim3 grid(cross_grid(a.n_items, a.kv_heads)), block(NW * 64);
+    if (pass == MIGNN_CROSS_FORWARD)
+        hipLaunchKernelGGL((cross_fwd16_kernel<T, DP, NW, CB>), grid, block, 0, st, a);
+    else if (pass == MIGNN_CROSS_DQ)
+        hipLaunchKernelGGL((cross_dq16_kernel<T, DP, NW, CB>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((cross_dkv16_kernel<T, DP, NW, CB>), grid, block, 0, st, a);
+}
 
 template <typename T, int DP>
 void launch16(const CrossArgs& a, int pass, hipStream_t st) {
-    const dim3 grid(cross_grid(a.n_items, a.kv_heads)), block(NW * 64);
-    if (pass == MIGNN_CROSS_FORWARD)
-        hipLaunchKernelGGL((cross_fwd16_kernel<T, DP, NW, 1>), grid, block, 0, st, a);
-    else if (pass == MIGNN_CROSS_DQ)
-        hipLaunchKernelGGL((cross_dq16_kernel<T, DP, NW, 1>), grid, block, 0, st, a);
-    else
-        hipLaunchKernelGGL((cross_dkv16_kernel<T, DP, NW, 1>), grid, block, 0, st, a);
+    if (a.tile == CROSS_ROWS) launch16_tile<T, DP, 1, 1>(a, pass, st);
+    else launch16_tile<T, DP, 4, 1>(a, pass, st);
 }
 
 template <typename T>

@@ -1,0 +1,182 @@
+// Cross attention of few rows (probe points): up to CROSS_FEW rows of one
+// sequence and kv head -- queries times heads of the group -- against all its
+// keys (formulas: cross_attn.hip).
+//
+// Bound by memory: K and V are read once, for all rows, and nothing is
+// computed twice.  A key's row is spread over LPK lanes, 16 bytes each, so a
+// wave reads 64 / LPK keys at a time, UNROLL of them in flight; the scores
+// are butterflies over the LPK lanes, and every group of lanes keeps a running
+// maximum, sum and output of its own keys in registers.  No LDS until the end,
+// where the groups and then the block's waves are joined.  The matrix
+// instructions would spend 32 columns on these rows, and the staging of tiles
+// costs more than the arithmetic: fp32 here for every type.
+#include "cross_attn.hpp"
+
+namespace mignn {
+namespace {
+
+constexpr int WAVES = 4;
+constexpr int UNROLL = 4;
+
+// R rows (a power of two that holds the sequence's); LPK lanes a key, V elements each
+template <typename T, int R, int LPK>
+__global__ __launch_bounds__(WAVES * 64) void cross_few_kernel(CrossArgs a) {
+    constexpr int V = 16 / sizeof(T), KPW = 64 / LPK;
+    int item, kvh;
+    if (!cross_work(a, a.n_items, item, kvh)) return;
+    const CrossItem it = a.items[item];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, grp = lane / LPK;
+    const int c0 = sub * V;
+    const bool in = c0 < a.d;
+    const int rows = it.r1 - it.r0;
+    float q[R][V], o[R][V], m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) q[r][i] = o[r][i] = 0.f;
+        if (r < rows && in) {
+            const int row = it.r0 + r, t = row / a.group;
+            load_row(static_cast<const T*>(a.q) + (it.q_begin + static_cast<int64_t>(t)) * a.ldq +
+                         (kvh * a.group + row - t * a.group) * a.ldqh + c0, q[r]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) q[r][i] *= a.c;
+        }
+    }
+    const T* kb = static_cast<const T*>(a.k) + kvh * a.ldkh + c0;
+    const T* vb = static_cast<const T*>(a.v) + kvh * a.ldvh + c0;
+    for (int k0 = it.c0 + wave * KPW * UNROLL; k0 < it.c1; k0 += WAVES * KPW * UNROLL) {
+        float kf[UNROLL][V], vf[UNROLL][V];
+        bool ok[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int k = k0 + u * KPW + grp;
+            const int64_t key = it.k_begin + static_cast<int64_t>(k < it.c1 ? k : it.c1 - 1);
+            ok[u] = k < it.c1 && (!a.mask || a.mask[key]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) kf[u][i] = vf[u][i] = 0.f;
+            if (in) {
+                load_row(kb + key * a.ldk, kf[u]);
+                load_row(vb + key * a.ldv, vf[u]);
+            }
+        }
+        float s[R][UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float x = 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) x = fmaf(q[r][i], kf[u][i], x);
+#pragma unroll
+                for (int b = 1; b < LPK; b <<= 1) x += __shfl_xor(x, b);
+                s[r][u] = ok[u] ? x : -INFINITY;
+            }
+        // what the mask leaves out may hold anything, and 0 inf is no 0
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            if (!ok[u]) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) vf[u][i] = 0.f;
+            }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float mn = m[r];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) mn = fmaxf(mn, s[r][u]);
+            const float base = mn == -INFINITY ? 0.f : mn;
+            const float f = __builtin_amdgcn_exp2f(m[r] - base);
+            m[r] = mn;
+            l[r] *= f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[r][i] *= f;
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const float p = __builtin_amdgcn_exp2f(s[r][u] - base);
+                l[r] += p;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[r][i] = fmaf(p, vf[u][i], o[r][i]);
+            }
+        }
+    }
+    // the wave's groups, then the block's waves: each joined onto the largest maximum
+    __shared__ float st[WAVES][R][2];
+    __shared__ float os[WAVES][R][LPK * V];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float mx = m[r];
+#pragma unroll
+        for (int b = LPK; b < 64; b <<= 1) mx = fmaxf(mx, __shfl_xor(mx, b));
+        const float f = __builtin_amdgcn_exp2f(m[r] - (mx == -INFINITY ? 0.f : mx));
+        l[r] *= f;
+#pragma unroll
+        for (int b = LPK; b < 64; b <<= 1) l[r] += __shfl_xor(l[r], b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            o[r][i] *= f;
+#pragma unroll
+            for (int b = LPK; b < 64; b <<= 1) o[r][i] += __shfl_xor(o[r][i], b);
+            if (grp == 0) os[wave][r][c0 + i] = o[r][i];
+        }
+        if (lane == 0) st[wave][r][0] = mx, st[wave][r][1] = l[r];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * a.d; i += WAVES * 64) {
+        const int r = i / a.d, c = i - r * a.d;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) mx = fmaxf(mx, st[w][r][0]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f, v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float f = __builtin_amdgcn_exp2f(st[w][r][0] - base);
+            sum = fmaf(st[w][r][1], f, sum);
+            v = fmaf(os[w][r][c], f, v);
+        }
+        if (it.slot >= 0) {
+            float* p = a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * CROSS_FEW + r) * (a.d + 2);
+            p[c] = v;
+            if (c == 0) p[a.d] = mx, p[a.d + 1] = sum;
+            continue;
+        }
+        const int row = it.r0 + r, t = row / a.group;
+        const int64_t at = (it.q_begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group + row - t * a.group;
+        const float out = sum == 0.f ? 0.f : v / sum;
+        static_cast<T*>(a.out)[at * a.d + c] = static_cast<T>(out);
+        if (a.o32) a.o32[at * a.d + c] = out;
+        if (a.lse && c == 0) a.lse[at] = sum == 0.f ? INFINITY : base + log2f(sum);
+    }
+}
+
+template <typename T, int R>
+void launch_few(const CrossArgs& a, hipStream_t st) {
+    const dim3 grid(cross_grid(a.n_items, a.kv_heads)), block(WAVES * 64);
+    const int lanes = a.d / (16 / static_cast<int>(sizeof(T)));
+#define MIGNN_FEW(L) hipLaunchKernelGGL((cross_few_kernel<T, R, L>), grid, block, 0, st, a)
+    if (lanes <= 4) MIGNN_FEW(4);
+    else if (lanes <= 8) MIGNN_FEW(8);
+    else if (lanes <= 16) MIGNN_FEW(16);
+    else if constexpr (sizeof(T) == 4) MIGNN_FEW(32);
+#undef MIGNN_FEW
+}
+
+template <typename T>
+void launch_few_t(const CrossArgs& a, hipStream_t st) {
+    const int rows = a.rows;
+    if (rows <= 1) launch_few<T, 1>(a, st);
+    else if (rows <= 2) launch_few<T, 2>(a, st);
+    else if (rows <= 4) launch_few<T, 4>(a, st);
+    else launch_few<T, CROSS_FEW>(a, st);
+}
+
+}  // namespace
+
+int cross_few(const CrossArgs& a, int dtype, hipStream_t st) {
+    if (dtype == MIGNN_ROW_F32) launch_few_t<float>(a, st);
+    else if (dtype == MIGNN_ROW_BF16) launch_few_t<bf16_t>(a, st);
+    else launch_few_t<f16_t>(a, st);
+    return launch_status("cross_few_kernel");
+}
+
+}  // namespace mignn

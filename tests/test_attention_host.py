@@ -196,10 +196,10 @@ def test_c_entry_points_check_arguments():
 
 def test_call_struct_layout_matches_header():
     """The ctypes mirror of mignn_cross_call has the C layout (x86-64)."""
-    assert ctypes.sizeof(_lib.CrossPass) == 32
+    assert ctypes.sizeof(_lib.CrossPass) == 40
     assert _lib.CrossCall.ldq.offset == 32 and _lib.CrossCall.n_keys.offset == 80
     assert _lib.CrossCall.scale.offset == 104 and _lib.CrossCall.scratch.offset == 112
-    assert ctypes.sizeof(_lib.CrossCall) == 128 + 3 * 32
+    assert ctypes.sizeof(_lib.CrossCall) == 128 + 3 * 40
 
 
 def test_oracle_gradients_match_differences():
