@@ -119,11 +119,21 @@ struct Stage {
     }
 };
 
-// Which of the 64 keys from k0 on take part (bit = key), for every lane
-__device__ __forceinline__ uint64_t key_bits(const CrossArgs& a, int64_t key0, int left, int lane) {
-    const bool ok = lane < left && (!a.mask || a.mask[key0 + lane]);
-    return __builtin_amdgcn_ballot_w64(ok);
-}
+// Which of the 64 keys from key0 on take part (bit = key), for every lane: the
+// mask's byte is loaded ahead of the rows it goes with and looked at when they
+// are (a comparison at the load would wait for every load before it)
+struct KeyBits {
+    uint32_t byte;
+    int left;
+    __device__ __forceinline__ void load(const CrossArgs& a, int64_t key0, int n, int lane) {
+        left = n;
+        byte = 1u;
+        if (a.mask) byte = a.mask[key0 + (lane < n ? lane : n - 1)];
+    }
+    __device__ __forceinline__ uint64_t bits(int lane) const {
+        return __builtin_amdgcn_ballot_w64(lane < left && byte != 0u);
+    }
+};
 
 __device__ __forceinline__ float swap_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -219,13 +229,15 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd16_kernel(CrossArgs a) {
     const T* kbase = static_cast<const T*>(a.k) + kvh * a.ldkh;
     const T* vbase = static_cast<const T*>(a.v) + kvh * a.ldvh;
     Stage<T, DP, NT> sk, sv;
-    uint64_t bits = 0, next = 0;
+    KeyBits kb;
+    uint64_t bits = 0;
     if (it.c0 < it.c1) {
         const int64_t key0 = it.k_begin + static_cast<int64_t>(it.c0);
         const int left = it.c1 - it.c0;
+        kb.load(a, key0, left, lane);
         sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
         sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
-        bits = key_bits(a, key0, left, lane);
+        bits = kb.bits(lane);
         sk.write(lds, ~0ull);
         sv.write(lds + TILE, bits);
     }
@@ -238,28 +250,28 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd16_kernel(CrossArgs a) {
         if (more) {
             const int64_t key0 = it.k_begin + static_cast<int64_t>(k0 + KT);
             const int left = it.c1 - k0 - KT;
+            kb.load(a, key0, left, lane);
             sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
             sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
-            next = key_bits(a, key0, left, lane);
         }
         f32x16 s[CB][2] = {};
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                const vec8<T> f = row_frag<T, DP>(kt, 32 * kb, i, col, half);
+                const vec8<T> f = row_frag<T, DP>(kt, 32 * hb, i, col, half);
 #pragma unroll
-                for (int cb = 0; cb < CB; ++cb) s[cb][kb] = mfma16(f, qf[cb][i], s[cb][kb]);
+                for (int cb = 0; cb < CB; ++cb) s[cb][hb] = mfma16(f, qf[cb][i], s[cb][hb]);
             }
         if (bits != ~0ull) {
             const uint64_t mine = bits >> (4 * half);
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (!((mine >> (32 * kb + acc_row(r))) & 1u)) {
+                    if (!((mine >> (32 * hb + acc_row(r))) & 1u)) {
 #pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) s[cb][kb][r] = -INFINITY;
+                        for (int cb = 0; cb < CB; ++cb) s[cb][hb][r] = -INFINITY;
                     }
         }
 #pragma unroll
@@ -301,12 +313,12 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd16_kernel(CrossArgs a) {
         }
         if (more) {
             char* dst = lds + (buf ^ 1) * 2 * TILE;
+            bits = kb.bits(lane);
             sk.write(dst, ~0ull);
-            sv.write(dst + TILE, next);
+            sv.write(dst + TILE, bits);
         }
         __syncthreads();
         buf ^= 1;
-        bits = next;
     }
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
@@ -374,13 +386,15 @@ __global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
     const T* kbase = static_cast<const T*>(a.k) + kvh * a.ldkh;
     const T* vbase = static_cast<const T*>(a.v) + kvh * a.ldvh;
     Stage<T, DP, NT> sk, sv;
-    uint64_t bits = 0, next = 0;
+    KeyBits kb;
+    uint64_t bits = 0;
     if (it.c0 < it.c1) {
         const int64_t key0 = it.k_begin + static_cast<int64_t>(it.c0);
         const int left = it.c1 - it.c0;
+        kb.load(a, key0, left, lane);
         sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
         sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
-        bits = key_bits(a, key0, left, lane);
+        bits = kb.bits(lane);
         sk.write(lds, bits);
         sv.write(lds + TILE, bits);
     }
@@ -393,17 +407,17 @@ __global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
         if (more) {
             const int64_t key0 = it.k_begin + static_cast<int64_t>(k0 + KT);
             const int left = it.c1 - k0 - KT;
+            kb.load(a, key0, left, lane);
             sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
             sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
-            next = key_bits(a, key0, left, lane);
         }
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int hb = 0; hb < 2; ++hb) {
             f32x16 s[CB] = {}, dp[CB] = {};
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                const vec8<T> fk = row_frag<T, DP>(kt, 32 * kb, i, col, half);
-                const vec8<T> fv = row_frag<T, DP>(vt, 32 * kb, i, col, half);
+                const vec8<T> fk = row_frag<T, DP>(kt, 32 * hb, i, col, half);
+                const vec8<T> fv = row_frag<T, DP>(vt, 32 * hb, i, col, half);
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
                     s[cb] = mfma16(fk, qf[cb][i], s[cb]);
@@ -417,7 +431,7 @@ __global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
                     s[cb][r] = __builtin_amdgcn_exp2f(fmaf(s[cb][r], a.c, sc[cb].up - lse[cb])) *
                                (dp[cb][r] - delta[cb]);
             if (bits != ~0ull) {
-                const uint32_t mine = static_cast<uint32_t>(bits >> (32 * kb + 4 * half));
+                const uint32_t mine = static_cast<uint32_t>(bits >> (32 * hb + 4 * half));
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (!((mine >> acc_row(r)) & 1u)) {
@@ -434,7 +448,7 @@ __global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
                 for (int cb = 0; cb < CB; ++cb) p[cb] = pack8<T>(s[cb], t);
 #pragma unroll
                 for (int b = 0; b < DP / 32; ++b) {
-                    const vec8<T> f = tr_frag<T, DP>(kt, trl, 32 * kb + 16 * t, b);
+                    const vec8<T> f = tr_frag<T, DP>(kt, trl, 32 * hb + 16 * t, b);
 #pragma unroll
                     for (int cb = 0; cb < CB; ++cb) acc[cb][b] = mfma16(f, p[cb], acc[cb][b]);
                 }
@@ -442,12 +456,12 @@ __global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
         }
         if (more) {
             char* dst = lds + (buf ^ 1) * 2 * TILE;
-            sk.write(dst, next);
-            sv.write(dst + TILE, next);
+            bits = kb.bits(lane);
+            sk.write(dst, bits);
+            sv.write(dst + TILE, bits);
         }
         __syncthreads();
         buf ^= 1;
-        bits = next;
     }
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {

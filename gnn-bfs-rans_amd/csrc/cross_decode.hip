@@ -16,12 +16,39 @@ namespace mignn {
 namespace {
 
 constexpr int WAVES = 4;
-constexpr int UNROLL = 4;
+
+// sum over the LPK (4..32) lanes of a key, for each of them: butterflies whose
+// exchanges are lane permutations of the adder itself (a mirror of 8 or 16
+// lanes serves as an exchange of their halves once the halves are uniform)
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int LPK>
+__device__ __forceinline__ float key_sum(float v) {
+    v = dpp_add<0xb1>(v);                            // quad_perm 1 0 3 2
+    v = dpp_add<0x4e>(v);                            // quad_perm 2 3 0 1
+    if constexpr (LPK >= 8) v = dpp_add<0x141>(v);   // row_half_mirror
+    if constexpr (LPK >= 16) v = dpp_add<0x140>(v);  // row_mirror
+    if constexpr (LPK >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
+// One thread's share of UNROLL keys, in flight
+template <typename T, int UNROLL>
+struct KeyLoad {
+    static constexpr int V = 16 / sizeof(T);
+    RowVec<T, V> k[UNROLL], v[UNROLL];
+    uint32_t ok[UNROLL];   // as loaded: a comparison here would wait for all loads before it
+};
 
 // R rows (a power of two that holds the sequence's); LPK lanes a key, V elements each
 template <typename T, int R, int LPK>
 __global__ __launch_bounds__(WAVES * 64) void cross_few_kernel(CrossArgs a) {
-    constexpr int V = 16 / sizeof(T), KPW = 64 / LPK;
+    constexpr int V = 16 / sizeof(T), KPW = 64 / LPK, UNROLL = R == 8 ? 2 : 4;
     int item, kvh;
     if (!cross_work(a, a.n_items, item, kvh)) return;
     const CrossItem it = a.items[item];
@@ -45,21 +72,36 @@ __global__ __launch_bounds__(WAVES * 64) void cross_few_kernel(CrossArgs a) {
     }
     const T* kb = static_cast<const T*>(a.k) + kvh * a.ldkh + c0;
     const T* vb = static_cast<const T*>(a.v) + kvh * a.ldvh + c0;
-    for (int k0 = it.c0 + wave * KPW * UNROLL; k0 < it.c1; k0 += WAVES * KPW * UNROLL) {
-        float kf[UNROLL][V], vf[UNROLL][V];
-        bool ok[UNROLL];
+    KeyLoad<T, UNROLL> now, next;
+    auto load = [&](KeyLoad<T, UNROLL>& n, int k0) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const int k = k0 + u * KPW + grp;
             const int64_t key = it.k_begin + static_cast<int64_t>(k < it.c1 ? k : it.c1 - 1);
-            ok[u] = k < it.c1 && (!a.mask || a.mask[key]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) kf[u][i] = vf[u][i] = 0.f;
+            n.ok[u] = a.mask ? a.mask[key] : 1u;
+            n.k[u] = n.v[u] = RowVec<T, V>{};
             if (in) {
-                load_row(kb + key * a.ldk, kf[u]);
-                load_row(vb + key * a.ldv, vf[u]);
+                __builtin_memcpy(&n.k[u], kb + key * a.ldk, 16);
+                __builtin_memcpy(&n.v[u], vb + key * a.ldv, 16);
             }
         }
+    };
+    constexpr int STEP = WAVES * KPW * UNROLL;
+    int k0 = it.c0 + wave * KPW * UNROLL;
+    if (k0 < it.c1) load(now, k0);
+    for (; k0 < it.c1; k0 += STEP, now = next) {
+        if (k0 + STEP < it.c1) load(next, k0 + STEP);
+        bool ok[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) ok[u] = now.ok[u] != 0u && k0 + u * KPW + grp < it.c1;
+        float kf[UNROLL][V], vf[UNROLL][V];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                kf[u][i] = static_cast<float>(now.k[u].v[i]);
+                vf[u][i] = static_cast<float>(now.v[u].v[i]);
+            }
         float s[R][UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
@@ -68,8 +110,7 @@ __global__ __launch_bounds__(WAVES * 64) void cross_few_kernel(CrossArgs a) {
                 float x = 0.f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) x = fmaf(q[r][i], kf[u][i], x);
-#pragma unroll
-                for (int b = 1; b < LPK; b <<= 1) x += __shfl_xor(x, b);
+                x = key_sum<LPK>(x);
                 s[r][u] = ok[u] ? x : -INFINITY;
             }
         // what the mask leaves out may hold anything, and 0 inf is no 0
