@@ -122,7 +122,7 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd_kernel(CrossArgs a) {
     __shared__ __attribute__((aligned(16))) float ks[32 * (DP + 4)], vs[32 * (DP + 4)];
     int item, kvh;
     if (!cross_work(a, a.n_items, item, kvh)) return;
-    const CrossItem it = a.items[item];
+    const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int row = it.r0 + wave * 32 + col;
     const bool live = row < it.r1;
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(CrossArgs a) {
     __shared__ __attribute__((aligned(16))) float ks[32 * (DP + 4)], vs[32 * (DP + 4)];
     int item, kvh;
     if (!cross_work(a, a.n_items, item, kvh)) return;
-    const CrossItem it = a.items[item];
+    const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int row = it.r0 + wave * 32 + col;
     const bool live = row < it.r1;
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(NW * 64) void cross_dkv_kernel(CrossArgs a) {
     __shared__ __attribute__((aligned(16))) float ls[32], ds[32];
     int item, kvh;
     if (!cross_work(a, a.n_items, item, kvh)) return;
-    const CrossItem it = a.items[item];
+    const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int key = it.r0 + wave * 32 + col;
     const int64_t kt = it.k_begin + static_cast<int64_t>(key);
@@ -417,6 +417,7 @@ struct PassShape {
     int tile;        // rows of a tile
     int64_t longest; // of the r side
     int64_t chunk;
+    int64_t unit;    // chunks are a multiple of it
 };
 struct PassPlan {
     int64_t items = 0, joins = 0, slots = 0;
@@ -429,9 +430,10 @@ struct PassPlan {
 // CUs, eight small ones) when its tiles alone are fewer; not under `least`,
 // where the parts' join would cost what the split gains.
 PassShape pass_shape(const int64_t* rows, const int64_t* keys, int64_t batch, int pass, int kv_heads,
-                     int dtype) {
+                     int group) {
     const bool dkv = pass == MIGNN_CROSS_DKV;
-    PassShape s{128, 0, 0};
+    // (dk / dv: whole queries, as many as an LDS tile holds)
+    PassShape s{128, 0, 0, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
     for (int64_t b = 0; b < batch; ++b) {
         const int64_t r = dkv ? keys[b] : rows[b];
         if (r > s.longest) s.longest = r;
@@ -446,7 +448,7 @@ PassShape pass_shape(const int64_t* rows, const int64_t* keys, int64_t batch, in
     const int64_t target = s.tile == 128 ? 512 : 2048, least = s.tile == 128 ? 256 : 128;
     s.chunk = static_cast<int64_t>(work * kv_heads / static_cast<double>(target));
     if (s.chunk < least) s.chunk = least;
-    s.chunk = (s.chunk + 63) / 64 * 64;
+    s.chunk = (s.chunk + s.unit - 1) / s.unit * s.unit;
     return s;
 }
 
@@ -459,8 +461,8 @@ PassPlan plan_pass(const PassShape& shape, const int64_t* rows, const int64_t* q
         const int64_t rn = dkv ? keys[b] : rows[b], cn = dkv ? rows[b] : keys[b];
         int64_t parts = (cn + chunk - 1) / chunk;
         if (parts < 1) parts = 1;
-        // equal parts, each a multiple of 64 but the last
-        const int64_t len = cn == 0 ? 0 : ((cn + parts - 1) / parts + 63) / 64 * 64;
+        // equal parts, each a multiple of the unit but the last
+        const int64_t len = cn == 0 ? 0 : ((cn + parts - 1) / parts + shape.unit - 1) / shape.unit * shape.unit;
         if (len > 0) parts = (cn + len - 1) / len;
         for (int64_t r0 = 0; r0 < rn; r0 += tile) {
             const int64_t r1 = r0 + tile < rn ? r0 + tile : rn;
@@ -556,6 +558,8 @@ int check_dims(const char* who, int heads, int kv_heads, int d, int dtype) {
     MIGNN_REQUIRE(row_type_ok(dtype), "%s: unknown row type %d", who, dtype);
     MIGNN_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads <= 65535,
                   "%s: %d query heads over %d key heads", who, heads, kv_heads);
+    MIGNN_REQUIRE(heads / kv_heads <= MIGNN_CROSS_MAX_GROUP, "%s: more than %d query heads a key head", who,
+                  MIGNN_CROSS_MAX_GROUP);
     MIGNN_REQUIRE(d > 0 && d % 8 == 0 && d <= MIGNN_CROSS_MAX_D, "%s: head width %d (a multiple of 8, <= %d)",
                   who, d, MIGNN_CROSS_MAX_D);
     return MIGNN_OK;
@@ -567,6 +571,9 @@ int check_rows(const char* who, const char* what, const void* p, int64_t ldt, in
     MIGNN_REQUIRE(p && aligned16(p) && ldt >= 0 && ldh >= 0 && ldt * es % 16 == 0 &&
                       ldh * es % 16 == 0,
                   "%s: %s needs a 16-byte aligned pointer and strides", who, what);
+    // the staging of 64 rows addresses them by 32-bit offsets
+    MIGNN_REQUIRE(ldt <= MIGNN_CROSS_MAX_STRIDE && ldh <= MIGNN_CROSS_MAX_STRIDE,
+                  "%s: %s has strides above %d elements", who, what, MIGNN_CROSS_MAX_STRIDE);
     return MIGNN_OK;
 }
 
@@ -597,7 +604,7 @@ extern "C" int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, in
     int64_t* rows = static_cast<int64_t*>(malloc(sizeof(int64_t) * (batch > 0 ? batch : 1)));
     MIGNN_REQUIRE(rows, "cross_plan: out of host memory");
     for (int64_t b = 0; b < batch; ++b) rows[b] = q_lens[b] * group;
-    const PassShape sh = pass_shape(rows, k_lens, batch, pass, kv_heads, dtype);
+    const PassShape sh = pass_shape(rows, k_lens, batch, pass, kv_heads, static_cast<int>(group));
     const PassPlan p = plan_pass(sh, rows, q_lens, k_lens, batch, pass == MIGNN_CROSS_DKV,
                                  static_cast<CrossItem*>(items), static_cast<CrossJoin*>(joins));
     free(rows);

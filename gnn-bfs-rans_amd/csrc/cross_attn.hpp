@@ -11,6 +11,7 @@ using f32x16 = __attribute__((ext_vector_type(16))) float;
 
 constexpr int CROSS_ROWS = 32;    // rows (or keys) a wave owns: one MFMA tile edge
 constexpr int CROSS_FEW = 8;      // rows that cross_few takes
+constexpr int CROSS_STAGE = 64;   // rows of an LDS tile of the 16-bit kernels
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // One workgroup's share of a pass, per kv head.  "Rows" are the (query, head
@@ -49,6 +50,28 @@ struct CrossArgs {
     int32_t tile, rows;          // of the pass: rows (keys) of a tile, of the longest sequence
     float scale, c;              // c = scale log2(e)
 };
+
+// A uniform value that the compiler cannot see to be one
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t uniform(const void* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(v)))) |
+           static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(v >> 32)))) << 32;
+}
+__device__ __forceinline__ CrossItem load_item(const CrossArgs& a, int item) {
+    CrossItem it = a.items[item];
+    it.q_begin = uniform(it.q_begin), it.k_begin = uniform(it.k_begin);
+    it.r0 = uniform(it.r0), it.r1 = uniform(it.r1);
+    it.c0 = uniform(it.c0), it.c1 = uniform(it.c1);
+    it.slot = uniform(it.slot);
+    return it;
+}
+
+// 16 bytes at base + voffset; a lane whose bytes do not end by num_records
+// reads zeros and asks for nothing
+__device__ f32x4 raw_buffer_load_f32x4(i32x4 rsrc, int voffset, int soffset, int aux) __asm(
+    "llvm.amdgcn.raw.buffer.load.v4f32");
+constexpr int NO_LOAD = INT32_MIN;   // a voffset past every num_records
 
 // Block -> (item, kv head).  Consecutive blocks go to the 8 XCDs in turn; each
 // XCD gets one run of the (head-major) work, so that the tiles that read one

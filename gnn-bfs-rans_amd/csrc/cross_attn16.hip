@@ -40,7 +40,7 @@ __device__ __forceinline__ f32x16 mfma16(vec8<f16_t> a, vec8<f16_t> b, f32x16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-constexpr int KT = 64;   // rows of an LDS tile
+constexpr int KT = CROSS_STAGE;
 
 template <int DP>
 constexpr int pitch() { return DP * 2 + 32; }
@@ -92,30 +92,47 @@ __device__ __forceinline__ vec8<T> pack8(const f32x16& w, int t) {
     return v;
 }
 
-// One thread's share of a 64-row tile on its way from memory to LDS
+// One thread's share of a 64-row tile on its way from memory to LDS: buffer
+// loads at constant offsets from a scalar base that moves on with the tiles
 template <typename T, int DP, int NT>
 struct Stage {
     static constexpr int C8 = DP / 8, N = KT * C8 / NT;
     static_assert(KT * C8 % NT == 0, "tile share");
-    u32x4 v[N];
+    f32x4 v[N];
+    int off[N];
+    uint32_t bytes;
     __device__ __forceinline__ static int row(int j) { return (threadIdx.x + j * NT) / C8; }
     __device__ __forceinline__ static int chunk(int j) { return (threadIdx.x + j * NT) % C8; }
-    // rows from..to - 1 of a matrix of row stride ld; rows past the end repeat the last
-    __device__ __forceinline__ void load(const T* base, int64_t ld, int left, int d) {
+    // tile row r is row r / group, head r % group of a matrix of strides ldt, ldh
+    __device__ __forceinline__ void init(int64_t ldt, int64_t ldh, int group, int d) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int r = row(j) < left ? row(j) : left - 1;
-            v[j] = u32x4{};
-            if (chunk(j) * 8 < d)
-                v[j] = *reinterpret_cast<const u32x4*>(base + r * ld + chunk(j) * 8);
+            const int t = row(j) / group, h = row(j) - t * group;
+            off[j] = chunk(j) * 8 < d ? static_cast<int>((t * ldt + h * ldh + chunk(j) * 8) * sizeof(T))
+                                      : NO_LOAD;
         }
+        // (63 rows' and all heads' strides fit: checked by the host)
+        bytes = uniform(static_cast<int>((KT / group * ldt + group * ldh + d) * sizeof(T)));
     }
-    __device__ __forceinline__ void write(char* tile, uint64_t keep) const {
+    // the `left` rows from `base` on; zeros after them
+    __device__ __forceinline__ void load(const T* base, int left) {
+        const i32x4 rsrc = buffer_rsrc(uniform(base), bytes);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const u32x4 x = (keep >> row(j)) & 1u ? v[j] : u32x4{};
-            *reinterpret_cast<u32x4*>(tile + row(j) * pitch<DP>() + chunk(j) * 16) = x;
-        }
+        for (int j = 0; j < N; ++j)
+            v[j] = raw_buffer_load_f32x4(rsrc, left >= KT || row(j) < left ? off[j] : NO_LOAD, 0, 0);
+    }
+    __device__ __forceinline__ void write(char* tile) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            *reinterpret_cast<f32x4*>(tile + row(j) * pitch<DP>() + chunk(j) * 16) = v[j];
+    }
+    // rows whose bit is clear as zeros
+    __device__ __forceinline__ void write(char* tile, uint64_t keep) const {
+        if (keep == ~0ull) return write(tile);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            *reinterpret_cast<f32x4*>(tile + row(j) * pitch<DP>() + chunk(j) * 16) =
+                (keep >> row(j)) & 1u ? v[j] : f32x4{};
     }
 };
 
@@ -202,14 +219,15 @@ struct DsScale {
 };
 
 template <typename T, int DP, int NW, int CB>
-__global__ __launch_bounds__(NW * 64) void cross_fwd16_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, 2) void cross_fwd16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];   // K, V; twice
     int item, kvh;
     if (!cross_work(a, a.n_items, item, kvh)) return;
-    const CrossItem it = a.items[item];
+    const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
+    constexpr f32x16 zero = {};
     vec8<T> qf[CB][DP / 16];
     int row[CB];
     int64_t at[CB];
@@ -229,16 +247,18 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd16_kernel(CrossArgs a) {
     const T* kbase = static_cast<const T*>(a.k) + kvh * a.ldkh;
     const T* vbase = static_cast<const T*>(a.v) + kvh * a.ldvh;
     Stage<T, DP, NT> sk, sv;
+    sk.init(a.ldk, 0, 1, a.d);
+    sv.init(a.ldv, 0, 1, a.d);
     KeyBits kb;
     uint64_t bits = 0;
     if (it.c0 < it.c1) {
         const int64_t key0 = it.k_begin + static_cast<int64_t>(it.c0);
         const int left = it.c1 - it.c0;
         kb.load(a, key0, left, lane);
-        sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
-        sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
+        sk.load(kbase + key0 * a.ldk, left);
+        sv.load(vbase + key0 * a.ldv, left);
         bits = kb.bits(lane);
-        sk.write(lds, ~0ull);
+        sk.write(lds);
         sv.write(lds + TILE, bits);
     }
     __syncthreads();
@@ -251,17 +271,17 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd16_kernel(CrossArgs a) {
             const int64_t key0 = it.k_begin + static_cast<int64_t>(k0 + KT);
             const int left = it.c1 - k0 - KT;
             kb.load(a, key0, left, lane);
-            sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
-            sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
+            sk.load(kbase + key0 * a.ldk, left);
+            sv.load(vbase + key0 * a.ldv, left);
         }
-        f32x16 s[CB][2] = {};
+        f32x16 s[CB][2];
 #pragma unroll
         for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const vec8<T> f = row_frag<T, DP>(kt, 32 * hb, i, col, half);
 #pragma unroll
-                for (int cb = 0; cb < CB; ++cb) s[cb][hb] = mfma16(f, qf[cb][i], s[cb][hb]);
+                for (int cb = 0; cb < CB; ++cb) s[cb][hb] = mfma16(f, qf[cb][i], i == 0 ? zero : s[cb][hb]);
             }
         if (bits != ~0ull) {
             const uint64_t mine = bits >> (4 * half);
@@ -314,7 +334,7 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd16_kernel(CrossArgs a) {
         if (more) {
             char* dst = lds + (buf ^ 1) * 2 * TILE;
             bits = kb.bits(lane);
-            sk.write(dst, ~0ull);
+            sk.write(dst);
             sv.write(dst + TILE, bits);
         }
         __syncthreads();
@@ -341,14 +361,15 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd16_kernel(CrossArgs a) {
 }
 
 template <typename T, int DP, int NW, int CB>
-__global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, 2) void cross_dq16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
     int item, kvh;
     if (!cross_work(a, a.n_items, item, kvh)) return;
-    const CrossItem it = a.items[item];
+    const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
+    constexpr f32x16 zero = {};
     vec8<T> qf[CB][DP / 16], gf[CB][DP / 16];
     int row[CB];
     int64_t at[CB];
@@ -386,14 +407,16 @@ __global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
     const T* kbase = static_cast<const T*>(a.k) + kvh * a.ldkh;
     const T* vbase = static_cast<const T*>(a.v) + kvh * a.ldvh;
     Stage<T, DP, NT> sk, sv;
+    sk.init(a.ldk, 0, 1, a.d);
+    sv.init(a.ldv, 0, 1, a.d);
     KeyBits kb;
     uint64_t bits = 0;
     if (it.c0 < it.c1) {
         const int64_t key0 = it.k_begin + static_cast<int64_t>(it.c0);
         const int left = it.c1 - it.c0;
         kb.load(a, key0, left, lane);
-        sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
-        sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
+        sk.load(kbase + key0 * a.ldk, left);
+        sv.load(vbase + key0 * a.ldv, left);
         bits = kb.bits(lane);
         sk.write(lds, bits);
         sv.write(lds + TILE, bits);
@@ -408,20 +431,20 @@ __global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
             const int64_t key0 = it.k_begin + static_cast<int64_t>(k0 + KT);
             const int left = it.c1 - k0 - KT;
             kb.load(a, key0, left, lane);
-            sk.load(kbase + key0 * a.ldk, a.ldk, left, a.d);
-            sv.load(vbase + key0 * a.ldv, a.ldv, left, a.d);
+            sk.load(kbase + key0 * a.ldk, left);
+            sv.load(vbase + key0 * a.ldv, left);
         }
 #pragma unroll
         for (int hb = 0; hb < 2; ++hb) {
-            f32x16 s[CB] = {}, dp[CB] = {};
+            f32x16 s[CB], dp[CB];
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const vec8<T> fk = row_frag<T, DP>(kt, 32 * hb, i, col, half);
                 const vec8<T> fv = row_frag<T, DP>(vt, 32 * hb, i, col, half);
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
-                    s[cb] = mfma16(fk, qf[cb][i], s[cb]);
-                    dp[cb] = mfma16(fv, gf[cb][i], dp[cb]);
+                    s[cb] = mfma16(fk, qf[cb][i], i == 0 ? zero : s[cb]);
+                    dp[cb] = mfma16(fv, gf[cb][i], i == 0 ? zero : dp[cb]);
                 }
             }
 #pragma unroll
@@ -475,42 +498,17 @@ __global__ __launch_bounds__(NW * 64) void cross_dq16_kernel(CrossArgs a) {
     }
 }
 
-// One thread's share of a tile of 64 (query, head) rows
-template <typename T, int DP, int NT>
-struct RowStage {
-    static constexpr int C8 = DP / 8, N = KT * C8 / NT;
-    u32x4 v[N];
-    __device__ __forceinline__ void load(const T* base, int64_t ldt, int64_t ldh, int r0, int r1, int group,
-                                         int d) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int r = r0 + (threadIdx.x + j * NT) / C8, c = (threadIdx.x + j * NT) % C8 * 8;
-            v[j] = u32x4{};
-            if (r < r1 && c < d) {
-                const int t = r / group;
-                v[j] = *reinterpret_cast<const u32x4*>(base + t * ldt + (r - t * group) * ldh + c);
-            }
-        }
-    }
-    __device__ __forceinline__ void write(char* tile) const {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int i = threadIdx.x + j * NT;
-            *reinterpret_cast<u32x4*>(tile + i / C8 * pitch<DP>() + i % C8 * 16) = v[j];
-        }
-    }
-};
-
 template <typename T, int DP, int NW, int CB>
-__global__ __launch_bounds__(NW * 64) void cross_dkv16_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, DP <= 96 ? 2 : 1) void cross_dkv16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];   // lse, delta
     int item, kvh;
     if (!cross_work(a, a.n_items, item, kvh)) return;
-    const CrossItem it = a.items[item];
+    const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
+    constexpr f32x16 zero = {};
     vec8<T> kf[CB][DP / 16], vf[CB][DP / 16];
     int key[CB];
     bool keep[CB];
@@ -531,16 +529,21 @@ __global__ __launch_bounds__(NW * 64) void cross_dkv16_kernel(CrossArgs a) {
     for (int cb = 0; cb < CB; ++cb) gain[cb] = __builtin_amdgcn_exp2f(sc[cb].up - PB_UP<T>);
     const T* qbase = static_cast<const T*>(a.q) + it.q_begin * a.ldq + kvh * a.group * a.ldqh;
     const T* gbase = static_cast<const T*>(a.dout) + it.q_begin * a.lddo + kvh * a.group * a.lddoh;
-    RowStage<T, DP, NT> sq, sg;
+    Stage<T, DP, NT> sq, sg;
+    sq.init(a.ldq, a.ldqh, a.group, a.d);
+    sg.init(a.lddo, a.lddoh, a.group, a.d);
+    // whole queries a tile: the offsets are the same in every tile
+    const int tokens = KT / a.group, step = tokens * a.group;
+    const int my_t = threadIdx.x / a.group, my_h = threadIdx.x - my_t * a.group;
     float lse = INFINITY, delta = 0.f;
-    auto load = [&](int r0) {
-        sq.load(qbase, a.ldq, a.ldqh, r0, it.c1, a.group, a.d);
-        sg.load(gbase, a.lddo, a.lddoh, r0, it.c1, a.group, a.d);
+    auto load = [&](int r0, int t0) {
+        const int left = it.c1 - r0 < step ? it.c1 - r0 : step;
+        sq.load(qbase + t0 * a.ldq, left);
+        sg.load(gbase + t0 * a.lddo, left);
         if (threadIdx.x < KT) {   // rows past the end: lse = inf, P = 0
-            const int r = r0 + threadIdx.x, t = r / a.group;
             lse = INFINITY, delta = 0.f;
-            if (r < it.c1) {
-                const int64_t at = (it.q_begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group + r - t * a.group;
+            if (static_cast<int>(threadIdx.x) < left) {
+                const int64_t at = (it.q_begin + static_cast<int64_t>(t0 + my_t)) * a.heads + kvh * a.group + my_h;
                 lse = a.lse[at] - PB_UP<T>;
                 delta = a.delta[at];
             }
@@ -552,27 +555,27 @@ __global__ __launch_bounds__(NW * 64) void cross_dkv16_kernel(CrossArgs a) {
         if (threadIdx.x < KT) st[buf][0][threadIdx.x] = lse, st[buf][1][threadIdx.x] = delta;
     };
     if (it.c0 < it.c1) {
-        load(it.c0);
+        load(it.c0, it.c0 / a.group);
         write(0);
     }
     __syncthreads();
     int buf = 0;
-    for (int r0 = it.c0; r0 < it.c1; r0 += KT) {
+    for (int r0 = it.c0, t0 = it.c0 / a.group; r0 < it.c1; r0 += step, t0 += tokens) {
         const char* qt = lds + buf * 2 * TILE;
         const char* gt = qt + TILE;
-        const bool more = r0 + KT < it.c1;
-        if (more) load(r0 + KT);
+        const bool more = r0 + step < it.c1;
+        if (more) load(r0 + step, t0 + tokens);
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
-            f32x16 s[CB] = {}, dp[CB] = {};
+            f32x16 s[CB], dp[CB];
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const vec8<T> fq = row_frag<T, DP>(qt, 32 * rb, i, col, half);
                 const vec8<T> fg = row_frag<T, DP>(gt, 32 * rb, i, col, half);
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
-                    s[cb] = mfma16(fq, kf[cb][i], s[cb]);
-                    dp[cb] = mfma16(fg, vf[cb][i], dp[cb]);
+                    s[cb] = mfma16(fq, kf[cb][i], i == 0 ? zero : s[cb]);
+                    dp[cb] = mfma16(fg, vf[cb][i], i == 0 ? zero : dp[cb]);
                 }
             }
 #pragma unroll
