@@ -46,29 +46,41 @@ def _row_type(what: str, t: torch.Tensor) -> int:
 
 
 def _on_device(what: str, ref: torch.Tensor, **others):
-    if ref.device.type != "cuda":
+    """Raises unless `ref` is on a ROCm device and the others are with it."""
+    if not ref.is_cuda:
         raise RuntimeError(f"mignn {what} runs on ROCm devices only (no CPU path)")
     for name, t in others.items():
         if t is not None and t.device != ref.device:
             raise RuntimeError(f"mignn {what}: {name} is on {t.device}, not on {ref.device}")
 
 
-class _device_of:
-    """Makes a tensor's device current around a launch (nothing to do when it
-    is)."""
-    __slots__ = ("index", "prev")
+_get_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-    def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
 
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
+def _launch(fn, what: str, index: int, *args):
+    """fn(*args, stream) with device `index` current and its current stream."""
+    prev = _get_device()
+    if prev != index:
+        torch.cuda.set_device(index)
+    try:
+        rc = fn(*args, _raw_stream(index))
+    finally:
+        if prev != index:
+            torch.cuda.set_device(prev)
+    if rc:
+        _lib.check(rc, what)
 
-    def __exit__(self, *exc):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
+
+def _first_order(backward):
+    """A backward whose kernels autograd cannot see: under create_graph its
+    gradients refuse to be differentiated again (the wrapper costs a few
+    microseconds, so it is taken only then)."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return staticmethod(run)
 
 
 def _grad(*ts) -> bool:
@@ -92,11 +104,10 @@ def _norm_forward(x, weight, residual, eps: float, code: int):
     n, h = x.shape
     y = torch.empty((n, h), dtype=x.dtype, device=x.device)
     s = None if residual is None else torch.empty_like(y)
-    with _device_of(x):
-        _lib.check(_lib.lib().mignn_rms_norm(
-            P(x), x.stride(0), P(residual), 0 if residual is None else residual.stride(0),
-            P(weight), weight.dtype == torch.float32, n, h, eps, code, P(y), h, P(s), h,
-            _lib.stream(x.device)), "mignn_rms_norm")
+    _launch(_lib.lib().mignn_rms_norm, "mignn_rms_norm", x.device.index,
+            x.data_ptr(), x.stride(0), P(residual),
+            0 if residual is None else residual.stride(0), weight.data_ptr(),
+            weight.dtype == torch.float32, n, h, eps, code, y.data_ptr(), h, P(s), h)
     return y, s
 
 
@@ -114,8 +125,7 @@ class _RMSNorm(Function):
             ctx.save_for_backward(x, weight, residual)
         return y if s is None else (y, s)
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, ds=None):
         x, weight, residual = ctx.saved_tensors
         if dy is None:
@@ -135,12 +145,12 @@ class _RMSNorm(Function):
             dw = torch.empty_like(weight)
             nbytes = L.mignn_rms_norm_backward_scratch_bytes(n, h, ctx.code)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        with _device_of(x):
-            _lib.check(L.mignn_rms_norm_backward(
-                P(x), x.stride(0), P(residual), 0 if residual is None else residual.stride(0),
-                P(weight), weight.dtype == torch.float32, n, h, ctx.eps, ctx.code, P(dy),
-                dy.stride(0), P(ds), 0 if ds is None else ds.stride(0), P(dx), h, P(dw),
-                P(scratch), nbytes, _lib.stream(x.device)), "mignn_rms_norm_backward")
+        _launch(L.mignn_rms_norm_backward, "mignn_rms_norm_backward", x.device.index,
+                x.data_ptr(), x.stride(0), P(residual),
+                0 if residual is None else residual.stride(0), weight.data_ptr(),
+                weight.dtype == torch.float32, n, h, ctx.eps, ctx.code, dy.data_ptr(),
+                dy.stride(0), P(ds), 0 if ds is None else ds.stride(0), dx.data_ptr(), h, P(dw),
+                P(scratch), nbytes)
         return dx, dw, dx if ctx.residual else None, None, None
 
 
@@ -211,11 +221,15 @@ class RotaryAxes:
 
 def _heads(t: torch.Tensor, align: int = 1) -> torch.Tensor:
     """[rows, heads, d] with contiguous columns; align: bytes that the pointer
-    and the strides are multiples of (a copy if need be)."""
-    es = t.element_size()
-    if (t.shape[2] > 1 and t.stride(2) != 1) or t.data_ptr() % align or \
-            t.stride(0) * es % align or t.stride(1) * es % align:
+    and the strides are multiples of, the strides then also within the kernels'
+    32-bit offsets (a copy if need be)."""
+    st, sh, sd = t.stride()
+    if sd != 1 and t.shape[2] > 1:
         return t.clone(memory_format=torch.contiguous_format)
+    if align > 1:
+        es = t.element_size()
+        if (t.data_ptr() | st * es | sh * es) % align or max(st, sh) > _lib.CROSS_MAX_STRIDE:
+            return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -225,11 +239,10 @@ def _turn(x, pos, axes: RotaryAxes, code: int, inverse: bool):
     if pos.shape[1] > 1 and pos.stride(1) != 1:
         pos = pos.contiguous()
     y = torch.empty((n, heads, d), dtype=x.dtype, device=x.device)
-    with _device_of(x):
-        _lib.check(_lib.lib().mignn_rotary(
-            P(x), x.stride(0), x.stride(1), n, heads, d, P(pos), _POS[pos.dtype], pos.stride(0),
-            P(axes.freq), P(axes.axis), axes.total, axes.interleaved, inverse, code, P(y),
-            heads * d, d, _lib.stream(x.device)), "mignn_rotary")
+    _launch(_lib.lib().mignn_rotary, "mignn_rotary", x.device.index,
+            x.data_ptr(), x.stride(0), x.stride(1), n, heads, d, pos.data_ptr(), _POS[pos.dtype],
+            pos.stride(0), axes.freq.data_ptr(), axes.axis.data_ptr(), axes.total,
+            axes.interleaved, inverse, code, y.data_ptr(), heads * d, d)
     return y
 
 
@@ -240,8 +253,7 @@ class _Rotary(Function):
         ctx.save_for_backward(pos)
         return _turn(x, pos, axes, code, False)
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         (pos,) = ctx.saved_tensors
         return _turn(dy, pos, ctx.axes, ctx.code, True), None, None, None
@@ -308,6 +320,8 @@ class CrossPlan:
         kv_heads = heads if kv_heads is None else kv_heads
         if heads < 1 or kv_heads < 1 or heads % kv_heads:
             raise ValueError(f"CrossPlan: {heads} query heads over {kv_heads} key heads")
+        if heads // kv_heads > _lib.CROSS_MAX_GROUP:
+            raise ValueError(f"CrossPlan: more than {_lib.CROSS_MAX_GROUP} query heads a key head")
         if head_dim < 8 or head_dim % 8 or head_dim > _lib.CROSS_MAX_D:
             raise ValueError(f"CrossPlan: head_dim must be a multiple of 8 up to "
                              f"{_lib.CROSS_MAX_D}, got {head_dim}")
@@ -375,12 +389,10 @@ def _cross_forward(q, k, v, plan: CrossPlan, mask, scale: float, train: bool):
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
         if q.dtype != torch.float32:
             out32 = torch.empty(q.shape, dtype=torch.float32, device=q.device)
-    with _device_of(q):
-        scratch = _scratch(plan._scratch[0], q.device)
-        c = _cross_call(q, k, v, plan, mask, scale, scratch)
-        _lib.check(_lib.lib().mignn_cross_attn_forward(
-            ctypes.addressof(c), P(out), P(out32), P(lse), _lib.stream(q.device)),
-            "mignn_cross_attn_forward")
+    scratch = _scratch(plan._scratch[0], q.device)
+    c = _cross_call(q, k, v, plan, mask, scale, scratch)
+    _launch(_lib.lib().mignn_cross_attn_forward, "mignn_cross_attn_forward", q.device.index,
+            ctypes.addressof(c), out.data_ptr(), P(out32), P(lse))
     return out, (out if out32 is None else out32), lse
 
 
@@ -394,8 +406,7 @@ class _CrossAttention(Function):
         ctx.save_for_backward(q, k, v, mask, out32, lse)
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         q, k, v, mask, out32, lse = ctx.saved_tensors
         plan = ctx.plan
@@ -406,13 +417,12 @@ class _CrossAttention(Function):
             dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
             dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
         delta = torch.empty_like(lse)
-        with _device_of(q):
-            scratch = _scratch(plan._scratch[1], q.device)
-            c = _cross_call(q, k, v, plan, mask, ctx.scale, scratch)
-            _lib.check(_lib.lib().mignn_cross_attn_backward(
-                ctypes.addressof(c), P(dout), dout.stride(0), dout.stride(1), P(out32), P(lse),
-                P(delta), P(dq), P(dk), P(dv), _lib.stream(q.device)),
-                "mignn_cross_attn_backward")
+        scratch = _scratch(plan._scratch[1], q.device)
+        c = _cross_call(q, k, v, plan, mask, ctx.scale, scratch)
+        _launch(_lib.lib().mignn_cross_attn_backward, "mignn_cross_attn_backward",
+                q.device.index, ctypes.addressof(c), dout.data_ptr(), dout.stride(0),
+                dout.stride(1), out32.data_ptr(), lse.data_ptr(), delta.data_ptr(),
+                dq.data_ptr(), P(dk), P(dv))
         need = ctx.needs_input_grad
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None,
                 None, None)
@@ -450,3 +460,102 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Cro
             raise ValueError("cross_attention: gradients need a plan built with train=True")
         return _CrossAttention.apply(q, k, v, plan, key_mask, scale)
     return _cross_forward(q, k, v, plan, key_mask, scale, False)[0]
+
+
+# ---------------------------------------------------------------------------
+# The block
+
+def graph_lengths(batch: Optional[torch.Tensor], num_nodes: int, num_graphs: Optional[int] = None):
+    """Rows of each graph of a `Batch` (its `batch` vector, sorted as
+    `Batch.from_data_list` makes it); one graph without a vector.  Reads the
+    vector on the host."""
+    if batch is None:
+        return [num_nodes]
+    b = batch.detach().cpu()
+    if b.numel() != num_nodes or (b.numel() > 1 and bool((b[1:] < b[:-1]).any())):
+        raise ValueError("graph_lengths: batch must be a sorted vector, one entry a row")
+    return torch.bincount(b, minlength=num_graphs or 0).tolist()
+
+
+class CrossAttention(nn.Module):
+    """Rows of one graph read the states of another:
+
+        q = turn(Wq norm(x)),  k = turn(Wk norm(context)),  v = Wv norm(context)
+        (y, s) = norm(Wo attend(q, k, v), residual=x)
+
+    `turn` is `rotary` by the rows' positions (cell centres), so that scores
+    depend on where the cells lie to each other.  Returns (y, s): the normed
+    rows and the stream s = x + the attention's output.  fp32, on the device;
+    differentiable in the rows, the context and the parameters."""
+
+    def __init__(self, hidden_dim: int, heads: int = 4, kv_heads: Optional[int] = None,
+                 axes: int = 3, base: float = 100.0, position_scale: float = 64.0,
+                 eps: float = 1e-6):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if heads < 1 or hidden_dim % heads or kv_heads < 1 or heads % kv_heads:
+            raise ValueError(f"CrossAttention: hidden_dim {hidden_dim} over {heads} heads, "
+                             f"{kv_heads} key heads")
+        d = hidden_dim // heads
+        if d % 8 or d > _lib.CROSS_MAX_D:
+            raise ValueError(f"CrossAttention: head width {d} must be a multiple of 8 up to "
+                             f"{_lib.CROSS_MAX_D}")
+        if not 1 <= axes <= d // 2:
+            raise ValueError(f"CrossAttention: {axes} position axes for heads of width {d}")
+        self.hidden_dim, self.heads, self.kv_heads, self.head_dim = hidden_dim, heads, kv_heads, d
+        self.axes, self.base, self.position_scale = axes, base, position_scale
+        self.eps = eps
+        self.norm_x = nn.Parameter(torch.ones(hidden_dim))
+        self.norm_context = nn.Parameter(torch.ones(hidden_dim))
+        self.norm_out = nn.Parameter(torch.ones(hidden_dim))
+        self.lin_query = nn.Linear(hidden_dim, heads * d)
+        self.lin_key = nn.Linear(hidden_dim, kv_heads * d)
+        self.lin_value = nn.Linear(hidden_dim, kv_heads * d)
+        self.lin_out = nn.Linear(heads * d, hidden_dim)
+        self._axes = None
+
+    def plan(self, q_lens, k_lens, train: bool = True, device="cuda") -> CrossPlan:
+        """The work lists for rows and context rows per graph."""
+        return CrossPlan(q_lens, k_lens, heads=self.heads, kv_heads=self.kv_heads,
+                         head_dim=self.head_dim, device=device, train=train)
+
+    def _rotary_axes(self, device) -> RotaryAxes:
+        if self._axes is None or self._axes.device != device:
+            half = self.head_dim // 2
+            pairs = [half // self.axes + (a < half % self.axes) for a in range(self.axes)]
+            self._axes = RotaryAxes(pairs, base=self.base,
+                                    scales=(self.position_scale,) * self.axes, device=device)
+        return self._axes
+
+    def keys_values(self, context: torch.Tensor, context_pos: torch.Tensor):
+        """(k, v) of the context rows: computed once for many `attend` calls."""
+        n = context.shape[0]
+        h = rms_norm(context, self.norm_context, eps=self.eps)
+        k = T.linear(h, self.lin_key.weight, self.lin_key.bias)
+        v = T.linear(h, self.lin_value.weight, self.lin_value.bias)
+        k = rotary(k.view(n, self.kv_heads, self.head_dim), context_pos[:, :self.axes],
+                   self._rotary_axes(context.device))
+        return k, v.view(n, self.kv_heads, self.head_dim)
+
+    def attend(self, x: torch.Tensor, pos: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+               plan: CrossPlan, key_mask: Optional[torch.Tensor] = None):
+        """(y, s) of rows x at positions pos [N, >= axes] over given keys and values."""
+        n = x.shape[0]
+        q = T.linear(rms_norm(x, self.norm_x, eps=self.eps), self.lin_query.weight,
+                     self.lin_query.bias)
+        q = rotary(q.view(n, self.heads, self.head_dim), pos[:, :self.axes],
+                   self._rotary_axes(x.device))
+        o = cross_attention(q, k, v, plan, key_mask=key_mask)
+        o = T.linear(o.reshape(n, self.heads * self.head_dim), self.lin_out.weight,
+                     self.lin_out.bias)
+        return rms_norm(o, self.norm_out, residual=x, eps=self.eps)
+
+    def forward(self, x, pos, context, context_pos, plan: CrossPlan,
+                key_mask: Optional[torch.Tensor] = None):
+        for name, t in (("x", x), ("context", context)):
+            if t.dim() != 2 or t.shape[1] != self.hidden_dim or t.dtype != torch.float32:
+                raise ValueError(f"CrossAttention: {name} must be float32 [N, {self.hidden_dim}], "
+                                 f"got {t.dtype} {tuple(t.shape)}")
+        _on_device("CrossAttention", x, context=context, parameters=self.norm_x)
+        k, v = self.keys_values(context, context_pos)
+        return self.attend(x, pos, k, v, plan, key_mask)

@@ -48,6 +48,7 @@ import torch.nn as nn
 
 from . import _lib
 from . import train_ops as T
+from .attention import CrossAttention, graph_lengths
 from ._lib import (CSR_ONE_SELF_LOOP, CSR_TRANSPOSE, CSR_VERBATIM, EPI_AFFINE, EPI_BIAS, EPI_RELU,
                    EPI_RESIDUAL)
 
@@ -1340,10 +1341,17 @@ class FlowGNN(nn.Module):
 
 
 class FlowGNNSurrogate(nn.Module):
-    """Encoder/decoder composition of FlowGNN (reference gnn_model.py:223-291)."""
+    """Encoder/decoder composition of FlowGNN (reference gnn_model.py:223-291).
+
+    cross_heads > 0 adds, between encoder and decoder, cross attention to the
+    encoder's states of a second graph (`context` of the forward: a coarser or
+    wider mesh of the same flow, any size): every node reads every context node
+    of its graph, where the convolutions carry information one edge a layer.
+    With the default 0 the model and its state_dict are the reference's."""
 
     def __init__(self, input_dim: int = 3, hidden_dim: int = 128, num_layers: int = 4,
-                 layer_type: str = "GCN", use_edge_attr: bool = True, dropout: float = 0.1):
+                 layer_type: str = "GCN", use_edge_attr: bool = True, dropout: float = 0.1,
+                 cross_heads: int = 0):
         super().__init__()
         self.encoder = FlowGNN(input_dim=input_dim, hidden_dim=hidden_dim, output_dim=hidden_dim,
                                num_layers=num_layers // 2, layer_type=layer_type,
@@ -1351,9 +1359,30 @@ class FlowGNNSurrogate(nn.Module):
         self.decoder = FlowGNN(input_dim=hidden_dim, hidden_dim=hidden_dim, output_dim=8,
                                num_layers=num_layers // 2, layer_type=layer_type,
                                use_edge_attr=use_edge_attr, dropout=dropout)
+        self.cross = CrossAttention(hidden_dim, cross_heads, axes=min(3, input_dim)) \
+            if cross_heads else None
 
-    def forward(self, x, edge_index, edge_attr=None, boundary_conditions=None):
+    def forward(self, x, edge_index, edge_attr=None, boundary_conditions=None, context=None,
+                batch=None, plan=None):
+        """context (only with cross_heads > 0, and then required): the second
+        graph, a `Data` / `Batch` whose x has the nodes' features; batch: the
+        nodes' graph of each row when there are several (context.batch then
+        too); plan: `self.cross.plan(...)` of the two graphs' sizes, built here
+        when not given."""
+        if (context is None) != (self.cross is None):
+            raise ValueError("FlowGNNSurrogate: context is for cross_heads > 0, which needs it")
         encoded = self.encoder(x, edge_index, edge_attr)
+        if context is not None:
+            states = self.encoder(context.x, context.edge_index, context.edge_attr)
+            if plan is None:
+                context_batch = getattr(context, "batch", None)
+                if (batch is None) != (context_batch is None):
+                    raise ValueError("FlowGNNSurrogate: batch and context.batch go together")
+                kl = graph_lengths(context_batch, context.x.shape[0])
+                ql = graph_lengths(batch, x.shape[0], len(kl))
+                kl += [0] * (len(ql) - len(kl))
+                plan = self.cross.plan(ql, kl, train=torch.is_grad_enabled(), device=x.device)
+            encoded, _ = self.cross(encoded, x.detach(), states, context.x.detach(), plan)
         if boundary_conditions is not None:
             encoded = encoded + boundary_conditions
         return self.decoder(encoded, edge_index, edge_attr)

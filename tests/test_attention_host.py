@@ -63,6 +63,7 @@ def test_cross_plan_refusals():
             ([1.5], [2], ok, ValueError, "whole numbers"),
             ([1], [1], dict(ok, kv_heads=3), ValueError, "4 query heads over 3"),
             ([1], [1], dict(ok, heads=0), ValueError, "0 query heads"),
+            ([1], [1], dict(ok, heads=65, kv_heads=1), ValueError, "more than 64"),
             ([1], [1], dict(ok, head_dim=12), ValueError, "head_dim"),
             ([1], [1], dict(ok, head_dim=136), ValueError, "head_dim"),
             ([1], [1], dict(ok, head_dim=0), ValueError, "head_dim"),
@@ -235,3 +236,36 @@ def test_oracle_gradients_match_differences():
         back = orc.rotary(orc.rotary(u, pos, (3, 2), interleaved=il), pos, (3, 2), interleaved=il,
                           inverse=True)
         assert (back - u).abs().max() < 1e-12
+
+
+def test_block_and_surrogate_refusals():
+    from mignn import Data, FlowGNNSurrogate
+    for args in [(30, 4), (64, 0), (64, 3), (512, 2), (64, 16)]:
+        with pytest.raises(ValueError, match="CrossAttention"):
+            A.CrossAttention(*args)
+    with pytest.raises(ValueError, match="position axes"):
+        A.CrossAttention(32, 4, axes=5)
+    blk = A.CrossAttention(64, 4)
+    plan = blk.plan([3], [2], device="cpu")
+    x, c = torch.zeros(3, 64), torch.zeros(2, 64)
+    with pytest.raises(ValueError, match="context must be"):
+        blk(x, x[:, :3], c[:, :32], c[:, :3], plan)
+    with pytest.raises(RuntimeError, match="ROCm devices only"):
+        blk(x, x[:, :3], c, c[:, :3], plan)
+    ei = torch.zeros(2, 1, dtype=torch.long)
+    ctx = Data(x=torch.zeros(2, 3), edge_index=ei)
+    with pytest.raises(ValueError, match="context is for"):
+        FlowGNNSurrogate(hidden_dim=32)(torch.zeros(3, 3), ei, context=ctx)
+    with pytest.raises(ValueError, match="context is for"):
+        FlowGNNSurrogate(hidden_dim=32, cross_heads=4)(torch.zeros(3, 3), ei)
+    # the default model has the reference's parameters and no more
+    assert not [k for k in FlowGNNSurrogate(hidden_dim=32).state_dict() if k.startswith("cross")]
+
+
+def test_graph_lengths():
+    assert A.graph_lengths(None, 7) == [7]
+    assert A.graph_lengths(torch.tensor([0, 0, 2]), 3, 4) == [2, 0, 1, 0]
+    assert A.graph_lengths(torch.zeros(0, dtype=torch.long), 0, 2) == [0, 0]
+    for bad in (torch.tensor([1, 0]), torch.tensor([0])):
+        with pytest.raises(ValueError, match="sorted"):
+            A.graph_lengths(bad, 2)

@@ -468,3 +468,132 @@ def test_operators_in_captured_graphs():
         for i in (0, 1):
             for a, b in zip(outs[i], step(states[i])):
                 assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# the operators together: the block and the surrogate that calls it
+
+def block_oracle(blk, x, pos, context, cpos, ql, kl, mask=None):
+    """CrossAttention.forward in float64 (autograd through it gives its gradients)."""
+    def norm(t, w):
+        return t / torch.sqrt((t * t).mean(1, keepdim=True) + blk.eps) * w
+    p = {n: t.detach().double().cpu().requires_grad_() for n, t in blk.named_parameters()}
+    x, context = (t.detach().double().cpu().requires_grad_() for t in (x, context))
+    half, d = blk.head_dim // 2, blk.head_dim
+    pairs = [half // blk.axes + (a < half % blk.axes) for a in range(blk.axes)]
+
+    def turn(t, ps):
+        ang = torch.stack([ps[:, a].double().cpu() * blk.position_scale * blk.base ** (-i / m)
+                           for a, m in enumerate(pairs) for i in range(m)], 1)[:, None]
+        u, v = t[..., :half], t[..., half:]
+        return torch.cat([u * ang.cos() - v * ang.sin(), v * ang.cos() + u * ang.sin()], 2)
+    lin = lambda t, n: t @ p[n + ".weight"].T + p[n + ".bias"]  # noqa: E731
+    q = turn(lin(norm(x, p["norm_x"]), "lin_query").view(-1, blk.heads, d), pos)
+    c = norm(context, p["norm_context"])
+    k = turn(lin(c, "lin_key").view(-1, blk.kv_heads, d), cpos)
+    v = lin(c, "lin_value").view(-1, blk.kv_heads, d)
+    g, rows, qa, ka = blk.heads // blk.kv_heads, [], 0, 0
+    for lq, lk in zip(ql, kl):
+        keep = torch.arange(ka, ka + lk)
+        if mask is not None:
+            keep = keep[mask.cpu()[ka:ka + lk]]
+        heads = [torch.softmax(q[qa:qa + lq, h] @ k[keep, h // g].T / math.sqrt(d), 1)
+                 @ v[keep, h // g] if keep.numel() else 0.0 * q[qa:qa + lq, h]
+                 for h in range(blk.heads)]
+        rows.append(torch.cat(heads, 1))
+        qa, ka = qa + lq, ka + lk
+    s = x + lin(torch.cat(rows), "lin_out")
+    return norm(s, p["norm_out"]), s, x, context, p
+
+
+@pytest.mark.parametrize("kv", [4, 2])
+@pytest.mark.parametrize("ql,kl,masked", [([150, 33], [40, 300], False), ([70, 5, 9], [64, 0, 31], True),
+                                          ([1], [500], False)])
+def test_block(ql, kl, kv, masked):
+    """norm, projections, rotation, attention and the residual's norm in one
+    run: outputs and every gradient against the float64 block.  Bound: each of
+    the ~8 steps loses what its own test grants (at most (h + L + 64) u of its
+    magnitude, widths 64, L <= 300), through weights of norm about 1: 2^-24 *
+    8 * 512 = 2^-12 of the largest value of the tensor."""
+    blk = A.CrossAttention(64, 4, kv)
+    g = torch.Generator().manual_seed(1)
+    with torch.no_grad():
+        for n, t in blk.named_parameters():
+            t.copy_(torch.randn(t.shape, generator=g) * (0.1 if t.dim() == 1 else 0.125)
+                    + (1.0 if n.startswith("norm") else 0.0))
+    blk = blk.to(DEV)
+    x, ctx = rnd(sum(ql), 64, seed=2).requires_grad_(), rnd(sum(kl), 64, seed=3).requires_grad_()
+    pos = torch.rand(sum(ql), 3, generator=g).to(DEV)
+    cpos = torch.rand(sum(kl), 3, generator=g).to(DEV)
+    mask = (torch.rand(sum(kl), generator=g) < 0.7).to(DEV) if masked else None
+    plan = blk.plan(ql, kl)
+    y, s = blk(x, pos, ctx, cpos, plan, key_mask=mask)
+    dy, ds = rnd(*y.shape, seed=4), rnd(*y.shape, seed=5)
+    names, params = zip(*blk.named_parameters())
+    grads = torch.autograd.grad((y, s), (x, ctx) + params, (dy, ds))
+    ry, rs, rx, rc, rp = block_oracle(blk, x, pos, ctx, cpos, ql, kl, mask)
+    ref = torch.autograd.grad((ry, rs), (rx, rc) + tuple(rp[n] for n in names),
+                              (dy.double().cpu(), ds.double().cpu()))
+    for name, a, b in [("y", y, ry), ("s", s, rs)] + list(zip(("x", "context") + names, grads, ref)):
+        err = (a.detach().double().cpu() - b.detach()).abs().max().item()
+        assert err <= 2.0 ** -12 * max(b.abs().max().item(), 1e-3), (name, err)
+    with torch.no_grad():
+        k, v = blk.keys_values(ctx, cpos)
+        y2, s2 = blk.attend(x, pos, k, v, plan, mask)
+    assert (y2 - y).abs().max() <= 2.0 ** -12 * y.abs().max()
+    assert (s2 - s).abs().max() <= 2.0 ** -12 * s.abs().max()
+
+
+def grid(nx, ny, nz, seed=0):
+    from mignn.synthetic import grid_graph
+    return grid_graph(nx, ny, nz, device=DEV, permute_seed=seed)
+
+
+@pytest.mark.parametrize("layer_type", ["GCN", "GAT"])
+def test_surrogate_with_context(layer_type):
+    """FlowGNNSurrogate(cross_heads): eval forward equals its parts run by hand,
+    a training step reaches every parameter, and the context's nodes matter."""
+    from mignn import Data, FlowGNNSurrogate
+    m = FlowGNNSurrogate(hidden_dim=64, num_layers=4, layer_type=layer_type, dropout=0.0,
+                         cross_heads=4).to(DEV)
+    x, ei = grid(8, 6, 5)
+    cx, cei = grid(4, 3, 3, seed=1)
+    ctx = Data(x=cx, edge_index=cei)
+    m.eval()
+    with torch.no_grad():
+        y = m(x, ei, context=ctx)
+        enc, states = m.encoder(x, ei), m.encoder(cx, cei)
+        plan = m.cross.plan([x.shape[0]], [cx.shape[0]], train=False)
+        h, _ = m.cross(enc, x, states, cx, plan)
+        assert torch.equal(y, m.decoder(h, ei))
+        assert torch.equal(y, m(x, ei, context=ctx, plan=plan))
+        assert not torch.equal(y, m(x, ei, context=Data(x=cx[:20], edge_index=cei[:, :0])))
+    m.train()
+    out = m(x, ei, context=ctx)
+    out.square().mean().backward()
+    missing = [n for n, p in m.named_parameters() if p.grad is None or not p.grad.abs().sum() > 0]
+    # (an attention output bias or a layer's bias ahead of a batch norm may have gradient 0)
+    assert not [n for n in missing if "bias" not in n], missing
+
+
+def test_surrogate_batch_of_graphs_reads_its_own_context():
+    """Two graphs with contexts of unlike size in one batch: each graph's
+    attention equals that of the graph alone."""
+    from mignn import Batch, Data
+    blk = A.CrossAttention(64, 4).to(DEV)
+    graphs = [grid(5, 4, 3), grid(4, 4, 4, seed=2)]
+    ctxs = [grid(3, 3, 3, seed=3), grid(6, 3, 3, seed=4)]
+    b = Batch.from_data_list([Data(x=x.cpu(), edge_index=e.cpu()) for x, e in graphs])
+    cb = Batch.from_data_list([Data(x=x.cpu(), edge_index=e.cpu()) for x, e in ctxs])
+    ql = A.graph_lengths(b.batch, b.num_nodes)
+    kl = A.graph_lengths(cb.batch, cb.num_nodes)
+    assert ql == [60, 64] and kl == [27, 54]
+    h, c = rnd(124, 64, seed=1), rnd(81, 64, seed=2)
+    with torch.no_grad():
+        y, _ = blk(h, b.x.to(DEV), c, cb.x.to(DEV), blk.plan(ql, kl))
+        a0 = c0 = 0
+        for n, k in zip(ql, kl):
+            one, _ = blk(h[a0:a0 + n], b.x[a0:a0 + n].to(DEV), c[c0:c0 + k], cb.x[c0:c0 + k].to(DEV),
+                         blk.plan([n], [k]))
+            assert (one - y[a0:a0 + n]).abs().max() <= 2.0 ** -12 * y.abs().max()
+            a0, c0 = a0 + n, c0 + k
