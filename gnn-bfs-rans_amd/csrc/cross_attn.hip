@@ -18,7 +18,7 @@
 // atomically and results do not depend on the order of workgroups.  The query
 // heads that share a kv head are rows of one tile: their keys are read once,
 // and dk, dv sum over them in place.
-#include "cross_attn.hpp"
+#include "mfma16.hpp"
 
 #include <cstdlib>
 
@@ -83,22 +83,6 @@ __device__ __forceinline__ void add_tile(const float* tile, const f32x16& w, f32
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b)
             acc[b] = mfma32(p[acc_row(r) * (DP + 4) + 32 * b], w[r], acc[b]);
-}
-
-template <typename T, int DP>
-__device__ __forceinline__ void store_acc(T* p, const f32x16 (&acc)[DP / 32], float f, int d,
-                                          int half) {
-#pragma unroll
-    for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int c = 32 * b + 8 * g + 4 * half;
-            if (c < d) {
-                const float o[4] = {acc[b][4 * g] * f, acc[b][4 * g + 1] * f, acc[b][4 * g + 2] * f,
-                                    acc[b][4 * g + 3] * f};
-                store_row(p + c, o);
-            }
-        }
 }
 
 struct RowRef {
@@ -540,6 +524,7 @@ int run_pass(CrossArgs a, const mignn_cross_pass& ps, int pass, int dtype, hipSt
     if (a.n_items > 0) {
         int rc;
         if (a.tile == CROSS_FEW) rc = cross_few(a, dtype, st);
+        else if (dtype == MIGNN_ROW_F32 && pass == MIGNN_CROSS_FORWARD && a.tile == 128) rc = cross_forward32(a, st);
         else if (dtype == MIGNN_ROW_F32) rc = cross_pass_exact(a, pass, st);
         else rc = cross_pass16(a, pass, dtype, st);
         if (rc) return rc;

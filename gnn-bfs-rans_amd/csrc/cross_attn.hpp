@@ -102,6 +102,8 @@ __device__ __forceinline__ float4 load4(const T* p) {
 
 // the 16-bit rows' kernels of a pass (cross_attn16.hip)
 int cross_pass16(const CrossArgs& a, int pass, int dtype, hipStream_t st);
+// the forward of fp32 rows in 128-row tiles (cross_attn32.hip)
+int cross_forward32(const CrossArgs& a, hipStream_t st);
 // the forward of up to CROSS_FEW rows a sequence (cross_decode.hip)
 int cross_few(const CrossArgs& a, int dtype, hipStream_t st);
 

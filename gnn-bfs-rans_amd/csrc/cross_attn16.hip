@@ -10,9 +10,7 @@
 //                       group);  B = P^T, the accumulator of S^T rounded in
 //                       place: the product over keys takes them in the order
 //                       in which its registers hold them
-// dq and dk / dv are made of the same two forms.  Row pitch: the tile's width
-// plus 32 bytes, so that neither 8 rows' 16-byte reads nor 4 rows' transposed
-// reads meet in a bank.
+// dq and dk / dv are made of the same two forms.
 //
 // P and dS are rounded to the rows' type ahead of their second product (the
 // matrix instruction takes both operands in one type); statistics, sums and
@@ -20,57 +18,12 @@
 // 1 / 5000 is already subnormal there, so P is carried up by a constant power
 // of two and dS by one that each row (dq) or key (dk) lowers when its values
 // would not fit (DsScale); the results are brought back in fp32.
-#include "cross_attn.hpp"
+#include "mfma16.hpp"
 
 namespace mignn {
 namespace {
 
-template <typename T>
-using vec8 = T __attribute__((ext_vector_type(8)));
-template <typename T>
-using vec2 = T __attribute__((ext_vector_type(2)));
-using s16x4 = __attribute__((ext_vector_type(4))) short;
-using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
-using lds_s16x4 = __attribute__((address_space(3))) s16x4;
-
-__device__ __forceinline__ f32x16 mfma16(vec8<bf16_t> a, vec8<bf16_t> b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mfma16(vec8<f16_t> a, vec8<f16_t> b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
 constexpr int KT = CROSS_STAGE;
-
-template <int DP>
-constexpr int pitch() { return DP * 2 + 32; }
-
-// the transposed read's share of a lane: row 4 half + (l % 16) / 4, columns
-// 16 ((l / 16) % 2) + 4 (l % 4) ..+3
-template <int DP>
-__device__ __forceinline__ int tr_lane(int lane) {
-    return (4 * (lane >> 5) + ((lane & 15) >> 2)) * pitch<DP>() + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
-}
-
-// A operand of a product over rows 16 t + (the accumulator's order) of a tile:
-// columns 32 b + l % 32
-template <typename T, int DP>
-__device__ __forceinline__ vec8<T> tr_frag(const char* tile, int trl, int row, int b) {
-    const char* p = tile + trl + row * pitch<DP>() + 64 * b;
-    union {
-        s16x4 h[2];
-        vec8<T> v;
-    } u;
-    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * pitch<DP>()));
-    return u.v;
-}
-
-// A operand of a product over columns: row r + l % 32, columns 16 i + 8 half ..+7
-template <typename T, int DP>
-__device__ __forceinline__ vec8<T> row_frag(const char* tile, int r, int i, int col, int half) {
-    return *reinterpret_cast<const vec8<T>*>(tile + (r + col) * pitch<DP>() + 32 * i + 16 * half);
-}
 
 // B operand rows held in registers
 template <typename T, int DP>
@@ -136,46 +89,6 @@ struct Stage {
     }
 };
 
-// Which of the 64 keys from key0 on take part (bit = key), for every lane: the
-// mask's byte is loaded ahead of the rows it goes with and looked at when they
-// are (a comparison at the load would wait for every load before it)
-struct KeyBits {
-    uint32_t byte;
-    int left;
-    __device__ __forceinline__ void load(const CrossArgs& a, int64_t key0, int n, int lane) {
-        left = n;
-        byte = 1u;
-        if (a.mask) byte = a.mask[key0 + (lane < n ? lane : n - 1)];
-    }
-    __device__ __forceinline__ uint64_t bits(int lane) const {
-        return __builtin_amdgcn_ballot_w64(lane < left && byte != 0u);
-    }
-};
-
-__device__ __forceinline__ float swap_max(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float swap_add(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-template <typename T, int DP>
-__device__ __forceinline__ void store_acc16(T* p, const f32x16 (&acc)[DP / 32], float f, int d, int half) {
-#pragma unroll
-    for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int c = 32 * b + 8 * g + 4 * half;
-            if (c < d) {
-                const float o[4] = {acc[b][4 * g] * f, acc[b][4 * g + 1] * f, acc[b][4 * g + 2] * f,
-                                    acc[b][4 * g + 3] * f};
-                store_row(p + c, o);
-            }
-        }
-}
-
 // fp16's P is kept 2^8 up: a weight down to 2^-22 of the largest keeps its
 // full precision, and 2^(8 + 6) stays below fp16's largest.  bf16 has fp32's
 // range.
@@ -183,9 +96,6 @@ template <typename T>
 constexpr float P_UP = 0.f;
 template <>
 constexpr float P_UP<f16_t> = 8.f;
-// the running maximum is raised when a score passes it by this power of two
-constexpr float MAX_SLACK = 6.f;
-
 template <typename T>
 constexpr bool NARROW = sizeof(T) == 2 && !__is_same(T, bf16_t);
 // P's power of two in the dk / dv kernel, where it is at most 1
@@ -348,14 +258,14 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_fwd16_kernel(CrossArgs a) {
         if (it.slot >= 0) {
             float* p = a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
                                  row[cb] - it.r0) * (a.d + 2);
-            store_acc16<float, DP>(p, o[cb], 1.f, a.d, half);
+            store_acc<float, DP>(p, o[cb], 1.f, a.d, half);
             if (half == 0) p[a.d] = m[cb] == -INFINITY ? -INFINITY : m2;
             else p[a.d + 1] = sum;
             continue;
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        store_acc16<T, DP>(static_cast<T*>(a.out) + at[cb] * a.d, o[cb], inv, a.d, half);
-        if (a.o32) store_acc16<float, DP>(a.o32 + at[cb] * a.d, o[cb], inv, a.d, half);
+        store_acc<T, DP>(static_cast<T*>(a.out) + at[cb] * a.d, o[cb], inv, a.d, half);
+        if (a.o32) store_acc<float, DP>(a.o32 + at[cb] * a.d, o[cb], inv, a.d, half);
         if (a.lse && half == 0) a.lse[at[cb]] = sum == 0.f ? INFINITY : m2 + log2f(sum);
     }
 }
@@ -491,10 +401,10 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_dq16_kernel(CrossArgs a) {
         if (row[cb] >= it.r1) continue;
         const float f = a.scale * sc[cb].back();
         if (it.slot >= 0)
-            store_acc16<float, DP>(a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
+            store_acc<float, DP>(a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
                                              row[cb] - it.r0) * a.d, acc[cb], f, a.d, half);
         else
-            store_acc16<T, DP>(static_cast<T*>(a.out) + at[cb] * a.d, acc[cb], f, a.d, half);
+            store_acc<T, DP>(static_cast<T*>(a.out) + at[cb] * a.d, acc[cb], f, a.d, half);
     }
 }
 
@@ -633,12 +543,12 @@ __global__ __launch_bounds__(NW * 64, DP <= 96 ? 2 : 1) void cross_dkv16_kernel(
         if (it.slot >= 0) {
             float* p = a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
                                  key[cb] - it.r0) * (2 * a.d);
-            store_acc16<float, DP>(p, dk[cb], fk, a.d, half);
-            store_acc16<float, DP>(p + a.d, dv[cb], fv, a.d, half);
+            store_acc<float, DP>(p, dk[cb], fk, a.d, half);
+            store_acc<float, DP>(p + a.d, dv[cb], fv, a.d, half);
         } else {
             const int64_t at = ((it.k_begin + static_cast<int64_t>(key[cb])) * a.kv_heads + kvh) * a.d;
-            store_acc16<T, DP>(static_cast<T*>(a.dk) + at, dk[cb], fk, a.d, half);
-            store_acc16<T, DP>(static_cast<T*>(a.dv) + at, dv[cb], fv, a.d, half);
+            store_acc<T, DP>(static_cast<T*>(a.dk) + at, dk[cb], fk, a.d, half);
+            store_acc<T, DP>(static_cast<T*>(a.dv) + at, dv[cb], fv, a.d, half);
         }
     }
 }
