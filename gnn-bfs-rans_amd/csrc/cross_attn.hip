@@ -20,6 +20,7 @@
 // and dk, dv sum over them in place.
 #include "mfma16.hpp"
 
+#include <algorithm>
 #include <cstdlib>
 
 namespace mignn {
@@ -105,7 +106,7 @@ template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64) void cross_fwd_kernel(CrossArgs a) {
     __shared__ __attribute__((aligned(16))) float ks[32 * (DP + 4)], vs[32 * (DP + 4)];
     int item, kvh;
-    if (!cross_work(a, a.n_items, item, kvh)) return;
+    if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int row = it.r0 + wave * 32 + col;
@@ -233,7 +234,7 @@ template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(CrossArgs a) {
     __shared__ __attribute__((aligned(16))) float ks[32 * (DP + 4)], vs[32 * (DP + 4)];
     int item, kvh;
-    if (!cross_work(a, a.n_items, item, kvh)) return;
+    if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int row = it.r0 + wave * 32 + col;
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(NW * 64) void cross_dkv_kernel(CrossArgs a) {
     __shared__ __attribute__((aligned(16))) float qs[32 * (DP + 4)], gs[32 * (DP + 4)];
     __shared__ __attribute__((aligned(16))) float ls[32], ds[32];
     int item, kvh;
-    if (!cross_work(a, a.n_items, item, kvh)) return;
+    if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int key = it.r0 + wave * 32 + col;
@@ -398,79 +399,113 @@ __global__ __launch_bounds__(256) void cross_join_grad_kernel(CrossArgs a, bool 
 
 // Tiles of the "r" side (rows or keys) times chunks of the "c" side.
 struct PassShape {
-    int tile;        // rows of a tile
-    int64_t longest; // of the r side
-    int64_t chunk;
-    int64_t unit;    // chunks are a multiple of it
+    int64_t tile;     // rows of a tile
+    int64_t longest;  // of the r side
+    int64_t slots;    // workgroups that the card holds at a time
+    int64_t least;    // shortest chunk: below it a part's join costs what the split gains
+    int64_t unit;     // chunks are a multiple of it
 };
 struct PassPlan {
-    int64_t items = 0, joins = 0, slots = 0;
+    int64_t items = 0, whole = 0, joins = 0, slots = 0;
+};
+struct Sequence {
+    int64_t rn, cn, qb, kb;   // r and c side, first query and key
 };
 
-// Tile: 8 rows where no sequence has more (forward: cross_few), 32 where none
-// has more than 32 (one wave: more workgroups, and three waves of four would
-// idle), else 128.
-// Chunk: the pass should have `target` workgroups (two for each of the 256
-// CUs, eight small ones) when its tiles alone are fewer; not under `least`,
-// where the parts' join would cost what the split gains.
-PassShape pass_shape(const int64_t* rows, const int64_t* keys, int64_t batch, int pass, int kv_heads,
-                     int group) {
+int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
+
+// Tile: 8 rows where no sequence has more (forward: cross_few).  Else 128, four
+// waves that share the staging of the other side, or 32, one wave, where
+// padding to 128 would add a quarter to the work (few rows, or many short
+// sequences: three snapshots' 64..257 states as keys, fp32 dk / dv 112 us in
+// tiles of 128).
+PassShape pass_shape(const Sequence* seq, int64_t batch, int pass, int d, int dtype, int group) {
     const bool dkv = pass == MIGNN_CROSS_DKV;
-    // (dk / dv: whole queries, as many as an LDS tile holds)
-    PassShape s{128, 0, 0, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
+    PassShape s{128, 0, 512, 256, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
+    double w32 = 0.0, w128 = 0.0;
     for (int64_t b = 0; b < batch; ++b) {
-        const int64_t r = dkv ? keys[b] : rows[b];
-        if (r > s.longest) s.longest = r;
+        if (seq[b].rn > s.longest) s.longest = seq[b].rn;
+        w32 += static_cast<double>(up(seq[b].rn, 32)) * static_cast<double>(seq[b].cn);
+        w128 += static_cast<double>(up(seq[b].rn, 128)) * static_cast<double>(seq[b].cn);
     }
     if (pass == MIGNN_CROSS_FORWARD && s.longest <= CROSS_FEW) s.tile = CROSS_FEW;
-    else if (s.longest <= CROSS_ROWS) s.tile = CROSS_ROWS;
-    double work = 0.0;
-    for (int64_t b = 0; b < batch; ++b) {
-        const int64_t r = dkv ? keys[b] : rows[b], c = dkv ? rows[b] : keys[b];
-        work += static_cast<double>((r + s.tile - 1) / s.tile) * static_cast<double>(c);
-    }
-    const int64_t target = s.tile == 128 ? 512 : 2048, least = s.tile == 128 ? 256 : 128;
-    s.chunk = static_cast<int64_t>(work * kv_heads / static_cast<double>(target));
-    if (s.chunk < least) s.chunk = least;
-    s.chunk = (s.chunk + s.unit - 1) / s.unit * s.unit;
+    else if (s.longest <= 32 || w128 > 1.25 * w32) s.tile = 32;
+    // registers and LDS: two workgroups of four waves a CU, one where the heads
+    // are wide and much is held in fp32; eight small ones
+    const bool wide = dtype == MIGNN_ROW_F32 ? d > 64 : dkv && d > 96;
+    if (s.tile != 128) s.slots = 2048, s.least = 128;
+    else if (wide) s.slots = 256;
     return s;
 }
 
-PassPlan plan_pass(const PassShape& shape, const int64_t* rows, const int64_t* queries, const int64_t* keys,
-                   int64_t batch, bool dkv, CrossItem* items, CrossJoin* joins) {
-    const int64_t chunk = shape.chunk, tile = shape.tile;
+// The chunk length that ends first when the tiles are fewer than the slots:
+// rounds of `slots` workgroups, each a chunk and the cost of starting one
+int64_t pick_chunk(const PassShape& s, const Sequence* seq, int64_t batch, int kv_heads) {
+    int64_t longest = 0;
+    for (int64_t b = 0; b < batch; ++b) longest = seq[b].cn > longest ? seq[b].cn : longest;
+    int64_t best = up(longest > 0 ? longest : 1, s.unit);
+    double best_cost = -1.0;
+    for (int64_t parts = 1; parts <= 256; ++parts) {
+        const int64_t len = up((longest + parts - 1) / parts, s.unit);
+        if (parts > 1 && len < s.least) break;
+        double items = 0.0;
+        for (int64_t b = 0; b < batch; ++b)
+            if (seq[b].cn > 0)
+                items += static_cast<double>((seq[b].rn + s.tile - 1) / s.tile) *
+                         static_cast<double>((seq[b].cn + len - 1) / len);
+        const int64_t rounds = (static_cast<int64_t>(items) * kv_heads + s.slots - 1) / s.slots;
+        const double cost = static_cast<double>(rounds) * static_cast<double>(len + s.least / 2);
+        if (best_cost < 0.0 || cost < best_cost) best = len, best_cost = cost;
+    }
+    return best;
+}
+
+// Whole tiles as long as they fill the slots round by round; what is left over
+// (all of it, when the tiles are fewer than the slots) is split along the c
+// side so that it fills the last round.
+PassPlan plan_pass(const PassShape& s, const Sequence* seq, int64_t batch, int kv_heads, bool dkv,
+                   CrossItem* items, CrossJoin* joins) {
+    int64_t tiles = 0;
+    for (int64_t b = 0; b < batch; ++b) tiles += (seq[b].rn + s.tile - 1) / s.tile;
+    const int64_t whole = tiles * kv_heads / s.slots * s.slots / kv_heads;
+    const int64_t rest = (tiles - whole) * kv_heads;
+    const int64_t chunk = whole == 0 ? pick_chunk(s, seq, batch, kv_heads) : 0;
+    const int64_t split = rest > 0 ? s.slots / rest : 1;
     PassPlan p;
-    int64_t qb = 0, kb = 0;
+    int64_t t = 0;
     for (int64_t b = 0; b < batch; ++b) {
-        const int64_t rn = dkv ? keys[b] : rows[b], cn = dkv ? rows[b] : keys[b];
-        int64_t parts = (cn + chunk - 1) / chunk;
-        if (parts < 1) parts = 1;
-        // equal parts, each a multiple of the unit but the last
-        const int64_t len = cn == 0 ? 0 : ((cn + parts - 1) / parts + shape.unit - 1) / shape.unit * shape.unit;
-        if (len > 0) parts = (cn + len - 1) / len;
-        for (int64_t r0 = 0; r0 < rn; r0 += tile) {
-            const int64_t r1 = r0 + tile < rn ? r0 + tile : rn;
+        const int64_t rn = seq[b].rn, cn = seq[b].cn;
+        for (int64_t r0 = 0; r0 < rn; r0 += s.tile, ++t) {
+            const int64_t r1 = r0 + s.tile < rn ? r0 + s.tile : rn;
+            int64_t parts = 1;
+            if (t >= whole && cn > 0) {
+                parts = whole == 0 ? (cn + chunk - 1) / chunk : split;
+                if (parts > cn / s.least) parts = cn / s.least;
+                if (parts < 1) parts = 1;
+            }
+            // equal parts, each a multiple of the unit but the last
+            const int64_t len = cn == 0 ? 0 : up((cn + parts - 1) / parts, s.unit);
+            if (len > 0) parts = (cn + len - 1) / len;
             if (joins && parts > 1)
-                joins[p.joins] = {static_cast<int32_t>(dkv ? kb : qb), static_cast<int32_t>(r0),
+                joins[p.joins] = {static_cast<int32_t>(dkv ? seq[b].kb : seq[b].qb), static_cast<int32_t>(r0),
                                   static_cast<int32_t>(r1), static_cast<int32_t>(p.slots),
                                   static_cast<int32_t>(parts), {0, 0, 0}};
-            for (int64_t s = 0; s < parts; ++s) {
+            for (int64_t k = 0; k < parts; ++k) {
                 if (items) {
-                    const int64_t c0 = s * len, c1 = c0 + len < cn ? c0 + len : cn;
-                    items[p.items] = {static_cast<int32_t>(qb), static_cast<int32_t>(kb),
+                    const int64_t c0 = k * len, c1 = c0 + len < cn ? c0 + len : cn;
+                    items[p.items] = {static_cast<int32_t>(seq[b].qb), static_cast<int32_t>(seq[b].kb),
                                       static_cast<int32_t>(r0), static_cast<int32_t>(r1),
                                       static_cast<int32_t>(c0), static_cast<int32_t>(c1),
-                                      parts > 1 ? static_cast<int32_t>(p.slots + s) : -1, 0};
+                                      parts > 1 ? static_cast<int32_t>(p.slots + k) : -1, 0};
                 }
                 ++p.items;
             }
+            if (t < whole) ++p.whole;
             if (parts > 1) {
                 ++p.joins;
                 p.slots += parts;
             }
         }
-        qb += queries[b];
-        kb += keys[b];
     }
     return p;
 }
@@ -481,7 +516,7 @@ int64_t part_width(int pass, int d) {
 
 template <int DP, int NW>
 void launch_exact(const CrossArgs& a, int pass, hipStream_t st) {
-    const dim3 grid(cross_grid(a.n_items, a.kv_heads)), block(NW * 64);
+    const dim3 grid(cross_grid(a)), block(NW * 64);
     if (pass == MIGNN_CROSS_FORWARD)
         hipLaunchKernelGGL((cross_fwd_kernel<float, DP, NW>), grid, block, 0, st, a);
     else if (pass == MIGNN_CROSS_DQ)
@@ -520,7 +555,7 @@ void launch_join(const CrossArgs& a, int pass, hipStream_t st) {
 int run_pass(CrossArgs a, const mignn_cross_pass& ps, int pass, int dtype, hipStream_t st) {
     a.items = static_cast<const CrossItem*>(ps.items);
     a.joins = static_cast<const CrossJoin*>(ps.joins);
-    a.n_items = ps.n_items, a.n_joins = ps.n_joins, a.tile = ps.tile, a.rows = ps.rows;
+    a.n_items = ps.n_items, a.n_joins = ps.n_joins, a.n_whole = ps.n_whole, a.tile = ps.tile, a.rows = ps.rows;
     if (a.n_items > 0) {
         int rc;
         if (a.tile == CROSS_FEW) rc = cross_few(a, dtype, st);
@@ -586,13 +621,22 @@ extern "C" int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, in
         keys += k_lens[b];
         MIGNN_REQUIRE(queries <= INT32_MAX && keys <= INT32_MAX, "cross_plan: more than 2^31 - 1 rows");
     }
-    int64_t* rows = static_cast<int64_t*>(malloc(sizeof(int64_t) * (batch > 0 ? batch : 1)));
-    MIGNN_REQUIRE(rows, "cross_plan: out of host memory");
-    for (int64_t b = 0; b < batch; ++b) rows[b] = q_lens[b] * group;
-    const PassShape sh = pass_shape(rows, k_lens, batch, pass, kv_heads, static_cast<int>(group));
-    const PassPlan p = plan_pass(sh, rows, q_lens, k_lens, batch, pass == MIGNN_CROSS_DKV,
-                                 static_cast<CrossItem*>(items), static_cast<CrossJoin*>(joins));
-    free(rows);
+    Sequence* seq = static_cast<Sequence*>(malloc(sizeof(Sequence) * (batch > 0 ? batch : 1)));
+    MIGNN_REQUIRE(seq, "cross_plan: out of host memory");
+    const bool dkv = pass == MIGNN_CROSS_DKV;
+    queries = keys = 0;
+    for (int64_t b = 0; b < batch; ++b) {
+        const int64_t rows = q_lens[b] * group;
+        seq[b] = {dkv ? k_lens[b] : rows, dkv ? rows : k_lens[b], queries, keys};
+        queries += q_lens[b];
+        keys += k_lens[b];
+    }
+    // the longest first: what starts last should be short
+    std::stable_sort(seq, seq + batch, [](const Sequence& x, const Sequence& y) { return x.cn > y.cn; });
+    const PassShape sh = pass_shape(seq, batch, pass, d, dtype, static_cast<int>(group));
+    const PassPlan p = plan_pass(sh, seq, batch, kv_heads, dkv, static_cast<CrossItem*>(items),
+                                 static_cast<CrossJoin*>(joins));
+    free(seq);
     MIGNN_REQUIRE(p.items * kv_heads <= INT32_MAX / 2 && p.joins <= INT32_MAX,
                   "cross_plan: too many tiles");
     info[0] = p.items;
@@ -602,6 +646,7 @@ extern "C" int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, in
     info[4] = keys;
     info[5] = sh.tile;
     info[6] = sh.longest;
+    info[7] = p.whole;
     return MIGNN_OK;
 }
 

@@ -46,7 +46,7 @@ struct CrossArgs {
     const CrossItem* items;
     const CrossJoin* joins;
     int64_t ldq, ldqh, ldk, ldkh, ldv, ldvh, lddo, lddoh;
-    int32_t n_items, n_joins, heads, kv_heads, group, d;
+    int32_t n_items, n_whole, n_joins, heads, kv_heads, group, d;
     int32_t tile, rows;          // of the pass: rows (keys) of a tile, of the longest sequence
     float scale, c;              // c = scale log2(e)
 };
@@ -73,20 +73,26 @@ __device__ f32x4 raw_buffer_load_f32x4(i32x4 rsrc, int voffset, int soffset, int
     "llvm.amdgcn.raw.buffer.load.v4f32");
 constexpr int NO_LOAD = INT32_MIN;   // a voffset past every num_records
 
-// Block -> (item, kv head).  Consecutive blocks go to the 8 XCDs in turn; each
-// XCD gets one run of the (head-major) work, so that the tiles that read one
-// head's keys and values share an L2.
-__device__ __forceinline__ bool cross_work(const CrossArgs& a, int n_items, int& item, int& kvh) {
-    const int64_t total = static_cast<int64_t>(n_items) * a.kv_heads;
-    const int64_t per = (total + 7) / 8;
-    const int64_t w = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per || w >= total) return false;
-    kvh = static_cast<int>(w / n_items);
-    item = static_cast<int>(w - static_cast<int64_t>(kvh) * n_items);
+// Block -> (item, kv head): the whole tiles' items first, then the split ones'.
+// Consecutive blocks go to the 8 XCDs in turn; each XCD gets one run of the
+// (head-major) work, so that the tiles that read one head's keys and values
+// share an L2.
+__device__ __forceinline__ bool cross_work(const CrossArgs& a, int& item, int& kvh) {
+    int n = a.n_whole, first = 0;
+    uint32_t b = blockIdx.x;
+    const uint32_t whole = (static_cast<uint32_t>(n) * a.kv_heads + 7u) / 8u * 8u;
+    if (b >= whole) b -= whole, first = n, n = a.n_items - n;
+    const uint32_t total = static_cast<uint32_t>(n) * a.kv_heads, per = (total + 7u) / 8u;
+    const uint32_t w = (b & 7u) * per + (b >> 3);
+    if ((b >> 3) >= per || w >= total) return false;
+    kvh = w / n;
+    item = first + w - static_cast<uint32_t>(kvh) * n;
     return true;
 }
-inline unsigned cross_grid(int64_t n_items, int kv_heads) {
-    return static_cast<unsigned>((n_items * kv_heads + 7) / 8 * 8);
+inline unsigned cross_grid(const CrossArgs& a) {
+    auto up8 = [](int64_t n) { return (n + 7) / 8 * 8; };
+    return static_cast<unsigned>(up8(static_cast<int64_t>(a.n_whole) * a.kv_heads) +
+                                 up8(static_cast<int64_t>(a.n_items - a.n_whole) * a.kv_heads));
 }
 
 // Position in the sequence of an accumulator's element: MFMA 32x32 results

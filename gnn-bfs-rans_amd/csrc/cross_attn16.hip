@@ -133,7 +133,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_fwd16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];   // K, V; twice
     int item, kvh;
-    if (!cross_work(a, a.n_items, item, kvh)) return;
+    if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_dq16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
     int item, kvh;
-    if (!cross_work(a, a.n_items, item, kvh)) return;
+    if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(NW * 64, DP <= 96 ? 2 : 1) void cross_dkv16_kernel(
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];   // lse, delta
     int item, kvh;
-    if (!cross_work(a, a.n_items, item, kvh)) return;
+    if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
@@ -555,7 +555,7 @@ __global__ __launch_bounds__(NW * 64, DP <= 96 ? 2 : 1) void cross_dkv16_kernel(
 
 template <typename T, int DP, int NW, int CB>
 void launch16_tile(const CrossArgs& a, int pass, hipStream_t st) {
-    const dim3 grid(cross_grid(a.n_items, a.kv_heads)), block(NW * 64);
+    const dim3 grid(cross_grid(a)), block(NW * 64);
     if (pass == MIGNN_CROSS_FORWARD)
         hipLaunchKernelGGL((cross_fwd16_kernel<T, DP, NW, CB>), grid, block, 0, st, a);
     else if (pass == MIGNN_CROSS_DQ)

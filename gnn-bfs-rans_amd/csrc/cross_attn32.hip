@@ -112,7 +112,7 @@ __global__ __launch_bounds__(NW * 64, DP <= 64 ? 2 : 1) void cross_fwd32_kernel(
     constexpr f32x16 zero = {};
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE3];   // K, V; twice
     int item, kvh;
-    if (!cross_work(a, a.n_items, item, kvh)) return;
+    if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(NW * 64, DP <= 64 ? 2 : 1) void cross_fwd32_kernel(
 template <int DP>
 void launch32(const CrossArgs& a, hipStream_t st) {
     constexpr int KT = DP == 32 ? 64 : 32;
-    hipLaunchKernelGGL((cross_fwd32_kernel<DP, KT, 4>), dim3(cross_grid(a.n_items, a.kv_heads)), dim3(256), 0, st,
+    hipLaunchKernelGGL((cross_fwd32_kernel<DP, KT, 4>), dim3(cross_grid(a)), dim3(256), 0, st,
                        a);
 }
 

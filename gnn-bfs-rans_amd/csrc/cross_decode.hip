@@ -50,7 +50,7 @@ template <typename T, int R, int LPK>
 __global__ __launch_bounds__(WAVES * 64) void cross_few_kernel(CrossArgs a) {
     constexpr int V = 16 / sizeof(T), KPW = 64 / LPK, UNROLL = R == 8 ? 2 : 4;
     int item, kvh;
-    if (!cross_work(a, a.n_items, item, kvh)) return;
+    if (!cross_work(a, item, kvh)) return;
     const CrossItem it = a.items[item];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, grp = lane / LPK;
     const int c0 = sub * V;
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(WAVES * 64) void cross_few_kernel(CrossArgs a) {
 
 template <typename T, int R>
 void launch_few(const CrossArgs& a, hipStream_t st) {
-    const dim3 grid(cross_grid(a.n_items, a.kv_heads)), block(WAVES * 64);
+    const dim3 grid(cross_grid(a)), block(WAVES * 64);
     const int lanes = a.d / (16 / static_cast<int>(sizeof(T)));
 #define MIGNN_FEW(L) hipLaunchKernelGGL((cross_few_kernel<T, R, L>), grid, block, 0, st, a)
     if (lanes <= 4) MIGNN_FEW(4);

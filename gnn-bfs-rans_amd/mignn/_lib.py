@@ -37,7 +37,8 @@ class CrossPass(ctypes.Structure):
     """mignn_cross_pass"""
     _fields_ = [("items", c_void_p), ("joins", c_void_p), ("part_bytes", c_int64),
                 ("n_items", ctypes.c_int32), ("n_joins", ctypes.c_int32),
-                ("tile", ctypes.c_int32), ("rows", ctypes.c_int32)]
+                ("tile", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("n_whole", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 class CrossCall(ctypes.Structure):

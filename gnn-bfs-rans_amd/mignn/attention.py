@@ -332,7 +332,7 @@ class CrossPlan:
         self.dtype, self.train = dtype, bool(train)
         self.queries, self.keys = int(ql.sum()), int(kl.sum())
         L = _lib.lib()
-        info = np.zeros(7, np.int64)
+        info = np.zeros(8, np.int64)
         lists, spans, at = [], [], 0
         size = _lib.CROSS_ITEM_BYTES
         for kind in range(3 if train else 1):
@@ -345,7 +345,8 @@ class CrossPlan:
             n_items, n_joins, part = (int(v) for v in info[:3])
             buf = np.zeros((n_items + n_joins) * size, np.uint8)
             plan(buf.ctypes.data, buf.ctypes.data + n_items * size)
-            spans.append((at, at + n_items * size, part, n_items, n_joins, int(info[5]), int(info[6])))
+            spans.append((at, at + n_items * size, part, n_items, n_joins) +
+                         tuple(int(v) for v in info[5:]))
             lists.append(buf)
             at += buf.size
         host = torch.from_numpy(np.concatenate(lists))
@@ -355,10 +356,11 @@ class CrossPlan:
         call = _lib.CrossCall()
         call.heads, call.kv_heads, call.d = self.heads, self.kv_heads, self.head_dim
         call.dtype, call.n_keys = _ROW[dtype], self.keys
-        for kind, (items, joins, part, n_items, n_joins, tile, rows) in enumerate(spans):
+        for kind, (items, joins, part, n_items, n_joins, tile, rows, whole) in enumerate(spans):
             ps = call.passes[kind]
             ps.items, ps.joins, ps.part_bytes = base + items, base + joins, part
-            ps.n_items, ps.n_joins, ps.tile, ps.rows = n_items, n_joins, tile, rows
+            ps.n_items, ps.n_joins, ps.n_whole = n_items, n_joins, whole
+            ps.tile, ps.rows = tile, rows
         self._call = call
         parts = [s[2] for s in spans]
         self._scratch = (parts[0], max(parts[1:]) if train else 0)

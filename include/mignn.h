@@ -765,8 +765,8 @@ int mignn_rotary(const void* x, int64_t ldt, int64_t ldh, int64_t n, int heads, 
  * [keys, kv_heads, d], query head h reads kv head h / (heads / kv_heads).
  * mignn_cross_plan runs on the HOST: given the lengths it fills the work items
  * and joins of one pass (host memory, MIGNN_CROSS_ITEM_BYTES each; either may
- * be NULL to count) and info[7] = {items, joins, scratch bytes, queries, keys,
- * tile, rows} (tile, rows: for mignn_cross_pass).
+ * be NULL to count) and info[8] = {items, joins, scratch bytes, queries, keys,
+ * tile, rows, whole} (the last three: for mignn_cross_pass).
  * The caller copies them to the device. */
 #define MIGNN_CROSS_MAX_D 128
 #define MIGNN_CROSS_MAX_GROUP 64          /* query heads a key head */
@@ -782,6 +782,8 @@ typedef struct {
     int64_t part_bytes;
     int32_t n_items, n_joins;
     int32_t tile, rows;     /* rows (keys) of a tile; of the longest sequence */
+    int32_t n_whole;        /* items ahead of the split ones */
+    int32_t reserved;
 } mignn_cross_pass;
 typedef struct {
     const void *q, *k, *v;

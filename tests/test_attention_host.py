@@ -106,7 +106,8 @@ def _lists(plan, kind):
 @pytest.mark.parametrize("ql,kl,heads,kv", [
     ([1], [1], 1, 1), ([5], [0], 4, 4), ([0], [9], 4, 2), ([0, 0], [0, 0], 2, 1), ([], [], 2, 2),
     ([1], [20000], 8, 2), ([40000], [33], 4, 1), ([129, 0, 1, 4000], [1, 700, 0, 5000], 6, 3),
-    ([1] * 64, list(range(0, 64 * 97, 97)), 8, 2)])
+    ([1] * 64, list(range(0, 64 * 97, 97)), 8, 2),
+    ([33000], [3000], 4, 2), ([9000, 70, 30000], [300, 9000, 2000], 4, 4)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_cross_plan_covers_every_pair_once(ql, kl, heads, kv, dtype):
     """Every (row, key) pair of every sequence is in exactly one item of each
@@ -197,10 +198,10 @@ def test_c_entry_points_check_arguments():
 
 def test_call_struct_layout_matches_header():
     """The ctypes mirror of mignn_cross_call has the C layout (x86-64)."""
-    assert ctypes.sizeof(_lib.CrossPass) == 40
+    assert ctypes.sizeof(_lib.CrossPass) == 48
     assert _lib.CrossCall.ldq.offset == 32 and _lib.CrossCall.n_keys.offset == 80
     assert _lib.CrossCall.scale.offset == 104 and _lib.CrossCall.scratch.offset == 112
-    assert ctypes.sizeof(_lib.CrossCall) == 128 + 3 * 40
+    assert ctypes.sizeof(_lib.CrossCall) == 128 + 3 * 48
 
 
 def test_oracle_gradients_match_differences():
