@@ -176,16 +176,49 @@ __global__ __launch_bounds__(NW * 64) void cross_fwd_kernel(CrossArgs a) {
     if (a.lse && half == 0) a.lse[at] = l == 0.f ? INFINITY : m2 + log2f(l);
 }
 
-// Joins the parts of split rows onto their largest maximum.  WPR waves a row
-// share its parts (1 where parts are few, 4 where a row has many).
-template <typename T, int WPR>
+// Joins the parts of split rows onto their largest maximum.  Few parts: 4
+// columns of a row a thread.
+template <typename T>
 __global__ __launch_bounds__(256) void cross_join_fwd_kernel(CrossArgs a) {
     const CrossJoin jn = a.joins[blockIdx.x];
-    const int kvh = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r = blockIdx.z * (4 / WPR) + wave / WPR;
-    const bool live = r < jn.r1 - jn.r0;
+    const int kvh = blockIdx.y, i = blockIdx.z * 256 + threadIdx.x, d4 = a.d / 4;
+    const int r = i / d4, c = (i - r * d4) * 4;
+    if (r >= jn.r1 - jn.r0) return;
     const int64_t step = static_cast<int64_t>(a.kv_heads) * a.tile * (a.d + 2);   // part to part
-    const float* src = part_row(a, jn.slot, kvh, live ? r : 0, a.tile, a.d + 2);
+    const float* src = part_row(a, jn.slot, kvh, r, a.tile, a.d + 2);
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int p = 0; p < jn.parts; ++p) m = fmaxf(m, src[p * step + a.d]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < jn.parts; ++p) {
+        float x[4];
+        load_row(src + p * step + c, x);
+        const float f = __builtin_amdgcn_exp2f(src[p * step + a.d] - base);
+        l = fmaf(src[p * step + a.d + 1], f, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    const int row = jn.r0 + r, t = row / a.group;
+    const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group + (row - t * a.group);
+    store_row(static_cast<T*>(a.out) + at * a.d + c, o);
+    if (a.o32) store_row(a.o32 + at * a.d + c, o);
+    if (a.lse && c == 0) a.lse[at] = l == 0.f ? INFINITY : base + log2f(l);
+}
+
+// Many parts of few rows: one row a workgroup, its waves take every fourth part.
+template <typename T>
+__global__ __launch_bounds__(256) void cross_join_few_kernel(CrossArgs a) {
+    __shared__ float os[4][128];
+    const CrossJoin jn = a.joins[blockIdx.x];
+    const int kvh = blockIdx.y, r = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (r >= jn.r1 - jn.r0) return;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.tile * (a.d + 2);
+    const float* src = part_row(a, jn.slot, kvh, r, a.tile, a.d + 2);
     float m = -INFINITY;
     for (int p = lane; p < jn.parts; p += 64) m = fmaxf(m, src[p * step + a.d]);
     for (int b = 1; b < 64; b <<= 1) m = fmaxf(m, __shfl_xor(m, b));
@@ -199,8 +232,8 @@ __global__ __launch_bounds__(256) void cross_join_fwd_kernel(CrossArgs a) {
             l = fmaf(src[(p0 + lane) * step + a.d + 1], f, l);
         }
         const int n = jn.parts - p0 < 64 ? jn.parts - p0 : 64;
-#pragma unroll 4
-        for (int p = wave % WPR; p < n; p += WPR) {
+#pragma unroll 8
+        for (int p = wave; p < n; p += 4) {
             const float fp = __shfl(f, p);
             const float* row = src + (p0 + p) * step + lane;
             if (one) o[0] = fmaf(row[0], fp, o[0]);
@@ -208,15 +241,11 @@ __global__ __launch_bounds__(256) void cross_join_fwd_kernel(CrossArgs a) {
         }
     }
     for (int b = 1; b < 64; b <<= 1) l += __shfl_xor(l, b);
-    if constexpr (WPR > 1) {
-        __shared__ float os[4][128];
-        os[wave][lane] = o[0], os[wave][lane + 64] = o[1];
-        __syncthreads();
-        if (wave % WPR) return;
+    os[wave][lane] = o[0], os[wave][lane + 64] = o[1];
+    __syncthreads();
+    if (wave) return;
 #pragma unroll
-        for (int w = 1; w < WPR; ++w) o[0] += os[wave + w][lane], o[1] += os[wave + w][lane + 64];
-    }
-    if (!live) return;
+    for (int w = 1; w < 4; ++w) o[0] += os[w][lane], o[1] += os[w][lane + 64];
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int row = jn.r0 + r, t = row / a.group;
     const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group + (row - t * a.group);
@@ -365,32 +394,33 @@ __global__ __launch_bounds__(NW * 64) void cross_dkv_kernel(CrossArgs a) {
     }
 }
 
-// Sums the parts of split gradients in slot order, one wave a row: dq, or dk
-// and dv side by side.
+// Sums the parts of split gradients in slot order, 4 columns of a row a thread:
+// dq, or dk and dv side by side.
 template <typename T>
 __global__ __launch_bounds__(256) void cross_join_grad_kernel(CrossArgs a, bool dkv) {
     const CrossJoin jn = a.joins[blockIdx.x];
-    const int kvh = blockIdx.y, lane = threadIdx.x & 63;
-    const int width = dkv ? 2 * a.d : a.d;
-    const int r = blockIdx.z * 4 + (threadIdx.x >> 6);
+    const int width = dkv ? 2 * a.d : a.d, w4 = width / 4;
+    const int kvh = blockIdx.y, i = blockIdx.z * 256 + threadIdx.x;
+    const int r = i / w4, c = (i - r * w4) * 4;
     if (r >= jn.r1 - jn.r0) return;
     const int64_t step = static_cast<int64_t>(a.kv_heads) * a.tile * width;
-    const float* src = part_row(a, jn.slot, kvh, r, a.tile, width);
-    const int row = jn.r0 + r;
-    for (int c = lane; c < width; c += 64) {
-        float v = 0.f;
+    const float* src = part_row(a, jn.slot, kvh, r, a.tile, width) + c;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-        for (int p = 0; p < jn.parts; ++p) v += src[p * step + c];
-        if (dkv) {
-            const int64_t at = ((jn.begin + static_cast<int64_t>(row)) * a.kv_heads + kvh) * a.d;
-            T* dst = static_cast<T*>(c < a.d ? a.dk : a.dv);
-            dst[at + (c < a.d ? c : c - a.d)] = static_cast<T>(v);
-        } else {
-            const int t = row / a.group;
-            const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group +
-                               (row - t * a.group);
-            static_cast<T*>(a.out)[at * a.d + c] = static_cast<T>(v);
-        }
+    for (int p = 0; p < jn.parts; ++p) {
+        float x[4];
+        load_row(src + p * step, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += x[e];
+    }
+    const int row = jn.r0 + r;
+    if (dkv) {
+        const int64_t at = ((jn.begin + static_cast<int64_t>(row)) * a.kv_heads + kvh) * a.d;
+        store_row(c < a.d ? static_cast<T*>(a.dk) + at + c : static_cast<T*>(a.dv) + at + c - a.d, v);
+    } else {
+        const int t = row / a.group;
+        const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group + (row - t * a.group);
+        store_row(static_cast<T*>(a.out) + at * a.d + c, v);
     }
 }
 
@@ -542,14 +572,14 @@ int cross_pass_exact(const CrossArgs& a, int pass, hipStream_t st) {
 template <typename T>
 void launch_join(const CrossArgs& a, int pass, hipStream_t st) {
     const unsigned rows = a.rows < a.tile ? a.rows : a.tile;
-    const dim3 grid(a.n_joins, a.kv_heads, (rows + 3) / 4);
+    auto grid = [&](unsigned width) { return dim3(a.n_joins, a.kv_heads, (rows * (width / 4) + 255) / 256); };
+    const bool dkv = pass == MIGNN_CROSS_DKV;
     if (pass != MIGNN_CROSS_FORWARD)
-        hipLaunchKernelGGL(cross_join_grad_kernel<T>, grid, dim3(256), 0, st, a, pass == MIGNN_CROSS_DKV);
+        hipLaunchKernelGGL(cross_join_grad_kernel<T>, grid(dkv ? 2 * a.d : a.d), dim3(256), 0, st, a, dkv);
     else if (a.tile == 128)
-        hipLaunchKernelGGL((cross_join_fwd_kernel<T, 1>), grid, dim3(256), 0, st, a);
-    else   // few rows in many parts
-        hipLaunchKernelGGL((cross_join_fwd_kernel<T, 4>), dim3(a.n_joins, a.kv_heads, rows), dim3(256), 0,
-                           st, a);
+        hipLaunchKernelGGL(cross_join_fwd_kernel<T>, grid(a.d), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL(cross_join_few_kernel<T>, dim3(a.n_joins, a.kv_heads, rows), dim3(256), 0, st, a);
 }
 
 int run_pass(CrossArgs a, const mignn_cross_pass& ps, int pass, int dtype, hipStream_t st) {
