@@ -48,7 +48,7 @@ struct KeyLoad {
 // R rows (a power of two that holds the sequence's); LPK lanes a key, V elements each
 template <typename T, int R, int LPK>
 __global__ __launch_bounds__(WAVES * 64) void cross_few_kernel(CrossArgs a) {
-    constexpr int V = 16 / sizeof(T), KPW = 64 / LPK, UNROLL = R == 8 ? 2 : 4;
+    constexpr int V = 16 / sizeof(T), KPW = 64 / LPK, UNROLL = R >= 4 ? 2 : 4;
     int item, kvh;
     if (!cross_work(a, item, kvh)) return;
     const CrossItem it = a.items[item];
