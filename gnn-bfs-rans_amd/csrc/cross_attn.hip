@@ -1,6 +1,6 @@
 // Cross attention of query rows to the states of another mesh
-// (mignn_cross_attn_forward, mignn_cross_attn_backward): the work plan, the
-// exact fp32 kernels and the joins of split work.
+// (mignn_cross_attn_forward, mignn_cross_attn_backward): the work plan and
+// the joins of split work.
 //
 //   s_ij = scale <q_i, k_j> over the keys j of the row's sequence that the mask keeps
 //   P_ij = 2^(c <q_i, k_j> - lse_i),  c = scale log2 e,  lse_i = log2 sum_j 2^(c <q_i, k_j>)
@@ -18,7 +18,7 @@
 // atomically and results do not depend on the order of workgroups.  The query
 // heads that share a kv head are rows of one tile: their keys are read once,
 // and dk, dv sum over them in place.
-#include "mfma16.hpp"
+#include "cross_attn.hpp"
 
 #include <algorithm>
 #include <cstdlib>
@@ -26,154 +26,11 @@
 namespace mignn {
 namespace {
 
-// A tile of 32 rows of q or do, or of k or v, into LDS as fp32, columns >= d
-// and rows that `keep` leaves out as zeros.
-template <typename T, int DP, int NT, typename Row>
-__device__ __forceinline__ void stage_tile(float* lds, int d, Row row_ptr) {
-    constexpr int C4 = DP / 4;
-    for (int i = threadIdx.x; i < 32 * C4; i += NT) {
-        const int r = i / C4, c = (i % C4) * 4;
-        const T* p = row_ptr(r);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p && c < d) v = load4(p + c);
-        st4(lds + r * (DP + 4) + c, v);
-    }
-}
-
-// 32 values a lane of one row: columns 8 i + 4 (lane / 32) + 0..3, the k order
-// of the products over columns
-template <typename T, int DP>
-__device__ __forceinline__ void load_frag(float4 (&f)[DP / 8], const T* p, int d, int half) {
-#pragma unroll
-    for (int i = 0; i < DP / 8; ++i) {
-        const int c = 8 * i + 4 * half;
-        f[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p && c < d) f[i] = load4(p + c);
-    }
-}
-
-__device__ __forceinline__ f32x16 mfma32(float a, float b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
-}
-
-// acc += (LDS tile row l % 32) . (fragment), over the columns
-template <int DP>
-__device__ __forceinline__ f32x16 dot_tile(const float* tile, const float4 (&f)[DP / 8], int col,
-                                           int half) {
-    f32x16 acc = {};
-    const float* p = tile + col * (DP + 4) + 4 * half;
-#pragma unroll
-    for (int i = 0; i < DP / 8; ++i) {
-        const float4 a = ld4(p + 8 * i);
-        acc = mfma32(a.x, f[i].x, acc);
-        acc = mfma32(a.y, f[i].y, acc);
-        acc = mfma32(a.z, f[i].z, acc);
-        acc = mfma32(a.w, f[i].w, acc);
-    }
-    return acc;
-}
-
-// acc[b] += tile^T (columns 32 b + l % 32) . w, over the tile's 32 rows in the
-// order in which w's registers hold them
-template <int DP>
-__device__ __forceinline__ void add_tile(const float* tile, const f32x16& w, f32x16 (&acc)[DP / 32],
-                                         int col, int half) {
-    const float* p = tile + 4 * half * (DP + 4) + col;
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int b = 0; b < DP / 32; ++b)
-            acc[b] = mfma32(p[acc_row(r) * (DP + 4) + 32 * b], w[r], acc[b]);
-}
-
-struct RowRef {
-    int64_t token;
-    int head;
-};
-__device__ __forceinline__ RowRef row_ref(const CrossArgs& a, const CrossItem& it, int row, int kvh) {
-    const int t = row / a.group;
-    return {it.q_begin + static_cast<int64_t>(t), kvh * a.group + (row - t * a.group)};
-}
-
 // partial results: [slot][kv head][rows of the tile][d + 2] (forward: o
 // unnormalised, maximum, sum; dq: dq; dk / dv: dk and dv, 2 d)
 __device__ __forceinline__ float* part_row(const CrossArgs& a, int slot, int kvh, int r, int rows,
                                            int width) {
     return a.part + ((static_cast<int64_t>(slot) * a.kv_heads + kvh) * rows + r) * width;
-}
-
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void cross_fwd_kernel(CrossArgs a) {
-    __shared__ __attribute__((aligned(16))) float ks[32 * (DP + 4)], vs[32 * (DP + 4)];
-    int item, kvh;
-    if (!cross_work(a, item, kvh)) return;
-    const CrossItem it = load_item(a, item);
-    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int row = it.r0 + wave * 32 + col;
-    const bool live = row < it.r1;
-    const RowRef ref = row_ref(a, it, row, kvh);
-    float4 qf[DP / 8];
-    load_frag<T, DP>(qf, live ? static_cast<const T*>(a.q) + ref.token * a.ldq + ref.head * a.ldqh
-                              : nullptr, a.d, half);
-    f32x16 o[DP / 32] = {};
-    float m = -INFINITY, l = 0.f;
-    for (int k0 = it.c0; k0 < it.c1; k0 += 32) {
-        const int64_t key0 = it.k_begin + static_cast<int64_t>(k0);
-        const int left = it.c1 - k0;
-        const bool ok = lane < 32 && lane < left && (!a.mask || a.mask[key0 + lane]);
-        const uint32_t bits = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok));
-        __syncthreads();
-        stage_tile<T, DP, NW * 64>(ks, a.d, [&](int r) {
-            return (bits >> r) & 1u ? static_cast<const T*>(a.k) + (key0 + r) * a.ldk + kvh * a.ldkh
-                                    : nullptr;
-        });
-        stage_tile<T, DP, NW * 64>(vs, a.d, [&](int r) {
-            return (bits >> r) & 1u ? static_cast<const T*>(a.v) + (key0 + r) * a.ldv + kvh * a.ldvh
-                                    : nullptr;
-        });
-        __syncthreads();
-        f32x16 s = dot_tile<DP>(ks, qf, col, half);
-        if (bits != 0xffffffffu) {
-            const uint32_t mine = bits >> (4 * half);
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (!((mine >> acc_row(r)) & 1u)) s[r] = -INFINITY;
-        }
-        float mx = s[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx);
-        const float base = mn == -INFINITY ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f((m - base) * a.c);
-        m = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -base * a.c));
-            sum += s[r];
-        }
-        l = fmaf(l, alpha, sum);
-#pragma unroll
-        for (int b = 0; b < DP / 32; ++b) o[b] *= alpha;
-        add_tile<DP>(vs, s, o, col, half);
-    }
-    l += __shfl_xor(l, 32);
-    if (!live) return;
-    const float m2 = (m == -INFINITY ? 0.f : m) * a.c;
-    if (it.slot >= 0) {
-        float* p = part_row(a, it.slot, kvh, wave * 32 + col, NW * 32, a.d + 2);
-        store_acc<float, DP>(p, o, 1.f, a.d, half);
-        if (half == 0) p[a.d] = m == -INFINITY ? -INFINITY : m2;
-        else p[a.d + 1] = l;
-        return;
-    }
-    // a row without keys: o = 0, and lse = inf makes every P of the backward 0
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int64_t at = ref.token * a.heads + ref.head;
-    store_acc<T, DP>(static_cast<T*>(a.out) + at * a.d, o, inv, a.d, half);
-    if (a.o32) store_acc<float, DP>(a.o32 + at * a.d, o, inv, a.d, half);
-    if (a.lse && half == 0) a.lse[at] = l == 0.f ? INFINITY : m2 + log2f(l);
 }
 
 // Joins the parts of split rows onto their largest maximum.  Few parts: 4
@@ -187,7 +44,6 @@ __global__ __launch_bounds__(256) void cross_join_fwd_kernel(CrossArgs a) {
     const int64_t step = static_cast<int64_t>(a.kv_heads) * a.tile * (a.d + 2);   // part to part
     const float* src = part_row(a, jn.slot, kvh, r, a.tile, a.d + 2);
     float m = -INFINITY;
-#pragma unroll 4
     for (int p = 0; p < jn.parts; ++p) m = fmaxf(m, src[p * step + a.d]);
     const float base = m == -INFINITY ? 0.f : m;
     float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -232,7 +88,6 @@ __global__ __launch_bounds__(256) void cross_join_few_kernel(CrossArgs a) {
             l = fmaf(src[(p0 + lane) * step + a.d + 1], f, l);
         }
         const int n = jn.parts - p0 < 64 ? jn.parts - p0 : 64;
-#pragma unroll 8
         for (int p = wave; p < n; p += 4) {
             const float fp = __shfl(f, p);
             const float* row = src + (p0 + p) * step + lane;
@@ -257,141 +112,6 @@ __global__ __launch_bounds__(256) void cross_join_few_kernel(CrossArgs a) {
         if (a.o32) a.o32[at * a.d + c] = o[i] * inv;
     }
     if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : base + log2f(l);
-}
-
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void cross_dq_kernel(CrossArgs a) {
-    __shared__ __attribute__((aligned(16))) float ks[32 * (DP + 4)], vs[32 * (DP + 4)];
-    int item, kvh;
-    if (!cross_work(a, item, kvh)) return;
-    const CrossItem it = load_item(a, item);
-    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int row = it.r0 + wave * 32 + col;
-    const bool live = row < it.r1;
-    const RowRef ref = row_ref(a, it, row, kvh);
-    const int64_t at = ref.token * a.heads + ref.head;
-    float4 qf[DP / 8], gf[DP / 8];
-    load_frag<T, DP>(qf, live ? static_cast<const T*>(a.q) + ref.token * a.ldq + ref.head * a.ldqh
-                              : nullptr, a.d, half);
-    load_frag<T, DP>(gf, live ? static_cast<const T*>(a.dout) + ref.token * a.lddo +
-                                    ref.head * a.lddoh : nullptr, a.d, half);
-    float delta = 0.f;
-    {
-        const float* o = live ? a.out32 + at * a.d : nullptr;
-#pragma unroll
-        for (int i = 0; i < DP / 8; ++i) {
-            const int c = 8 * i + 4 * half;
-            if (!o || c >= a.d) continue;
-            const float4 v = ld4(o + c);
-            delta = fmaf(v.x, gf[i].x, fmaf(v.y, gf[i].y, fmaf(v.z, gf[i].z, fmaf(v.w, gf[i].w, delta))));
-        }
-        delta += __shfl_xor(delta, 32);
-        // the dk / dv kernel's: written by the item of the row's first keys
-        if (live && half == 0 && it.c0 == 0) a.delta[at] = delta;
-    }
-    const float lse = live ? a.lse[at] : INFINITY;
-    f32x16 acc[DP / 32] = {};
-    for (int k0 = it.c0; k0 < it.c1; k0 += 32) {
-        const int64_t key0 = it.k_begin + static_cast<int64_t>(k0);
-        const int left = it.c1 - k0;
-        const bool ok = lane < 32 && lane < left && (!a.mask || a.mask[key0 + lane]);
-        const uint32_t bits = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok));
-        __syncthreads();
-        stage_tile<T, DP, NW * 64>(ks, a.d, [&](int r) {
-            return (bits >> r) & 1u ? static_cast<const T*>(a.k) + (key0 + r) * a.ldk + kvh * a.ldkh
-                                    : nullptr;
-        });
-        stage_tile<T, DP, NW * 64>(vs, a.d, [&](int r) {
-            return (bits >> r) & 1u ? static_cast<const T*>(a.v) + (key0 + r) * a.ldv + kvh * a.ldvh
-                                    : nullptr;
-        });
-        __syncthreads();
-        f32x16 s = dot_tile<DP>(ks, qf, col, half);
-        const f32x16 dp = dot_tile<DP>(vs, gf, col, half);
-        const uint32_t mine = bits >> (4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse));
-            s[r] = (mine >> acc_row(r)) & 1u ? p * (dp[r] - delta) : 0.f;
-        }
-        add_tile<DP>(ks, s, acc, col, half);
-    }
-    if (!live) return;
-    if (it.slot >= 0)
-        store_acc<float, DP>(part_row(a, it.slot, kvh, wave * 32 + col, NW * 32, a.d), acc, a.scale,
-                             a.d, half);
-    else
-        store_acc<T, DP>(static_cast<T*>(a.out) + at * a.d, acc, a.scale, a.d, half);
-}
-
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void cross_dkv_kernel(CrossArgs a) {
-    __shared__ __attribute__((aligned(16))) float qs[32 * (DP + 4)], gs[32 * (DP + 4)];
-    __shared__ __attribute__((aligned(16))) float ls[32], ds[32];
-    int item, kvh;
-    if (!cross_work(a, item, kvh)) return;
-    const CrossItem it = load_item(a, item);
-    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int key = it.r0 + wave * 32 + col;
-    const int64_t kt = it.k_begin + static_cast<int64_t>(key);
-    const bool live = key < it.r1;
-    const bool keep = live && (!a.mask || a.mask[kt]);
-    float4 kf[DP / 8], vf[DP / 8];
-    load_frag<T, DP>(kf, keep ? static_cast<const T*>(a.k) + kt * a.ldk + kvh * a.ldkh : nullptr,
-                     a.d, half);
-    load_frag<T, DP>(vf, keep ? static_cast<const T*>(a.v) + kt * a.ldv + kvh * a.ldvh : nullptr,
-                     a.d, half);
-    f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
-    for (int r0 = it.c0; r0 < it.c1; r0 += 32) {
-        __syncthreads();
-        stage_tile<T, DP, NW * 64>(qs, a.d, [&](int r) -> const T* {
-            if (r0 + r >= it.c1) return nullptr;
-            const RowRef ref = row_ref(a, it, r0 + r, kvh);
-            return static_cast<const T*>(a.q) + ref.token * a.ldq + ref.head * a.ldqh;
-        });
-        stage_tile<T, DP, NW * 64>(gs, a.d, [&](int r) -> const T* {
-            if (r0 + r >= it.c1) return nullptr;
-            const RowRef ref = row_ref(a, it, r0 + r, kvh);
-            return static_cast<const T*>(a.dout) + ref.token * a.lddo + ref.head * a.lddoh;
-        });
-        if (threadIdx.x < 32) {
-            const bool in = r0 + static_cast<int>(threadIdx.x) < it.c1;
-            const RowRef ref = row_ref(a, it, r0 + threadIdx.x, kvh);
-            ls[threadIdx.x] = in ? a.lse[ref.token * a.heads + ref.head] : INFINITY;
-            ds[threadIdx.x] = in ? a.delta[ref.token * a.heads + ref.head] : 0.f;
-        }
-        __syncthreads();
-        f32x16 s = dot_tile<DP>(qs, kf, col, half);
-        f32x16 dp = dot_tile<DP>(gs, vf, col, half);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 lse = ld4(ls + 8 * g + 4 * half), del = ld4(ds + 8 * g + 4 * half);
-            const float lv[4] = {lse.x, lse.y, lse.z, lse.w}, ev[4] = {del.x, del.y, del.z, del.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = 4 * g + e;
-                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lv[e]));
-                dp[r] = s[r] * (dp[r] - ev[e]);
-            }
-        }
-        add_tile<DP>(gs, s, dv, col, half);
-        add_tile<DP>(qs, dp, dk, col, half);
-    }
-    if (!live) return;
-    // a key that the mask leaves out has no gradient, whatever its rows hold
-    if (!keep) {
-#pragma unroll
-        for (int b = 0; b < DP / 32; ++b) dk[b] = dv[b] = f32x16{};
-    }
-    if (it.slot >= 0) {
-        float* p = part_row(a, it.slot, kvh, wave * 32 + col, NW * 32, 2 * a.d);
-        store_acc<float, DP>(p, dk, a.scale, a.d, half);
-        store_acc<float, DP>(p + a.d, dv, 1.f, a.d, half);
-    } else {
-        const int64_t at = (kt * a.kv_heads + kvh) * a.d;
-        store_acc<T, DP>(static_cast<T*>(a.dk) + at, dk, a.scale, a.d, half);
-        store_acc<T, DP>(static_cast<T*>(a.dv) + at, dv, 1.f, a.d, half);
-    }
 }
 
 // Sums the parts of split gradients in slot order, 4 columns of a row a thread:
@@ -444,25 +164,20 @@ struct Sequence {
 
 int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 
-// Tile: 8 rows where no sequence has more (forward: cross_few).  Else 128, four
-// waves that share the staging of the other side, or 32, one wave, where
-// padding to 128 would add a quarter to the work (few rows, or many short
-// sequences: three snapshots' 64..257 states as keys, fp32 dk / dv 112 us in
-// tiles of 128).
+// Tile: 8 rows where no sequence has more (forward: cross_few), 32 (one wave)
+// where none has more than 32, else 128, four waves that share the staging of
+// the other side.  (32 for longer sequences saves padding but not time: LDS
+// holds few such workgroups; keys of three sequences of 78, 134 and 167: dk /
+// dv 108 us in tiles of 32, 61 in tiles of 128.)
 PassShape pass_shape(const Sequence* seq, int64_t batch, int pass, int d, int dtype, int group) {
     const bool dkv = pass == MIGNN_CROSS_DKV;
     PassShape s{128, 0, 512, 256, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
-    double w32 = 0.0, w128 = 0.0;
-    for (int64_t b = 0; b < batch; ++b) {
-        if (seq[b].rn > s.longest) s.longest = seq[b].rn;
-        w32 += static_cast<double>(up(seq[b].rn, 32)) * static_cast<double>(seq[b].cn);
-        w128 += static_cast<double>(up(seq[b].rn, 128)) * static_cast<double>(seq[b].cn);
-    }
+    for (int64_t b = 0; b < batch; ++b) s.longest = seq[b].rn > s.longest ? seq[b].rn : s.longest;
     if (pass == MIGNN_CROSS_FORWARD && s.longest <= CROSS_FEW) s.tile = CROSS_FEW;
-    else if (s.longest <= 32 || w128 > 1.25 * w32) s.tile = 32;
+    else if (s.longest <= CROSS_ROWS) s.tile = CROSS_ROWS;
     // registers and LDS: two workgroups of four waves a CU, one where the heads
     // are wide and much is held in fp32; eight small ones
-    const bool wide = dtype == MIGNN_ROW_F32 ? d > 64 : dkv && d > 96;
+    const bool wide = dtype == MIGNN_ROW_F32 ? d > 64 || (dkv && d > 32) : dkv && d > 96;
     if (s.tile != 128) s.slots = 2048, s.least = 128;
     else if (wide) s.slots = 256;
     return s;
@@ -544,31 +259,6 @@ int64_t part_width(int pass, int d) {
     return pass == MIGNN_CROSS_FORWARD ? d + 2 : pass == MIGNN_CROSS_DQ ? d : 2 * d;
 }
 
-template <int DP, int NW>
-void launch_exact(const CrossArgs& a, int pass, hipStream_t st) {
-    const dim3 grid(cross_grid(a)), block(NW * 64);
-    if (pass == MIGNN_CROSS_FORWARD)
-        hipLaunchKernelGGL((cross_fwd_kernel<float, DP, NW>), grid, block, 0, st, a);
-    else if (pass == MIGNN_CROSS_DQ)
-        hipLaunchKernelGGL((cross_dq_kernel<float, DP, NW>), grid, block, 0, st, a);
-    else
-        hipLaunchKernelGGL((cross_dkv_kernel<float, DP, NW>), grid, block, 0, st, a);
-}
-
-template <int DP>
-void launch_exact_d(const CrossArgs& a, int pass, hipStream_t st) {
-    if (a.tile == CROSS_ROWS) launch_exact<DP, 1>(a, pass, st);
-    else launch_exact<DP, 4>(a, pass, st);
-}
-
-int cross_pass_exact(const CrossArgs& a, int pass, hipStream_t st) {
-    if (a.d <= 32) launch_exact_d<32>(a, pass, st);
-    else if (a.d <= 64) launch_exact_d<64>(a, pass, st);
-    else if (a.d <= 96) launch_exact_d<96>(a, pass, st);
-    else launch_exact_d<128>(a, pass, st);
-    return launch_status("cross attention kernel");
-}
-
 template <typename T>
 void launch_join(const CrossArgs& a, int pass, hipStream_t st) {
     const unsigned rows = a.rows < a.tile ? a.rows : a.tile;
@@ -589,8 +279,7 @@ int run_pass(CrossArgs a, const mignn_cross_pass& ps, int pass, int dtype, hipSt
     if (a.n_items > 0) {
         int rc;
         if (a.tile == CROSS_FEW) rc = cross_few(a, dtype, st);
-        else if (dtype == MIGNN_ROW_F32 && pass == MIGNN_CROSS_FORWARD && a.tile == 128) rc = cross_forward32(a, st);
-        else if (dtype == MIGNN_ROW_F32) rc = cross_pass_exact(a, pass, st);
+        else if (dtype == MIGNN_ROW_F32) rc = cross_pass32(a, pass, st);
         else rc = cross_pass16(a, pass, dtype, st);
         if (rc) return rc;
     }

@@ -99,17 +99,10 @@ inline unsigned cross_grid(const CrossArgs& a) {
 // hold D[8 (r / 4) + 4 (lane / 32) + r % 4][lane % 32] in register r.
 __device__ __forceinline__ constexpr int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }
 
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p) {
-    float o[4];
-    load_row(p, o);
-    return make_float4(o[0], o[1], o[2], o[3]);
-}
-
 // the 16-bit rows' kernels of a pass (cross_attn16.hip)
 int cross_pass16(const CrossArgs& a, int pass, int dtype, hipStream_t st);
-// the forward of fp32 rows in 128-row tiles (cross_attn32.hip)
-int cross_forward32(const CrossArgs& a, hipStream_t st);
+// the fp32 rows' (cross_attn32.hip)
+int cross_pass32(const CrossArgs& a, int pass, hipStream_t st);
 // the forward of up to CROSS_FEW rows a sequence (cross_decode.hip)
 int cross_few(const CrossArgs& a, int dtype, hipStream_t st);
 

@@ -129,7 +129,7 @@ struct DsScale {
 };
 
 template <typename T, int DP, int NW, int CB>
-__global__ __launch_bounds__(NW * 64, 2) void cross_fwd16_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];   // K, V; twice
     int item, kvh;
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_fwd16_kernel(CrossArgs a) {
 }
 
 template <typename T, int DP, int NW, int CB>
-__global__ __launch_bounds__(NW * 64, 2) void cross_dq16_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_dq16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
     int item, kvh;
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_dq16_kernel(CrossArgs a) {
 }
 
 template <typename T, int DP, int NW, int CB>
-__global__ __launch_bounds__(NW * 64, DP <= 96 ? 2 : 1) void cross_dkv16_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cross_dkv16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];   // lse, delta

@@ -769,7 +769,7 @@ int mignn_rotary(const void* x, int64_t ldt, int64_t ldh, int64_t n, int heads, 
  * tile, rows, whole} (the last three: for mignn_cross_pass).
  * The caller copies them to the device. */
 #define MIGNN_CROSS_MAX_D 128
-#define MIGNN_CROSS_MAX_GROUP 64          /* query heads a key head */
+#define MIGNN_CROSS_MAX_GROUP 32          /* query heads a key head */
 #define MIGNN_CROSS_MAX_STRIDE (1 << 23)  /* of rows and heads, elements */
 #define MIGNN_CROSS_ITEM_BYTES 32
 enum { MIGNN_CROSS_FORWARD = 0, MIGNN_CROSS_DQ = 1, MIGNN_CROSS_DKV = 2 };

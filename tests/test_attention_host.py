@@ -63,7 +63,7 @@ def test_cross_plan_refusals():
             ([1.5], [2], ok, ValueError, "whole numbers"),
             ([1], [1], dict(ok, kv_heads=3), ValueError, "4 query heads over 3"),
             ([1], [1], dict(ok, heads=0), ValueError, "0 query heads"),
-            ([1], [1], dict(ok, heads=65, kv_heads=1), ValueError, "more than 64"),
+            ([1], [1], dict(ok, heads=33, kv_heads=1), ValueError, "more than 32"),
             ([1], [1], dict(ok, head_dim=12), ValueError, "head_dim"),
             ([1], [1], dict(ok, head_dim=136), ValueError, "head_dim"),
             ([1], [1], dict(ok, head_dim=0), ValueError, "head_dim"),
