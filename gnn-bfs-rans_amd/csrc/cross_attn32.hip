@@ -20,6 +20,8 @@ namespace {
 
 using B = bf16_t;
 
+constexpr int KT = 32;   // rows of an LDS tile
+
 // (two numbers at a time: one conversion instruction makes a pair)
 __device__ __forceinline__ void split2(float a, float b, uint32_t& h, uint32_t& m, uint32_t& l) {
     typedef B pair __attribute__((ext_vector_type(2)));
@@ -74,7 +76,7 @@ __device__ __forceinline__ Frag3 split_acc(const f32x16& w, int t) {
 }
 
 // One thread's share of KT rows of fp32, split at the store into three tiles
-template <int DP, int KT, int NT>
+template <int DP, int NT>
 struct Stage3 {
     static constexpr int C4 = DP / 4, N = KT * C4 / NT, TILE = KT * pitch<DP>();
     static_assert(KT * C4 % NT == 0, "tile share");
@@ -99,7 +101,7 @@ struct Stage3 {
             v[j] = raw_buffer_load_f32x4(rsrc, left >= KT || row(j) < left ? off[j] : NO_LOAD, 0, 0);
     }
     // rows whose bit is clear as zeros
-    __device__ __forceinline__ void write(char* tile, uint64_t keep) {
+    __device__ __forceinline__ void write(char* tile, uint32_t keep) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             if (!((keep >> row(j)) & 1u)) v[j] = f32x4{};
@@ -114,24 +116,25 @@ struct Stage3 {
     }
 };
 
-template <int DP, int KT>
-__device__ __forceinline__ Frag3 row3(const char* tile, int r, int i, int col, int half) {
+template <int DP>
+__device__ __forceinline__ Frag3 row3(const char* tile, int i, int col, int half) {
     constexpr int TILE = KT * pitch<DP>();
-    return {row_frag<B, DP>(tile, r, i, col, half), row_frag<B, DP>(tile + TILE, r, i, col, half),
-            row_frag<B, DP>(tile + 2 * TILE, r, i, col, half)};
+    return {row_frag<B, DP>(tile, 0, i, col, half), row_frag<B, DP>(tile + TILE, 0, i, col, half),
+            row_frag<B, DP>(tile + 2 * TILE, 0, i, col, half)};
 }
-template <int DP, int KT>
+template <int DP>
 __device__ __forceinline__ Frag3 tr3(const char* tile, int trl, int row, int b) {
     constexpr int TILE = KT * pitch<DP>();
     return {tr_frag<B, DP>(tile, trl, row, b), tr_frag<B, DP>(tile + TILE, trl, row, b),
             tr_frag<B, DP>(tile + 2 * TILE, trl, row, b)};
 }
 
-// KT keys a tile: 64 at the narrowest heads, else 32 (three tiles each of K
-// and V, twice: 74 to 111 KB of LDS)
-template <int DP, int KT, int NW>
-__global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_fwd32_kernel(CrossArgs a) {
-    constexpr int TILE3 = 3 * KT * pitch<DP>(), NT = NW * 64, KB = KT / 32;
+// (three tiles each of K and V, twice: 37 KB of LDS for heads of 32, 111 KB for
+// 128; 64 keys a tile measured 5 % slower)
+template <int DP, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP <= 32 ? 3 : DP <= 64 ? 2 : 1) void cross_fwd32_kernel(
+    CrossArgs a) {
+    constexpr int TILE3 = 3 * KT * pitch<DP>(), NT = NW * 64;
     constexpr f32x16 zero = {};
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE3];   // K, V; twice
     int item, kvh;
@@ -150,12 +153,11 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_fwd
     float m = -INFINITY, l = 0.f;   // m: the maximum in use, raw scores
     const float* kbase = static_cast<const float*>(a.k) + kvh * a.ldkh;
     const float* vbase = static_cast<const float*>(a.v) + kvh * a.ldvh;
-    Stage3<DP, KT, NT> sk, sv;
+    Stage3<DP, NT> sk, sv;
     sk.init(a.ldk, 0, 1, a.d);
     sv.init(a.ldv, 0, 1, a.d);
     KeyBits kb;
-    constexpr uint64_t ALL = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
-    uint64_t bits;
+    uint32_t bits;
     auto load = [&](int k0) {
         const int64_t key0 = it.k_begin + static_cast<int64_t>(k0);
         const int left = it.c1 - k0 < KT ? it.c1 - k0 : KT;
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_fwd
         sv.load(vbase + key0 * a.ldv, left);
     };
     auto write = [&](int buf) {
-        bits = kb.bits(lane);
+        bits = static_cast<uint32_t>(kb.bits(lane));
         sk.write(lds + buf * 2 * TILE3, bits);
         sv.write(lds + buf * 2 * TILE3 + TILE3, bits);
     };
@@ -177,21 +179,19 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_fwd
         const char* vt = kt + TILE3;
         const bool more = k0 + KT < it.c1;
         if (more) load(k0 + KT);
-        f32x16 s[KB];
+        f32x16 s;
 #pragma unroll
-        for (int hb = 0; hb < KB; ++hb)
+        for (int i = 0; i < DP / 16; ++i)
+            s = mfma3(row3<DP>(kt, i, col, half), qf[i], i == 0 ? zero : s);
+        if (bits != ~0u) {
+            const uint32_t mine = bits >> (4 * half);
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i)
-                s[hb] = mfma3(row3<DP, KT>(kt, 32 * hb, i, col, half), qf[i], i == 0 ? zero : s[hb]);
-        if (bits != ALL) {
-            const uint64_t mine = bits >> (4 * half);
-#pragma unroll
-            for (int r = 0; r < 16 * KB; ++r)
-                if (!((mine >> (32 * (r >> 4) + acc_row(r & 15))) & 1u)) s[r >> 4][r & 15] = -INFINITY;
+            for (int r = 0; r < 16; ++r)
+                if (!((mine >> acc_row(r)) & 1u)) s[r] = -INFINITY;
         }
-        float mx = s[0][0];
+        float mx = s[0];
 #pragma unroll
-        for (int r = 1; r < 16 * KB; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
         mx = swap_max(mx);
         if (__any((mx - m) * a.c > MAX_SLACK)) {
             const float mn = fmaxf(m, mx);
@@ -204,17 +204,16 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_fwd
         const float shift = -(m == -INFINITY ? 0.f : m) * a.c;
         float sum = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16 * KB; ++r) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[r >> 4][r & 15], a.c, shift));
-            s[r >> 4][r & 15] = p;
-            sum += p;
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, shift));
+            sum += s[r];
         }
         l += sum;
 #pragma unroll
-        for (int t = 0; t < KT / 16; ++t) {
-            const Frag3 p = split_acc(s[t >> 1], t & 1);
+        for (int t = 0; t < 2; ++t) {
+            const Frag3 p = split_acc(s, t);
 #pragma unroll
-            for (int b = 0; b < DP / 32; ++b) o[b] = mfma3(tr3<DP, KT>(vt, trl, 16 * t, b), p, o[b]);
+            for (int b = 0; b < DP / 32; ++b) o[b] = mfma3(tr3<DP>(vt, trl, 16 * t, b), p, o[b]);
         }
         if (more) write(buf ^ 1);
         __syncthreads();
@@ -237,7 +236,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_fwd
 
 template <int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq32_kernel(CrossArgs a) {
-    constexpr int KT = 32, TILE3 = 3 * KT * pitch<DP>(), NT = NW * 64;
+    constexpr int TILE3 = 3 * KT * pitch<DP>(), NT = NW * 64;
     constexpr f32x16 zero = {};
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE3];   // K, V; twice
     int item, kvh;
@@ -274,11 +273,11 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq3
     f32x16 acc[DP / 32] = {};
     const float* kbase = static_cast<const float*>(a.k) + kvh * a.ldkh;
     const float* vbase = static_cast<const float*>(a.v) + kvh * a.ldvh;
-    Stage3<DP, KT, NT> sk, sv;
+    Stage3<DP, NT> sk, sv;
     sk.init(a.ldk, 0, 1, a.d);
     sv.init(a.ldv, 0, 1, a.d);
     KeyBits kb;
-    uint64_t bits;
+    uint32_t bits;
     auto load = [&](int k0) {
         const int64_t key0 = it.k_begin + static_cast<int64_t>(k0);
         const int left = it.c1 - k0 < KT ? it.c1 - k0 : KT;
@@ -287,7 +286,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq3
         sv.load(vbase + key0 * a.ldv, left);
     };
     auto write = [&](int buf) {
-        bits = kb.bits(lane);
+        bits = static_cast<uint32_t>(kb.bits(lane));
         sk.write(lds + buf * 2 * TILE3, bits);
         sv.write(lds + buf * 2 * TILE3 + TILE3, bits);
     };
@@ -303,10 +302,10 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq3
         f32x16 s, dp;
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            s = mfma3(row3<DP, KT>(kt, 0, i, col, half), qf[i], i == 0 ? zero : s);
-            dp = mfma3(row3<DP, KT>(vt, 0, i, col, half), gf[i], i == 0 ? zero : dp);
+            s = mfma3(row3<DP>(kt, i, col, half), qf[i], i == 0 ? zero : s);
+            dp = mfma3(row3<DP>(vt, i, col, half), gf[i], i == 0 ? zero : dp);
         }
-        const uint32_t mine = static_cast<uint32_t>(bits) >> (4 * half);
+        const uint32_t mine = bits >> (4 * half);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
@@ -316,7 +315,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq3
         for (int t = 0; t < 2; ++t) {
             const Frag3 p = split_acc(s, t);
 #pragma unroll
-            for (int b = 0; b < DP / 32; ++b) acc[b] = mfma3(tr3<DP, KT>(kt, trl, 16 * t, b), p, acc[b]);
+            for (int b = 0; b < DP / 32; ++b) acc[b] = mfma3(tr3<DP>(kt, trl, 16 * t, b), p, acc[b]);
         }
         if (more) write(buf ^ 1);
         __syncthreads();
@@ -333,7 +332,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq3
 
 template <int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv32_kernel(CrossArgs a) {
-    constexpr int KT = 32, TILE3 = 3 * KT * pitch<DP>(), NT = NW * 64;
+    constexpr int TILE3 = 3 * KT * pitch<DP>(), NT = NW * 64;
     constexpr f32x16 zero = {};
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE3];   // q, do; twice
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];    // lse, delta
@@ -351,7 +350,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv
     f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
     const float* qbase = static_cast<const float*>(a.q) + it.q_begin * a.ldq + kvh * a.group * a.ldqh;
     const float* gbase = static_cast<const float*>(a.dout) + it.q_begin * a.lddo + kvh * a.group * a.lddoh;
-    Stage3<DP, KT, NT> sq, sg;
+    Stage3<DP, NT> sq, sg;
     sq.init(a.ldq, a.ldqh, a.group, a.d);
     sg.init(a.lddo, a.lddoh, a.group, a.d);
     // whole queries a tile: the offsets are the same in every tile
@@ -373,8 +372,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv
         }
     };
     auto write = [&](int buf) {
-        sq.write(lds + buf * 2 * TILE3, ~0ull);
-        sg.write(lds + buf * 2 * TILE3 + TILE3, ~0ull);
+        sq.write(lds + buf * 2 * TILE3, ~0u);
+        sg.write(lds + buf * 2 * TILE3 + TILE3, ~0u);
         if (threadIdx.x < KT) st[buf][0][threadIdx.x] = lse, st[buf][1][threadIdx.x] = delta;
     };
     int r0 = it.c0, t0 = it.c0 / a.group, buf = 0;
@@ -389,8 +388,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv
         f32x16 s, dp;
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            s = mfma3(row3<DP, KT>(qt, 0, i, col, half), kf[i], i == 0 ? zero : s);
-            dp = mfma3(row3<DP, KT>(gt, 0, i, col, half), vf[i], i == 0 ? zero : dp);
+            s = mfma3(row3<DP>(qt, i, col, half), kf[i], i == 0 ? zero : s);
+            dp = mfma3(row3<DP>(gt, i, col, half), vf[i], i == 0 ? zero : dp);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -408,8 +407,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv
             const Frag3 p = split_acc(s, t), ds = split_acc(dp, t);
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b) {
-                dv[b] = mfma3(tr3<DP, KT>(gt, trl, 16 * t, b), p, dv[b]);
-                dk[b] = mfma3(tr3<DP, KT>(qt, trl, 16 * t, b), ds, dk[b]);
+                dv[b] = mfma3(tr3<DP>(gt, trl, 16 * t, b), p, dv[b]);
+                dk[b] = mfma3(tr3<DP>(qt, trl, 16 * t, b), ds, dk[b]);
             }
         }
         if (more) write(buf ^ 1);
@@ -437,10 +436,9 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv
 
 template <int DP, int NW>
 void launch32(const CrossArgs& a, int pass, hipStream_t st) {
-    constexpr int KT = DP == 32 && NW == 4 ? 64 : 32;
     const dim3 grid(cross_grid(a)), block(NW * 64);
     if (pass == MIGNN_CROSS_FORWARD)
-        hipLaunchKernelGGL((cross_fwd32_kernel<DP, KT, NW>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((cross_fwd32_kernel<DP, NW>), grid, block, 0, st, a);
     else if (pass == MIGNN_CROSS_DQ)
         hipLaunchKernelGGL((cross_dq32_kernel<DP, NW>), grid, block, 0, st, a);
     else
