@@ -165,16 +165,21 @@ struct Sequence {
 int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 
 // Tile: 8 rows where no sequence has more (forward: cross_few), 32 (one wave)
-// where none has more than 32, else 128, four waves that share the staging of
-// the other side.  (32 for longer sequences saves padding but not time: LDS
+// where none has more than 32 or there are few results of 16 bits (those tiles
+// are the exacter ones), else 128, four waves that share the staging of the
+// other side.  (32 for longer sequences saves padding but not time: LDS
 // holds few such workgroups; keys of three sequences of 78, 134 and 167: dk /
 // dv 108 us in tiles of 32, 61 in tiles of 128.)
 PassShape pass_shape(const Sequence* seq, int64_t batch, int pass, int d, int dtype, int group) {
     const bool dkv = pass == MIGNN_CROSS_DKV;
     PassShape s{128, 0, 512, 256, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
-    for (int64_t b = 0; b < batch; ++b) s.longest = seq[b].rn > s.longest ? seq[b].rn : s.longest;
+    int64_t results = 0;   // of one kv head
+    for (int64_t b = 0; b < batch; ++b) {
+        s.longest = seq[b].rn > s.longest ? seq[b].rn : s.longest;
+        results += seq[b].rn * d;
+    }
     if (pass == MIGNN_CROSS_FORWARD && s.longest <= CROSS_FEW) s.tile = CROSS_FEW;
-    else if (s.longest <= CROSS_ROWS) s.tile = CROSS_ROWS;
+    else if (s.longest <= CROSS_ROWS || (dtype != MIGNN_ROW_F32 && results < 16384)) s.tile = CROSS_ROWS;
     // registers and LDS: two workgroups of four waves a CU, one where the heads
     // are wide and much is held in fp32; eight small ones
     const bool wide = dtype == MIGNN_ROW_F32 ? d > 64 || (dkv && d > 32) : dkv && d > 96;

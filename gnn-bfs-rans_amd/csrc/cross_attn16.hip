@@ -1,8 +1,7 @@
 // Cross attention of bf16 and fp16 rows on the 16-bit matrix instructions
 // (formulas and pass structure: cross_attn.hip).
 //
-// A wave owns CB blocks of 32 rows (forward, dq) or keys (dk / dv) as MFMA
-// columns.  The other side comes in LDS tiles of 64, double buffered through
+// A wave owns 32 rows (forward, dq) or keys (dk / dv) as MFMA columns.  The other side comes in LDS tiles of 64, double buffered through
 // registers: while a tile is worked on, the next one's rows are in flight.
 //   S^T (keys x rows)   A = key rows, 16 bytes a lane;  B = q, in registers
 //   O^T (d x rows)      A = V^T, read transposed from the row-major tile
@@ -13,8 +12,10 @@
 // dq and dk / dv are made of the same two forms.
 //
 // P and dS are rounded to the rows' type ahead of their second product (the
-// matrix instruction takes both operands in one type); statistics, sums and
-// accumulators are fp32.  bf16 has fp32's range.  fp16 has not: a weight of
+// matrix instruction takes both operands in one type), which adds to a result
+// about what its own rounding does; statistics, sums and accumulators are fp32.
+// Tiles of 32 (few rows or few results: bound by latency, not by the matrix
+// unit) carry the roundings' remainders through a second product instead.  bf16 has fp32's range.  fp16 has not: a weight of
 // 1 / 5000 is already subnormal there, so P is carried up by a constant power
 // of two and dS by one that each row (dq) or key (dk) lowers when its values
 // would not fit (DsScale); the results are brought back in fp32.
@@ -43,6 +44,15 @@ __device__ __forceinline__ vec8<T> pack8(const f32x16& w, int t) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(w[8 * t + i]);
     return v;
+}
+
+// what pack8's rounding left, rounded
+template <typename T>
+__device__ __forceinline__ vec8<T> rest8(const f32x16& w, const vec8<T>& v, int t) {
+    vec8<T> x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<T>(w[8 * t + i] - static_cast<float>(v[i]));
+    return x;
 }
 
 // One thread's share of a 64-row tile on its way from memory to LDS: buffer
@@ -128,7 +138,7 @@ struct DsScale {
     __device__ __forceinline__ float back() const { return NARROW<T> ? __builtin_amdgcn_exp2f(-up) : 1.f; }
 };
 
-template <typename T, int DP, int NW, int CB>
+template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];   // K, V; twice
@@ -138,22 +148,15 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
     constexpr f32x16 zero = {};
-    vec8<T> qf[CB][DP / 16];
-    int row[CB];
-    int64_t at[CB];
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        row[cb] = it.r0 + (wave * CB + cb) * 32 + col;
-        const int t = row[cb] / a.group, h = kvh * a.group + row[cb] - t * a.group;
-        const int64_t token = it.q_begin + static_cast<int64_t>(t);
-        at[cb] = token * a.heads + h;
-        load_frag16<T, DP>(qf[cb], row[cb] < it.r1 ? static_cast<const T*>(a.q) + token * a.ldq + h * a.ldqh
-                                                   : nullptr, a.d, half);
-    }
-    f32x16 o[CB][DP / 32] = {};
-    float m[CB], l[CB];   // m: the maximum in use, raw scores
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) m[cb] = -INFINITY, l[cb] = 0.f;
+    vec8<T> qf[DP / 16];
+    const int row = it.r0 + wave * 32 + col;
+    const int t = row / a.group, h = kvh * a.group + row - t * a.group;
+    const int64_t token = it.q_begin + static_cast<int64_t>(t);
+    const int64_t at = token * a.heads + h;
+    load_frag16<T, DP>(qf, row < it.r1 ? static_cast<const T*>(a.q) + token * a.ldq + h * a.ldqh
+                                               : nullptr, a.d, half);
+    f32x16 o[DP / 32] = {};
+    float m = -INFINITY, l = 0.f;   // m: the maximum in use, raw scores
     const T* kbase = static_cast<const T*>(a.k) + kvh * a.ldkh;
     const T* vbase = static_cast<const T*>(a.v) + kvh * a.ldvh;
     Stage<T, DP, NT> sk, sv;
@@ -184,14 +187,13 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd
             sk.load(kbase + key0 * a.ldk, left);
             sv.load(vbase + key0 * a.ldv, left);
         }
-        f32x16 s[CB][2];
+        f32x16 s[2];
 #pragma unroll
         for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const vec8<T> f = row_frag<T, DP>(kt, 32 * hb, i, col, half);
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb) s[cb][hb] = mfma16(f, qf[cb][i], i == 0 ? zero : s[cb][hb]);
+                s[hb] = mfma16(f, qf[i], i == 0 ? zero : s[hb]);
             }
         if (bits != ~0ull) {
             const uint64_t mine = bits >> (4 * half);
@@ -199,46 +201,39 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd
             for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (!((mine >> (32 * hb + acc_row(r))) & 1u)) {
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) s[cb][hb][r] = -INFINITY;
-                    }
+                    if (!((mine >> (32 * hb + acc_row(r))) & 1u)) s[hb][r] = -INFINITY;
         }
+        float mx = s[0][0];
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-            float mx = s[cb][0][0];
+        for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
+        mx = swap_max(mx);
+        // (m = -inf: any score raises it)
+        if (__any((mx - m) * a.c > MAX_SLACK)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+            m = mn;
+            l *= alpha;
 #pragma unroll
-            for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[cb][r >> 4][r & 15]);
-            mx = swap_max(mx);
-            // (m = -inf: any score raises it)
-            if (__any((mx - m[cb]) * a.c > MAX_SLACK)) {
-                const float mn = fmaxf(m[cb], mx);
-                const float alpha = m[cb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[cb] - mn) * a.c);
-                m[cb] = mn;
-                l[cb] *= alpha;
-#pragma unroll
-                for (int b = 0; b < DP / 32; ++b) o[cb][b] *= alpha;
-            }
-            const float shift = P_UP<T> - (m[cb] == -INFINITY ? 0.f : m[cb]) * a.c;
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 32; ++r) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[cb][r >> 4][r & 15], a.c, shift));
-                s[cb][r >> 4][r & 15] = p;
-                sum += p;
-            }
-            l[cb] += sum;
+            for (int b = 0; b < DP / 32; ++b) o[b] *= alpha;
         }
+        const float shift = P_UP<T> - (m == -INFINITY ? 0.f : m) * a.c;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[r >> 4][r & 15], a.c, shift));
+            s[r >> 4][r & 15] = p;
+            sum += p;
+        }
+        l += sum;
 #pragma unroll
         for (int t = 0; t < KT / 16; ++t) {
-            vec8<T> p[CB];
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) p[cb] = pack8<T>(s[cb][t >> 1], t & 1);
+            const vec8<T> p = pack8<T>(s[t >> 1], t & 1);
+            const vec8<T> rest = NW == 1 ? rest8<T>(s[t >> 1], p, t & 1) : p;
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b) {
                 const vec8<T> f = tr_frag<T, DP>(vt, trl, 16 * t, b);
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb) o[cb][b] = mfma16(f, p[cb], o[cb][b]);
+                if constexpr (NW == 1) o[b] = mfma16(f, rest, o[b]);
+                o[b] = mfma16(f, p, o[b]);
             }
         }
         if (more) {
@@ -250,27 +245,24 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd
         __syncthreads();
         buf ^= 1;
     }
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        const float sum = swap_add(l[cb]);
-        if (row[cb] >= it.r1) continue;
-        const float m2 = (m[cb] == -INFINITY ? 0.f : m[cb]) * a.c - P_UP<T>;
-        if (it.slot >= 0) {
-            float* p = a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
-                                 row[cb] - it.r0) * (a.d + 2);
-            store_acc<float, DP>(p, o[cb], 1.f, a.d, half);
-            if (half == 0) p[a.d] = m[cb] == -INFINITY ? -INFINITY : m2;
-            else p[a.d + 1] = sum;
-            continue;
-        }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        store_acc<T, DP>(static_cast<T*>(a.out) + at[cb] * a.d, o[cb], inv, a.d, half);
-        if (a.o32) store_acc<float, DP>(a.o32 + at[cb] * a.d, o[cb], inv, a.d, half);
-        if (a.lse && half == 0) a.lse[at[cb]] = sum == 0.f ? INFINITY : m2 + log2f(sum);
+    const float sum = swap_add(l);
+    if (row >= it.r1) return;
+    const float m2 = (m == -INFINITY ? 0.f : m) * a.c - P_UP<T>;
+    if (it.slot >= 0) {
+        float* p = a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * 32) +
+                             row - it.r0) * (a.d + 2);
+        store_acc<float, DP>(p, o, 1.f, a.d, half);
+        if (half == 0) p[a.d] = m == -INFINITY ? -INFINITY : m2;
+        else p[a.d + 1] = sum;
+        return;
     }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    store_acc<T, DP>(static_cast<T*>(a.out) + at * a.d, o, inv, a.d, half);
+    if (a.o32) store_acc<float, DP>(a.o32 + at * a.d, o, inv, a.d, half);
+    if (a.lse && half == 0) a.lse[at] = sum == 0.f ? INFINITY : m2 + log2f(sum);
 }
 
-template <typename T, int DP, int NW, int CB>
+template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_dq16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
@@ -280,40 +272,34 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_dq1
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
     constexpr f32x16 zero = {};
-    vec8<T> qf[CB][DP / 16], gf[CB][DP / 16];
-    int row[CB];
-    int64_t at[CB];
-    float lse[CB], delta[CB];
+    vec8<T> qf[DP / 16], gf[DP / 16];
+    const int row = it.r0 + wave * 32 + col;
+    const bool live = row < it.r1;
+    const int t = row / a.group, h = kvh * a.group + row - t * a.group;
+    const int64_t token = it.q_begin + static_cast<int64_t>(t);
+    const int64_t at = token * a.heads + h;
+    load_frag16<T, DP>(qf, live ? static_cast<const T*>(a.q) + token * a.ldq + h * a.ldqh : nullptr,
+                       a.d, half);
+    load_frag16<T, DP>(gf, live ? static_cast<const T*>(a.dout) + token * a.lddo + h * a.lddoh
+                                    : nullptr, a.d, half);
+    float del = 0.f;
+    if (live) {
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        row[cb] = it.r0 + (wave * CB + cb) * 32 + col;
-        const bool live = row[cb] < it.r1;
-        const int t = row[cb] / a.group, h = kvh * a.group + row[cb] - t * a.group;
-        const int64_t token = it.q_begin + static_cast<int64_t>(t);
-        at[cb] = token * a.heads + h;
-        load_frag16<T, DP>(qf[cb], live ? static_cast<const T*>(a.q) + token * a.ldq + h * a.ldqh : nullptr,
-                           a.d, half);
-        load_frag16<T, DP>(gf[cb], live ? static_cast<const T*>(a.dout) + token * a.lddo + h * a.lddoh
-                                        : nullptr, a.d, half);
-        float del = 0.f;
-        if (live) {
+        for (int i = 0; i < DP / 16; ++i) {
+            const int c = 16 * i + 8 * half;
+            if (c >= a.d) continue;
+            const float4 x = ld4(a.out32 + at * a.d + c), y = ld4(a.out32 + at * a.d + c + 4);
+            const float ov[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
-                const int c = 16 * i + 8 * half;
-                if (c >= a.d) continue;
-                const float4 x = ld4(a.out32 + at[cb] * a.d + c), y = ld4(a.out32 + at[cb] * a.d + c + 4);
-                const float ov[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) del = fmaf(ov[e], static_cast<float>(gf[cb][i][e]), del);
-            }
+            for (int e = 0; e < 8; ++e) del = fmaf(ov[e], static_cast<float>(gf[i][e]), del);
         }
-        delta[cb] = swap_add(del);
-        // the dk / dv kernel's: written by the item of the row's first keys
-        if (live && half == 0 && it.c0 == 0) a.delta[at[cb]] = delta[cb];
-        lse[cb] = live ? a.lse[at[cb]] : INFINITY;
     }
-    f32x16 acc[CB][DP / 32] = {};
-    DsScale<T> sc[CB];
+    const float delta = swap_add(del);
+    // the dk / dv kernel's: written by the item of the row's first keys
+    if (live && half == 0 && it.c0 == 0) a.delta[at] = delta;
+    const float lse = live ? a.lse[at] : INFINITY;
+    f32x16 acc[DP / 32] = {};
+    DsScale<T> sc;
     const T* kbase = static_cast<const T*>(a.k) + kvh * a.ldkh;
     const T* vbase = static_cast<const T*>(a.v) + kvh * a.ldvh;
     Stage<T, DP, NT> sk, sv;
@@ -346,44 +332,34 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_dq1
         }
 #pragma unroll
         for (int hb = 0; hb < 2; ++hb) {
-            f32x16 s[CB], dp[CB];
+            f32x16 s, dp;
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const vec8<T> fk = row_frag<T, DP>(kt, 32 * hb, i, col, half);
                 const vec8<T> fv = row_frag<T, DP>(vt, 32 * hb, i, col, half);
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb) {
-                    s[cb] = mfma16(fk, qf[cb][i], i == 0 ? zero : s[cb]);
-                    dp[cb] = mfma16(fv, gf[cb][i], i == 0 ? zero : dp[cb]);
-                }
+                s = mfma16(fk, qf[i], i == 0 ? zero : s);
+                dp = mfma16(fv, gf[i], i == 0 ? zero : dp);
             }
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s[cb][r] = __builtin_amdgcn_exp2f(fmaf(s[cb][r], a.c, sc[cb].up - lse[cb])) *
-                               (dp[cb][r] - delta[cb]);
+                    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, sc.up - lse)) *
+                               (dp[r] - delta);
             if (bits != ~0ull) {
                 const uint32_t mine = static_cast<uint32_t>(bits >> (32 * hb + 4 * half));
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (!((mine >> acc_row(r)) & 1u)) {
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) s[cb][r] = 0.f;
-                    }
+                    if (!((mine >> acc_row(r)) & 1u)) s[r] = 0.f;
             }
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) sc[cb].fit(s[cb], acc[cb]);
+            sc.fit(s, acc);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                vec8<T> p[CB];
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb) p[cb] = pack8<T>(s[cb], t);
+                const vec8<T> p = pack8<T>(s, t);
+                const vec8<T> rest = NW == 1 ? rest8<T>(s, p, t) : p;
 #pragma unroll
                 for (int b = 0; b < DP / 32; ++b) {
                     const vec8<T> f = tr_frag<T, DP>(kt, trl, 32 * hb + 16 * t, b);
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) acc[cb][b] = mfma16(f, p[cb], acc[cb][b]);
+                    if constexpr (NW == 1) acc[b] = mfma16(f, rest, acc[b]);
+                    acc[b] = mfma16(f, p, acc[b]);
                 }
             }
         }
@@ -396,19 +372,16 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_dq1
         __syncthreads();
         buf ^= 1;
     }
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        if (row[cb] >= it.r1) continue;
-        const float f = a.scale * sc[cb].back();
-        if (it.slot >= 0)
-            store_acc<float, DP>(a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
-                                             row[cb] - it.r0) * a.d, acc[cb], f, a.d, half);
-        else
-            store_acc<T, DP>(static_cast<T*>(a.out) + at[cb] * a.d, acc[cb], f, a.d, half);
-    }
+    if (row >= it.r1) return;
+    const float f = a.scale * sc.back();
+    if (it.slot >= 0)
+        store_acc<float, DP>(a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * 32) +
+                                         row - it.r0) * a.d, acc, f, a.d, half);
+    else
+        store_acc<T, DP>(static_cast<T*>(a.out) + at * a.d, acc, f, a.d, half);
 }
 
-template <typename T, int DP, int NW, int CB>
+template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cross_dkv16_kernel(CrossArgs a) {
     constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
@@ -419,24 +392,17 @@ __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cro
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     const int trl = tr_lane<DP>(lane);
     constexpr f32x16 zero = {};
-    vec8<T> kf[CB][DP / 16], vf[CB][DP / 16];
-    int key[CB];
-    bool keep[CB];
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        key[cb] = it.r0 + (wave * CB + cb) * 32 + col;
-        const int64_t kt = it.k_begin + static_cast<int64_t>(key[cb]);
-        keep[cb] = key[cb] < it.r1 && (!a.mask || a.mask[kt]);
-        load_frag16<T, DP>(kf[cb], keep[cb] ? static_cast<const T*>(a.k) + kt * a.ldk + kvh * a.ldkh : nullptr,
-                           a.d, half);
-        load_frag16<T, DP>(vf[cb], keep[cb] ? static_cast<const T*>(a.v) + kt * a.ldv + kvh * a.ldvh : nullptr,
-                           a.d, half);
-    }
-    f32x16 dk[CB][DP / 32] = {}, dv[CB][DP / 32] = {};
-    DsScale<T> sc[CB];
-    float gain[CB];   // dS's power of two over P's
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) gain[cb] = __builtin_amdgcn_exp2f(sc[cb].up - PB_UP<T>);
+    vec8<T> kf[DP / 16], vf[DP / 16];
+    const int key = it.r0 + wave * 32 + col;
+    const int64_t kt = it.k_begin + static_cast<int64_t>(key);
+    const bool keep = key < it.r1 && (!a.mask || a.mask[kt]);
+    load_frag16<T, DP>(kf, keep ? static_cast<const T*>(a.k) + kt * a.ldk + kvh * a.ldkh : nullptr,
+                       a.d, half);
+    load_frag16<T, DP>(vf, keep ? static_cast<const T*>(a.v) + kt * a.ldv + kvh * a.ldvh : nullptr,
+                       a.d, half);
+    f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+    DsScale<T> sc;
+    float gain = __builtin_amdgcn_exp2f(sc.up - PB_UP<T>);   // dS's power of two over P's
     const T* qbase = static_cast<const T*>(a.q) + it.q_begin * a.ldq + kvh * a.group * a.ldqh;
     const T* gbase = static_cast<const T*>(a.dout) + it.q_begin * a.lddo + kvh * a.group * a.lddoh;
     Stage<T, DP, NT> sq, sg;
@@ -477,16 +443,13 @@ __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cro
         if (more) load(r0 + step, t0 + tokens);
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
-            f32x16 s[CB], dp[CB];
+            f32x16 s, dp;
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const vec8<T> fq = row_frag<T, DP>(qt, 32 * rb, i, col, half);
                 const vec8<T> fg = row_frag<T, DP>(gt, 32 * rb, i, col, half);
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb) {
-                    s[cb] = mfma16(fq, kf[cb][i], i == 0 ? zero : s[cb]);
-                    dp[cb] = mfma16(fg, vf[cb][i], i == 0 ? zero : dp[cb]);
-                }
+                s = mfma16(fq, kf[i], i == 0 ? zero : s);
+                dp = mfma16(fg, vf[i], i == 0 ? zero : dp);
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -496,34 +459,27 @@ __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cro
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * g + e;
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) {
-                        s[cb][r] = __builtin_amdgcn_exp2f(fmaf(s[cb][r], a.c, -lv[e]));
-                        dp[cb][r] = s[cb][r] * (dp[cb][r] - ev[e]);
-                        if constexpr (NARROW<T>) dp[cb][r] *= gain[cb];
-                    }
+                    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lv[e]));
+                    dp[r] = s[r] * (dp[r] - ev[e]);
+                    if constexpr (NARROW<T>) dp[r] *= gain;
                 }
             }
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
-                if (sc[cb].fit(dp[cb], dk[cb])) gain[cb] = __builtin_amdgcn_exp2f(sc[cb].up - PB_UP<T>);
+            if (sc.fit(dp, dk)) gain = __builtin_amdgcn_exp2f(sc.up - PB_UP<T>);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                vec8<T> p[CB], ds[CB];
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb) {
-                    p[cb] = pack8<T>(s[cb], t);
-                    ds[cb] = pack8<T>(dp[cb], t);
-                }
+                const vec8<T> p = pack8<T>(s, t), ds = pack8<T>(dp, t);
+                const vec8<T> p_rest = NW == 1 ? rest8<T>(s, p, t) : p;
+                const vec8<T> ds_rest = NW == 1 ? rest8<T>(dp, ds, t) : ds;
 #pragma unroll
                 for (int b = 0; b < DP / 32; ++b) {
                     const vec8<T> fg = tr_frag<T, DP>(gt, trl, 32 * rb + 16 * t, b);
                     const vec8<T> fq = tr_frag<T, DP>(qt, trl, 32 * rb + 16 * t, b);
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) {
-                        dv[cb][b] = mfma16(fg, p[cb], dv[cb][b]);
-                        dk[cb][b] = mfma16(fq, ds[cb], dk[cb][b]);
+                    if constexpr (NW == 1) {
+                        dv[b] = mfma16(fg, p_rest, dv[b]);
+                        dk[b] = mfma16(fq, ds_rest, dk[b]);
                     }
+                    dv[b] = mfma16(fg, p, dv[b]);
+                    dk[b] = mfma16(fq, ds, dk[b]);
                 }
             }
         }
@@ -531,43 +487,40 @@ __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cro
         __syncthreads();
         buf ^= 1;
     }
+    if (key >= it.r1) return;
+    // a key that the mask leaves out has no gradient, whatever its rows hold
+    if (!keep) {
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        if (key[cb] >= it.r1) continue;
-        // a key that the mask leaves out has no gradient, whatever its rows hold
-        if (!keep[cb]) {
-#pragma unroll
-            for (int b = 0; b < DP / 32; ++b) dk[cb][b] = dv[cb][b] = f32x16{};
-        }
-        const float fk = a.scale * sc[cb].back(), fv = __builtin_amdgcn_exp2f(-PB_UP<T>);
-        if (it.slot >= 0) {
-            float* p = a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * CB * 32) +
-                                 key[cb] - it.r0) * (2 * a.d);
-            store_acc<float, DP>(p, dk[cb], fk, a.d, half);
-            store_acc<float, DP>(p + a.d, dv[cb], fv, a.d, half);
-        } else {
-            const int64_t at = ((it.k_begin + static_cast<int64_t>(key[cb])) * a.kv_heads + kvh) * a.d;
-            store_acc<T, DP>(static_cast<T*>(a.dk) + at, dk[cb], fk, a.d, half);
-            store_acc<T, DP>(static_cast<T*>(a.dv) + at, dv[cb], fv, a.d, half);
-        }
+        for (int b = 0; b < DP / 32; ++b) dk[b] = dv[b] = f32x16{};
+    }
+    const float fk = a.scale * sc.back(), fv = __builtin_amdgcn_exp2f(-PB_UP<T>);
+    if (it.slot >= 0) {
+        float* p = a.part + ((static_cast<int64_t>(it.slot) * a.kv_heads + kvh) * (NW * 32) +
+                             key - it.r0) * (2 * a.d);
+        store_acc<float, DP>(p, dk, fk, a.d, half);
+        store_acc<float, DP>(p + a.d, dv, fv, a.d, half);
+    } else {
+        const int64_t at = ((it.k_begin + static_cast<int64_t>(key)) * a.kv_heads + kvh) * a.d;
+        store_acc<T, DP>(static_cast<T*>(a.dk) + at, dk, fk, a.d, half);
+        store_acc<T, DP>(static_cast<T*>(a.dv) + at, dv, fv, a.d, half);
     }
 }
 
-template <typename T, int DP, int NW, int CB>
+template <typename T, int DP, int NW>
 void launch16_tile(const CrossArgs& a, int pass, hipStream_t st) {
     const dim3 grid(cross_grid(a)), block(NW * 64);
     if (pass == MIGNN_CROSS_FORWARD)
-        hipLaunchKernelGGL((cross_fwd16_kernel<T, DP, NW, CB>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((cross_fwd16_kernel<T, DP, NW>), grid, block, 0, st, a);
     else if (pass == MIGNN_CROSS_DQ)
-        hipLaunchKernelGGL((cross_dq16_kernel<T, DP, NW, CB>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((cross_dq16_kernel<T, DP, NW>), grid, block, 0, st, a);
     else
-        hipLaunchKernelGGL((cross_dkv16_kernel<T, DP, NW, CB>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((cross_dkv16_kernel<T, DP, NW>), grid, block, 0, st, a);
 }
 
 template <typename T, int DP>
 void launch16(const CrossArgs& a, int pass, hipStream_t st) {
-    if (a.tile == CROSS_ROWS) launch16_tile<T, DP, 1, 1>(a, pass, st);
-    else launch16_tile<T, DP, 4, 1>(a, pass, st);
+    if (a.tile == CROSS_ROWS) launch16_tile<T, DP, 1>(a, pass, st);
+    else launch16_tile<T, DP, 4>(a, pass, st);
 }
 
 template <typename T>
