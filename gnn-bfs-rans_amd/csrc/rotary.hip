@@ -6,10 +6,11 @@
 // A pair is columns (j, j + pairs), or (2j, 2j + 1) when interleaved; columns
 // from 2 pairs on pass through.  The gradient is the rotation by -t.
 //
-// Bound by memory: x read once and y written once.  The angle is formed in
-// fp64 as a number of turns (the table holds f_j / 2 pi), of which the
-// fraction goes to fp32: a far position costs no accuracy, and one thread's
-// sine and cosine serve all heads of a row.
+// Bound by memory: x read once and y written once.  A workgroup takes a run of
+// rows: first the sine and cosine of its rows' angles, once for all heads, into
+// LDS, then the rows in the order of memory, 16 bytes an access.  The angle is
+// formed in fp64 as a number of turns (the table holds f_j / 2 pi), of which
+// the fraction goes to fp32: a far position costs no accuracy.
 #include "row_types.hpp"
 
 namespace mignn {
@@ -21,7 +22,7 @@ struct RotArgs {
     const double* freq;
     const int32_t* axis;
     int64_t ldt, ldh, ldp, ldyt, ldyh, n;
-    int heads, d, pairs, pos_type, chunks, pass;
+    int heads, d, pairs, pos_type, chunks, pass, rows;   // rows of a workgroup
     bool inverse;
 };
 
@@ -35,58 +36,90 @@ __device__ __forceinline__ double load_pos(const RotArgs& a, int64_t row, int ax
     }
 }
 
-// V pairs a thread; chunk c < chunks: pairs, the last chunk ending at the last
-// pair (pairs >= V, or V = 1); the chunks after them: columns passed through.
+// Sine and cosine of f turns, |f| <= 1/2: the nearest quarter turn taken off
+// (exactly), Taylor's polynomials to the 9th and 10th power of what is left
+// (|2 pi r| <= pi / 4: cut off below 2e-9), and the quarter's exchange and signs.
+__device__ __forceinline__ void sincos_turns(float f, float& sn, float& cs) {
+    const float q = rintf(4.f * f), r = fmaf(q, -0.25f, f), z = r * r;
+    const float s = r * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 42.0586939f, -76.7058597f), 81.6052493f),
+                                     -41.3417022f), 6.28318531f);
+    const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -26.4262568f, 60.2446414f), -85.4568172f),
+                                              64.9393940f), -19.7392088f), 1.f);
+    const int n = static_cast<int>(q);
+    sn = n & 1 ? c : s;
+    cs = n & 1 ? s : c;
+    if (n & 2) sn = -sn;
+    if ((n + 1) & 2) cs = -cs;
+}
+
+// V pairs an access; chunk c < chunks of a head: pairs, the last chunk ending
+// at the last pair (pairs >= V, or V = 1); the chunks after them: columns
+// passed through.
 template <typename T, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
-    const int per_row = a.chunks + a.pass;
-    const int64_t total = a.n * per_row;
-    for (int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; t < total;
-         t += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t row = t / per_row;
-        const int c = static_cast<int>(t - row * per_row);
-        const T* x = static_cast<const T*>(a.x) + row * a.ldt;
-        T* y = static_cast<T*>(a.y) + row * a.ldyt;
+    extern __shared__ __attribute__((aligned(16))) float trig[];   // [rows][cos: pairs | sin: pairs]
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.rows;
+    const int rows = a.n - row0 < a.rows ? static_cast<int>(a.n - row0) : a.rows;
+    // a thread keeps its pair and goes through the rows
+    const int lanes = a.pairs < 256 ? a.pairs : 256, step = 256 / lanes;
+    const int first = threadIdx.x / lanes;
+    if (first < step)
+        for (int j = threadIdx.x - first * lanes; j < a.pairs; j += 256) {
+            const int axis = a.axis[j];
+            const double freq = a.freq[j];
+#pragma unroll 4
+            for (int r = first; r < rows; r += step) {
+                const double turns = load_pos(a, row0 + r, axis) * freq;
+                float sn, cs;
+                sincos_turns(static_cast<float>(turns - rint(turns)), sn, cs);
+                trig[2 * r * a.pairs + j] = cs;
+                trig[(2 * r + 1) * a.pairs + j] = a.inverse ? -sn : sn;
+            }
+        }
+    __syncthreads();
+    // (indices carried along: divisions would cost as much as the rest)
+    const int per_head = a.chunks + a.pass, per_row = a.heads * per_head;
+    const int dr = 256 / per_row, du = 256 - dr * per_row, dh = du / per_head, dc = du - dh * per_head;
+    int r = threadIdx.x / per_row, h = (threadIdx.x - r * per_row) / per_head;
+    int c = threadIdx.x - r * per_row - h * per_head;
+    for (; r < rows; r += dr, h += dh, c += dc) {
+        if (c >= per_head) c -= per_head, ++h;
+        if (h >= a.heads) {
+            h -= a.heads;
+            if (++r >= rows) break;
+        }
+        const T* x = static_cast<const T*>(a.x) + (row0 + r) * a.ldt + h * a.ldh;
+        T* y = static_cast<T*>(a.y) + (row0 + r) * a.ldyt + h * a.ldyh;
         if (c >= a.chunks) {
             const int c0 = 2 * a.pairs + (c - a.chunks) * V;
-            for (int h = 0; h < a.heads; ++h)
-                for (int i = c0; i < a.d && i < c0 + V; ++i) y[h * a.ldyh + i] = x[h * a.ldh + i];
+            for (int k = c0; k < a.d && k < c0 + V; ++k) y[k] = x[k];
             continue;
         }
         int j0 = c * V;
         if (j0 > a.pairs - V) j0 = a.pairs - V;
         float cs[V], sn[V];
+        load_row(trig + 2 * r * a.pairs + j0, cs);
+        load_row(trig + (2 * r + 1) * a.pairs + j0, sn);
+        if constexpr (INTERLEAVED) {
+            float v[2 * V], o[2 * V];
+            load_row(x + 2 * j0, v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const double turns = load_pos(a, row, a.axis[j0 + i]) * a.freq[j0 + i];
-            const float f = static_cast<float>(turns - rint(turns));
-            sincospif(2.f * f, &sn[i], &cs[i]);
-            if (a.inverse) sn[i] = -sn[i];
-        }
-        for (int h = 0; h < a.heads; ++h) {
-            const T* xh = x + h * a.ldh;
-            T* yh = y + h * a.ldyh;
-            if constexpr (INTERLEAVED) {
-                float u[2 * V], o[2 * V];
-                load_row(xh + 2 * j0, u);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    o[2 * i] = u[2 * i] * cs[i] - u[2 * i + 1] * sn[i];
-                    o[2 * i + 1] = u[2 * i + 1] * cs[i] + u[2 * i] * sn[i];
-                }
-                store_row(yh + 2 * j0, o);
-            } else {
-                float u[V], v[V], o[V], q[V];
-                load_row(xh + j0, u);
-                load_row(xh + a.pairs + j0, v);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    o[i] = u[i] * cs[i] - v[i] * sn[i];
-                    q[i] = v[i] * cs[i] + u[i] * sn[i];
-                }
-                store_row(yh + j0, o);
-                store_row(yh + a.pairs + j0, q);
+            for (int k = 0; k < V; ++k) {
+                o[2 * k] = v[2 * k] * cs[k] - v[2 * k + 1] * sn[k];
+                o[2 * k + 1] = v[2 * k + 1] * cs[k] + v[2 * k] * sn[k];
             }
+            store_row(y + 2 * j0, o);
+        } else {
+            float v[V], w[V], o[V], q[V];
+            load_row(x + j0, v);
+            load_row(x + a.pairs + j0, w);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                o[k] = v[k] * cs[k] - w[k] * sn[k];
+                q[k] = w[k] * cs[k] + v[k] * sn[k];
+            }
+            store_row(y + j0, o);
+            store_row(y + a.pairs + j0, q);
         }
     }
 }
@@ -98,9 +131,17 @@ int launch_rotary(RotArgs a, bool interleaved, hipStream_t st) {
     const int v = a.pairs < V ? 1 : (interleaved ? V / 2 : V);
     a.chunks = (a.pairs + v - 1) / v;
     a.pass = (a.d - 2 * a.pairs + v - 1) / v;
-    const unsigned grid = grid_for(a.n * (a.chunks + a.pass), 256);
+    // rows of a workgroup: about four accesses a thread, and at most 16 KB of angles
+    const int64_t per_row = static_cast<int64_t>(a.heads) * (a.chunks + a.pass);
+    int64_t rows = (1024 + per_row - 1) / per_row;
+    if (rows > 2048 / a.pairs) rows = 2048 / a.pairs;
+    a.rows = rows < 1 ? 1 : static_cast<int>(rows);
+    const int64_t blocks = (a.n + a.rows - 1) / a.rows;
+    MIGNN_REQUIRE(blocks <= INT32_MAX && per_row <= INT32_MAX / 4096, "rotary: too many rows or heads");
+    const unsigned grid = static_cast<unsigned>(blocks);
+    const size_t lds = static_cast<size_t>(a.rows) * a.pairs * 2 * sizeof(float);
 #define MIGNN_ROT(VV, I) \
-    hipLaunchKernelGGL((rotary_kernel<T, VV, I>), dim3(grid), dim3(256), 0, st, a)
+    hipLaunchKernelGGL((rotary_kernel<T, VV, I>), dim3(grid), dim3(256), lds, st, a)
     if (v == 1) {
         if (interleaved) MIGNN_ROT(1, true);
         else MIGNN_ROT(1, false);
@@ -128,6 +169,8 @@ extern "C" int mignn_rotary(const void* x, int64_t ldt, int64_t ldh, int64_t n, 
     MIGNN_REQUIRE(n >= 0 && heads >= 0 && d > 0 && pairs > 0 && 2 * static_cast<int64_t>(pairs) <= d,
                   "rotary: n = %lld, heads = %d, d = %d, pairs = %d", static_cast<long long>(n),
                   heads, d, pairs);
+    MIGNN_REQUIRE(pairs <= MIGNN_ROTARY_MAX_PAIRS, "rotary: %d pairs (at most %d)", pairs,
+                  MIGNN_ROTARY_MAX_PAIRS);
     if (n == 0 || heads == 0) return MIGNN_OK;
     MIGNN_REQUIRE(x && pos && freq && axis && y, "rotary: null pointer");
     RotArgs a{};

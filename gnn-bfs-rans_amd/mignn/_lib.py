@@ -26,7 +26,7 @@ ROW_F32, ROW_BF16, ROW_F16 = 0, 1, 2
 POS_F32, POS_F64, POS_I32, POS_I64 = 0, 1, 2, 3
 CROSS_FORWARD, CROSS_DQ, CROSS_DKV = 0, 1, 2
 CROSS_MAX_D, CROSS_ITEM_BYTES, RMS_NORM_MAX_H = 128, 32, 2048
-CROSS_MAX_GROUP, CROSS_MAX_STRIDE = 32, 1 << 23
+CROSS_MAX_GROUP, CROSS_MAX_STRIDE, ROTARY_MAX_PAIRS = 32, 1 << 23, 4096
 EPI_BIAS, EPI_RESIDUAL, EPI_AFFINE, EPI_RELU = 1, 2, 4, 8
 CSR_VERBATIM, CSR_ONE_SELF_LOOP, CSR_TRANSPOSE = 0, 1, 4
 

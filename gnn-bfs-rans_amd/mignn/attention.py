@@ -203,6 +203,9 @@ class RotaryAxes:
         self.pairs = tuple(int(m) for m in pairs)
         if not self.pairs or any(m < 0 for m in self.pairs) or sum(self.pairs) == 0:
             raise ValueError(f"RotaryAxes: pairs must be counts with a positive sum, got {pairs}")
+        if sum(self.pairs) > _lib.ROTARY_MAX_PAIRS:
+            raise ValueError(f"RotaryAxes: {sum(self.pairs)} pairs (at most "
+                             f"{_lib.ROTARY_MAX_PAIRS})")
         if not (base > 0.0 and math.isfinite(base)):
             raise ValueError(f"RotaryAxes: base must be positive and finite, got {base}")
         self.scales = tuple(float(s) for s in scales) if scales is not None \

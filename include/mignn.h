@@ -754,7 +754,8 @@ int mignn_rms_norm_backward(const void* x, int64_t ldx, const void* residual, in
  * `inverse`.  Pairs are columns (j, j + pairs), or (2j, 2j + 1) when
  * `interleaved`; columns from 2 pairs on are copied.  ldt / ldh, ldyt / ldyh:
  * strides of rows and heads in elements, columns contiguous; y must not
- * overlap x.  Every axis[j] indexes a column of pos. */
+ * overlap x.  Every axis[j] indexes a column of pos.  pairs <= MIGNN_ROTARY_MAX_PAIRS. */
+#define MIGNN_ROTARY_MAX_PAIRS 4096
 int mignn_rotary(const void* x, int64_t ldt, int64_t ldh, int64_t n, int heads, int d,
                  const void* pos, int pos_type, int64_t ldp, const double* freq,
                  const int32_t* axis, int pairs, int interleaved, int inverse, int dtype, void* y,

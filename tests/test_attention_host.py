@@ -47,7 +47,7 @@ def test_rotary_refusals():
             ((x, pos, ax), RuntimeError, "ROCm devices only")]:
         with pytest.raises(exc, match=msg):
             A.rotary(*args)
-    for pairs, kw in [((), {}), ((0, 0), {}), ((2, -1), {}), ((2,), {"base": 0.0}),
+    for pairs, kw in [((), {}), ((0, 0), {}), ((4097,), {}), ((2, -1), {}), ((2,), {"base": 0.0}),
                       ((2,), {"base": float("inf")}), ((2, 2), {"scales": (1.0,)}),
                       ((2,), {"scales": (float("nan"),)})]:
         with pytest.raises(ValueError):

@@ -162,7 +162,7 @@ def test_rms_norm_nan_stays_in_its_row():
 @pytest.mark.parametrize("n,heads,d,pairs", [
     (1, 4, 32, (6, 5, 5)), (37, 3, 20, (4, 4)), (130, 1, 6, (1, 1, 1)), (1000, 8, 64, (16, 16)),
     (77, 2, 40, (7, 0, 6)), (5, 2, 2, (1,)), (0, 2, 8, (4,)), (19, 5, 128, (22, 21, 21)),
-    (64, 1, 66, (11, 11, 10, 1))])
+    (64, 1, 66, (11, 11, 10, 1)), (3, 2, 8200, (4096,)), (700, 1, 4, (1, 1)), (2, 300, 16, (8,))])
 def test_rotary_and_gradient(n, heads, d, pairs, dt, interleaved):
     x = rnd(n, heads, d, seed=1, dt=dt).requires_grad_()
     pos = torch.rand(n, len(pairs), generator=torch.Generator().manual_seed(2)).to(DEV)
