@@ -1,0 +1,316 @@
+// The row operators (mignn.attention) as PyTorch calls with gradients: this
+// module (mignn/_ops.so) owns memory and the autograd graph, the arithmetic is
+// libmignn's C ABI.  In C++ because a call of a probe's size is a few
+// microseconds of work: a Python autograd function costs 60 us more a training
+// step, most of it in the engine's thread.  The arguments' checks are Python's
+// (mignn/attention.py); nothing here is called with unchecked shapes or types.
+#include <torch/extension.h>
+
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <cstring>
+#include <stdexcept>
+#include <string>
+
+#include "../../include/mignn.h"
+
+namespace {
+
+using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = c10::optional<Tensor>;
+
+// The library's entry points, by the addresses that the loader resolved (the
+// library is the one that mignn._lib loaded)
+struct Library {
+    decltype(&mignn_last_error) last_error;
+    decltype(&mignn_rms_norm) rms_norm;
+    decltype(&mignn_rms_norm_backward_scratch_bytes) rms_norm_backward_scratch_bytes;
+    decltype(&mignn_rms_norm_backward) rms_norm_backward;
+    decltype(&mignn_rotary) rotary;
+    decltype(&mignn_cross_attn_forward) cross_attn_forward;
+    decltype(&mignn_cross_attn_backward) cross_attn_backward;
+} lib;
+
+void bind(const std::vector<uint64_t>& at) {
+    if (at.size() * sizeof(uint64_t) != sizeof(lib)) throw std::invalid_argument("mignn: entry points");
+    std::memcpy(&lib, at.data(), sizeof(lib));
+}
+
+void check(int rc, const char* what) {
+    if (rc == 0) return;
+    throw std::runtime_error(std::string(what) + " failed (status " + std::to_string(rc) +
+                             "): " + lib.last_error());
+}
+
+void* stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* out(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+bool is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
+int row_type(const Tensor& t) {
+    return is_f32(t) ? MIGNN_ROW_F32 : t.scalar_type() == at::kBFloat16 ? MIGNN_ROW_BF16 : MIGNN_ROW_F16;
+}
+Tensor copied(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
+Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+bool needs_grad(std::initializer_list<const Tensor*> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : ts)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+// Gradients that autograd cannot differentiate again: under create_graph they
+// refuse it when asked.
+variable_list first_order(variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list real;
+    for (Tensor& g : grads)
+        if (g.defined()) real.push_back(g.detach().requires_grad_(true));
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        "mignn row operators: gradients are first order only", static_cast<int>(real.size()));
+    variable_list wrapped = (*error)(std::move(real));
+    size_t k = 0;
+    for (Tensor& g : grads)
+        if (g.defined()) g = wrapped[k++];
+    return grads;
+}
+
+// Rows with contiguous columns that do not overlap (a copy if need be)
+Tensor matrix(const Tensor& t) {
+    if (!t.defined() || ((t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1))))
+        return t;
+    return copied(t);
+}
+int64_t row_stride(const Tensor& t) { return t.defined() ? t.stride(0) : 0; }
+
+// ---------------------------------------------------------------------------
+// Root-mean-square norm
+
+std::pair<Tensor, Tensor> norm_forward(const Tensor& x_, const Tensor& w_, const Tensor& r_, double eps) {
+    c10::DeviceGuard guard(x_.device());
+    const Tensor x = matrix(x_), r = matrix(r_), w = w_.contiguous();
+    const int64_t n = x.size(0), h = x.size(1);
+    Tensor y = at::empty({n, h}, x.options());
+    Tensor s = r.defined() ? at::empty({n, h}, x.options()) : Tensor();
+    check(lib.rms_norm(ptr(x), row_stride(x), ptr(r), row_stride(r), ptr(w), is_f32(w), n, static_cast<int>(h),
+                       static_cast<float>(eps), row_type(x), out(y), h, out(s), h, stream(x)),
+          "mignn_rms_norm");
+    return {y, s};
+}
+
+struct RMSNorm : torch::autograd::Function<RMSNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& r,
+                                 double eps) {
+        auto [y, s] = norm_forward(x, w, value(r), eps);
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["residual"] = s.defined();
+        // fp32 rows: the stored s is the s that was normed; 16-bit rows: it is
+        // rounded, so the gradient adds x and the residual again
+        if (s.defined() && is_f32(x)) ctx->save_for_backward({s, w, Tensor()});
+        else ctx->save_for_backward({x, w, value(r)});
+        if (s.defined()) return {y, s};
+        return {y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const bool residual = ctx->saved_data["residual"].toBool();
+        const bool want_w = ctx->needs_input_grad(1);
+        const Tensor x = matrix(saved[0]), w = saved[1].contiguous(), r = matrix(saved[2]);
+        const Tensor dy = matrix(grads[0]), ds = residual ? matrix(grads[1]) : Tensor();
+        c10::DeviceGuard guard(x.device());
+        Tensor dx, dw;
+        if (!dy.defined()) {
+            dx = ds;
+            if (want_w) dw = at::zeros_like(w);
+        } else {
+            const int64_t n = x.size(0), h = x.size(1);
+            dx = at::empty({n, h}, x.options());
+            Tensor scratch;
+            size_t bytes = 0;
+            if (want_w) {
+                dw = at::empty(w.sizes(), w.options());
+                bytes = lib.rms_norm_backward_scratch_bytes(n, static_cast<int>(h), row_type(x));
+                scratch = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+            }
+            check(lib.rms_norm_backward(ptr(x), row_stride(x), ptr(r), row_stride(r), ptr(w), is_f32(w), n,
+                                        static_cast<int>(h), static_cast<float>(ctx->saved_data["eps"].toDouble()),
+                                        row_type(x), ptr(dy), row_stride(dy), ptr(ds), row_stride(ds), out(dx), h,
+                                        out(dw), out(scratch), bytes, stream(x)),
+                  "mignn_rms_norm_backward");
+        }
+        return first_order({dx, dw, residual ? dx : Tensor(), Tensor()});
+    }
+};
+
+py::object rms_norm(const Tensor& x, const Tensor& w, const OptTensor& r, double eps) {
+    if (needs_grad({&x, &w}) || (r.has_value() && needs_grad({&*r}))) {
+        variable_list o = RMSNorm::apply(x, w, r, eps);
+        if (o.size() == 1) return py::cast(o[0]);
+        return py::make_tuple(o[0], o[1]);
+    }
+    auto [y, s] = norm_forward(x, w, value(r), eps);
+    if (!s.defined()) return py::cast(y);
+    return py::make_tuple(y, s);
+}
+
+// ---------------------------------------------------------------------------
+// Rotary positions
+
+// [rows, heads, d] with contiguous columns; align: bytes that the pointer and
+// the strides are multiples of, the strides then also within the kernels'
+// 32-bit offsets (a copy if need be)
+Tensor heads_of(const Tensor& t, int64_t align = 1) {
+    if (t.size(2) > 1 && t.stride(2) != 1) return copied(t);
+    if (align > 1) {
+        const int64_t es = t.element_size(), a = t.stride(0), b = t.stride(1);
+        if ((reinterpret_cast<int64_t>(t.const_data_ptr()) | a * es | b * es) % align ||
+            std::max(a, b) > MIGNN_CROSS_MAX_STRIDE)
+            return copied(t);
+    }
+    return t;
+}
+
+Tensor turn(const Tensor& x_, const Tensor& pos_, const Tensor& freq, const Tensor& axis, bool interleaved,
+            bool inverse) {
+    c10::DeviceGuard guard(x_.device());
+    const Tensor x = heads_of(x_);
+    const Tensor pos = pos_.size(1) > 1 && pos_.stride(1) != 1 ? pos_.contiguous() : pos_;
+    const int pos_type = is_f32(pos) ? MIGNN_POS_F32 : pos.scalar_type() == at::kDouble ? MIGNN_POS_F64
+                         : pos.scalar_type() == at::kInt ? MIGNN_POS_I32 : MIGNN_POS_I64;
+    const int64_t n = x.size(0), heads = x.size(1), d = x.size(2);
+    Tensor y = at::empty({n, heads, d}, x.options());
+    check(lib.rotary(ptr(x), x.stride(0), x.stride(1), n, static_cast<int>(heads), static_cast<int>(d), ptr(pos),
+                     pos_type, pos.stride(0), static_cast<const double*>(ptr(freq)),
+                     static_cast<const int32_t*>(ptr(axis)), static_cast<int>(freq.numel()), interleaved, inverse,
+                     row_type(x), out(y), heads * d, d, stream(x)),
+          "mignn_rotary");
+    return y;
+}
+
+struct Rotary : torch::autograd::Function<Rotary> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& pos, const Tensor& freq,
+                          const Tensor& axis, bool interleaved) {
+        ctx->save_for_backward({pos, freq, axis});
+        ctx->saved_data["interleaved"] = interleaved;
+        return turn(x, pos, freq, axis, interleaved, false);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        return first_order({turn(grads[0], saved[0], saved[1], saved[2],
+                                 ctx->saved_data["interleaved"].toBool(), true),
+                            Tensor(), Tensor(), Tensor(), Tensor()});
+    }
+};
+
+Tensor rotary(const Tensor& x, const Tensor& pos, const Tensor& freq, const Tensor& axis, bool interleaved) {
+    if (needs_grad({&x})) return Rotary::apply(x, pos, freq, axis, interleaved);
+    return turn(x, pos, freq, axis, interleaved, false);
+}
+
+// ---------------------------------------------------------------------------
+// Cross attention
+
+// a plan's call, with the tensors of one use filled in
+mignn_cross_call call_of(const mignn_cross_call& plan, const Tensor& q, const Tensor& k, const Tensor& v,
+                         const Tensor& mask, double scale, const Tensor& scratch) {
+    mignn_cross_call c = plan;
+    c.q = ptr(q), c.k = ptr(k), c.v = ptr(v);
+    c.key_mask = static_cast<const uint8_t*>(ptr(mask));
+    c.ldq = q.stride(0), c.ldqh = q.stride(1);
+    c.ldk = k.stride(0), c.ldkh = k.stride(1);
+    c.ldv = v.stride(0), c.ldvh = v.stride(1);
+    c.scale = static_cast<float>(scale);
+    c.scratch = out(scratch);
+    c.scratch_bytes = scratch.defined() ? scratch.numel() : 0;
+    return c;
+}
+
+Tensor scratch_for(int64_t bytes, const Tensor& t) {
+    return bytes > 0 ? at::empty({bytes}, t.options().dtype(at::kByte)) : Tensor();
+}
+
+struct CrossOut {
+    Tensor out, out32, lse;
+};
+
+CrossOut cross_forward(const mignn_cross_call& plan, const Tensor& q_, const Tensor& k_, const Tensor& v_,
+                       const Tensor& mask, double scale, bool train) {
+    c10::DeviceGuard guard(q_.device());
+    const Tensor q = heads_of(q_, 16), k = heads_of(k_, 16), v = heads_of(v_, 16);
+    CrossOut o;
+    o.out = at::empty(q.sizes(), q.options());
+    if (train) {
+        o.lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+        if (!is_f32(q)) o.out32 = at::empty(q.sizes(), q.options().dtype(at::kFloat));
+    }
+    const Tensor scratch = scratch_for(plan.pass[MIGNN_CROSS_FORWARD].part_bytes, q);
+    const mignn_cross_call c = call_of(plan, q, k, v, mask, scale, scratch);
+    check(lib.cross_attn_forward(&c, out(o.out), static_cast<float*>(out(o.out32)),
+                                 static_cast<float*>(out(o.lse)), stream(q)),
+          "mignn_cross_attn_forward");
+    if (!o.out32.defined()) o.out32 = o.out;
+    return o;
+}
+
+struct CrossAttention : torch::autograd::Function<CrossAttention> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                          const OptTensor& mask, const Tensor& lists, const std::string& plan, double scale) {
+        mignn_cross_call c;
+        std::memcpy(&c, plan.data(), sizeof(c));
+        const CrossOut o = cross_forward(c, q, k, v, value(mask), scale, true);
+        // out32 (the fp32 output): <do, o> from the rounded output would leave
+        // the rounding of o in every dS.  lists: the plan's, kept alive
+        ctx->save_for_backward({q, k, v, value(mask), o.out32, o.lse, lists});
+        ctx->saved_data["plan"] = plan;
+        ctx->saved_data["scale"] = scale;
+        return o.out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        mignn_cross_call plan;
+        std::memcpy(&plan, ctx->saved_data["plan"].toStringRef().data(), sizeof(plan));
+        const Tensor q = heads_of(saved[0], 16), k = heads_of(saved[1], 16), v = heads_of(saved[2], 16);
+        const Tensor dout = heads_of(grads[0], 16), &mask = saved[3], &out32 = saved[4], &lse = saved[5];
+        c10::DeviceGuard guard(q.device());
+        Tensor dq = at::empty(q.sizes(), q.options()), dk, dv;
+        const bool keys = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+        if (keys) {
+            dk = at::empty(k.sizes(), k.options());
+            dv = at::empty(v.sizes(), v.options());
+        }
+        const Tensor delta = at::empty(lse.sizes(), lse.options());
+        const Tensor scratch = scratch_for(std::max(plan.pass[MIGNN_CROSS_DQ].part_bytes,
+                                                    plan.pass[MIGNN_CROSS_DKV].part_bytes), q);
+        const mignn_cross_call c = call_of(plan, q, k, v, mask, ctx->saved_data["scale"].toDouble(), scratch);
+        check(lib.cross_attn_backward(&c, ptr(dout), dout.stride(0), dout.stride(1),
+                                      static_cast<const float*>(ptr(out32)), static_cast<const float*>(ptr(lse)),
+                                      static_cast<float*>(out(delta)), out(dq), out(dk), out(dv), stream(q)),
+              "mignn_cross_attn_backward");
+        if (!ctx->needs_input_grad(0)) dq = Tensor();
+        if (!ctx->needs_input_grad(1)) dk = Tensor();
+        if (!ctx->needs_input_grad(2)) dv = Tensor();
+        return first_order({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()});
+    }
+};
+
+Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask,
+                       const Tensor& lists, uint64_t plan, double scale) {
+    const auto& c = *reinterpret_cast<const mignn_cross_call*>(plan);
+    if (needs_grad({&q, &k, &v}))
+        return CrossAttention::apply(q, k, v, mask, lists,
+                                     std::string(reinterpret_cast<const char*>(&c), sizeof(c)), scale);
+    return cross_forward(c, q, k, v, value(mask), scale, false).out;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.doc() = "row operators over libmignn (mignn.attention)";
+    m.def("bind", &bind);
+    m.def("rms_norm", &rms_norm);
+    m.def("rotary", &rotary);
+    m.def("cross_attention", &cross_attention);
+}

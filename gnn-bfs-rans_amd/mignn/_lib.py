@@ -292,6 +292,34 @@ def diag_lib():
     return _diag
 
 
+OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_ops.so")
+# the entry points that _ops.so calls, in the order of its table
+OPS_ENTRIES = ("mignn_last_error", "mignn_rms_norm", "mignn_rms_norm_backward_scratch_bytes",
+               "mignn_rms_norm_backward", "mignn_rotary", "mignn_cross_attn_forward",
+               "mignn_cross_attn_backward")
+_ops = None
+
+
+def ops():
+    """Load (once) and return the module of mignn.attention's operators
+    (_ops.so, csrc/torch_ops.cpp), bound to the loaded product library."""
+    global _ops
+    if _ops is None:
+        import importlib.machinery
+        import importlib.util
+        if not os.path.exists(OPS_PATH):
+            raise MignnError(
+                f"_ops.so not found at {OPS_PATH}: build it with "
+                "`python -c 'import __graft_entry__ as g; g.build()'`. There is no fallback.")
+        loader = importlib.machinery.ExtensionFileLoader("_ops", OPS_PATH)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_ops", loader))
+        loader.exec_module(mod)
+        h = lib()
+        mod.bind([ctypes.cast(getattr(h, n), c_void_p).value for n in OPS_ENTRIES])
+        _ops = mod
+    return _ops
+
+
 def ptr(t) -> int | None:
     """Device pointer of a tensor (None for None)."""
     if t is None:

@@ -8,8 +8,8 @@ over another graph of another size.
 
 Rows are fp32, bf16 or fp16; sums, softmax statistics and norms are fp32 and
 each output is rounded once.  All three run and differentiate in HIP kernels
-of libmignn.so on the tensors' device and its current stream; there is no CPU
-path.  Outputs and scratch come from PyTorch's allocator at every call, so
+of libmignn.so (through _ops.so, csrc/torch_ops.cpp) on the tensors' device and
+its current stream; there is no CPU path.  Outputs and scratch come from PyTorch's allocator at every call, so
 calls on several streams, or captured into several graphs, share nothing but
 the read-only `RotaryAxes` / `CrossPlan`.  Gradients are first order only.
 
@@ -25,24 +25,17 @@ from typing import Optional, Sequence, Tuple
 import numpy as np
 import torch
 import torch.nn as nn
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import train_ops as T
 
-P = _lib.ptr
-
 _ROW = {torch.float32: _lib.ROW_F32, torch.bfloat16: _lib.ROW_BF16, torch.float16: _lib.ROW_F16}
-_POS = {torch.float32: _lib.POS_F32, torch.float64: _lib.POS_F64, torch.int32: _lib.POS_I32,
-        torch.int64: _lib.POS_I64}
+_POS = (torch.float32, torch.float64, torch.int32, torch.int64)
 
 
-def _row_type(what: str, t: torch.Tensor) -> int:
-    code = _ROW.get(t.dtype)
-    if code is None:
+def _row_type(what: str, t: torch.Tensor):
+    if t.dtype not in _ROW:
         raise TypeError(f"{what}: rows must be float32, bfloat16 or float16, got {t.dtype}")
-    return code
 
 
 def _on_device(what: str, ref: torch.Tensor, **others):
@@ -54,105 +47,8 @@ def _on_device(what: str, ref: torch.Tensor, **others):
             raise RuntimeError(f"mignn {what}: {name} is on {t.device}, not on {ref.device}")
 
 
-_get_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _launch(fn, what: str, index: int, *args):
-    """fn(*args, stream) with device `index` current and its current stream."""
-    prev = _get_device()
-    if prev != index:
-        torch.cuda.set_device(index)
-    try:
-        rc = fn(*args, _raw_stream(index))
-    finally:
-        if prev != index:
-            torch.cuda.set_device(prev)
-    if rc:
-        _lib.check(rc, what)
-
-
-def _first_order(backward):
-    """A backward whose kernels autograd cannot see: under create_graph its
-    gradients refuse to be differentiated again (the wrapper costs a few
-    microseconds, so it is taken only then)."""
-    guarded = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return staticmethod(run)
-
-
-def _grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
-
-
 # ---------------------------------------------------------------------------
 # Root-mean-square norm
-
-def _matrix(t: torch.Tensor) -> torch.Tensor:
-    """Rows with contiguous columns that do not overlap (a copy if need be)."""
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        return t.contiguous()
-    return t
-
-
-def _norm_forward(x, weight, residual, eps: float, code: int):
-    x = _matrix(x)
-    residual = None if residual is None else _matrix(residual)
-    weight = weight.contiguous()
-    n, h = x.shape
-    y = torch.empty((n, h), dtype=x.dtype, device=x.device)
-    s = None if residual is None else torch.empty_like(y)
-    _launch(_lib.lib().mignn_rms_norm, "mignn_rms_norm", x.device.index,
-            x.data_ptr(), x.stride(0), P(residual),
-            0 if residual is None else residual.stride(0), weight.data_ptr(),
-            weight.dtype == torch.float32, n, h, eps, code, y.data_ptr(), h, P(s), h)
-    return y, s
-
-
-class _RMSNorm(Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps: float, code: int):
-        y, s = _norm_forward(x, weight, residual, eps, code)
-        ctx.eps, ctx.code, ctx.residual = eps, code, residual is not None
-        ctx.set_materialize_grads(False)
-        # fp32 rows: the stored s is the s that was normed; 16-bit rows: it is
-        # rounded, so the gradient adds x and the residual again
-        if s is not None and x.dtype == torch.float32:
-            ctx.save_for_backward(s, weight, None)
-        else:
-            ctx.save_for_backward(x, weight, residual)
-        return y if s is None else (y, s)
-
-    @_first_order
-    def backward(ctx, dy, ds=None):
-        x, weight, residual = ctx.saved_tensors
-        if dy is None:
-            dx = ds
-            dw = torch.zeros_like(weight) if ctx.needs_input_grad[1] else None
-            return dx, dw, dx if ctx.residual else None, None, None
-        x, dy = _matrix(x), _matrix(dy)
-        residual = None if residual is None else _matrix(residual)
-        ds = None if ds is None else _matrix(ds)
-        weight = weight.contiguous()
-        n, h = x.shape
-        dx = torch.empty((n, h), dtype=x.dtype, device=x.device)
-        dw = scratch = None
-        nbytes = 0
-        L = _lib.lib()
-        if ctx.needs_input_grad[1]:
-            dw = torch.empty_like(weight)
-            nbytes = L.mignn_rms_norm_backward_scratch_bytes(n, h, ctx.code)
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _launch(L.mignn_rms_norm_backward, "mignn_rms_norm_backward", x.device.index,
-                x.data_ptr(), x.stride(0), P(residual),
-                0 if residual is None else residual.stride(0), weight.data_ptr(),
-                weight.dtype == torch.float32, n, h, ctx.eps, ctx.code, dy.data_ptr(),
-                dy.stride(0), P(ds), 0 if ds is None else ds.stride(0), dx.data_ptr(), h, P(dw),
-                P(scratch), nbytes)
-        return dx, dw, dx if ctx.residual else None, None, None
-
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
              eps: float = 1e-6):
@@ -164,7 +60,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     or x's type.  H <= 2048."""
     if x.dim() != 2:
         raise ValueError(f"rms_norm: x must be [N, H], got {tuple(x.shape)}")
-    code = _row_type("rms_norm", x)
+    _row_type("rms_norm", x)
     h = x.shape[1]
     if not 1 <= h <= _lib.RMS_NORM_MAX_H:
         raise ValueError(f"rms_norm: width {h} is not in 1..{_lib.RMS_NORM_MAX_H}")
@@ -178,10 +74,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     if not eps >= 0.0:
         raise ValueError(f"rms_norm: eps must not be negative, got {eps}")
     _on_device("rms_norm", x, weight=weight, residual=residual)
-    if _grad(x, weight, residual):
-        return _RMSNorm.apply(x, weight, residual, float(eps), code)
-    y, s = _norm_forward(x, weight, residual, float(eps), code)
-    return y if s is None else (y, s)
+    return _lib.ops().rms_norm(x, weight, residual, eps)
 
 
 # ---------------------------------------------------------------------------
@@ -222,53 +115,13 @@ class RotaryAxes:
         self.device = self.freq.device
 
 
-def _heads(t: torch.Tensor, align: int = 1) -> torch.Tensor:
-    """[rows, heads, d] with contiguous columns; align: bytes that the pointer
-    and the strides are multiples of, the strides then also within the kernels'
-    32-bit offsets (a copy if need be)."""
-    st, sh, sd = t.stride()
-    if sd != 1 and t.shape[2] > 1:
-        return t.clone(memory_format=torch.contiguous_format)
-    if align > 1:
-        es = t.element_size()
-        if (t.data_ptr() | st * es | sh * es) % align or max(st, sh) > _lib.CROSS_MAX_STRIDE:
-            return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _turn(x, pos, axes: RotaryAxes, code: int, inverse: bool):
-    x = _heads(x)
-    n, heads, d = x.shape
-    if pos.shape[1] > 1 and pos.stride(1) != 1:
-        pos = pos.contiguous()
-    y = torch.empty((n, heads, d), dtype=x.dtype, device=x.device)
-    _launch(_lib.lib().mignn_rotary, "mignn_rotary", x.device.index,
-            x.data_ptr(), x.stride(0), x.stride(1), n, heads, d, pos.data_ptr(), _POS[pos.dtype],
-            pos.stride(0), axes.freq.data_ptr(), axes.axis.data_ptr(), axes.total,
-            axes.interleaved, inverse, code, y.data_ptr(), heads * d, d)
-    return y
-
-
-class _Rotary(Function):
-    @staticmethod
-    def forward(ctx, x, pos, axes, code: int):
-        ctx.axes, ctx.code = axes, code
-        ctx.save_for_backward(pos)
-        return _turn(x, pos, axes, code, False)
-
-    @_first_order
-    def backward(ctx, dy):
-        (pos,) = ctx.saved_tensors
-        return _turn(dy, pos, ctx.axes, ctx.code, True), None, None, None
-
-
 def rotary(x: torch.Tensor, pos: torch.Tensor, axes: RotaryAxes) -> torch.Tensor:
     """x [N, heads, d] with the pairs of every head turned by the row's
     position pos [N, len(axes.pairs)] (float32 / float64 coordinates or int32 /
     int64 indices; angles are formed in float64).  Positions get no gradient."""
     if x.dim() != 3:
         raise ValueError(f"rotary: x must be [N, heads, d], got {tuple(x.shape)}")
-    code = _row_type("rotary", x)
+    _row_type("rotary", x)
     if pos.dim() != 2 or pos.shape[0] != x.shape[0] or pos.shape[1] != len(axes.pairs):
         raise ValueError(f"rotary: pos must be [{x.shape[0]}, {len(axes.pairs)}], got "
                          f"{tuple(pos.shape)}")
@@ -280,9 +133,7 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, axes: RotaryAxes) -> torch.Tensor
     if torch.is_grad_enabled() and pos.requires_grad:
         raise NotImplementedError("rotary: positions get no gradient (pass pos.detach())")
     _on_device("rotary", x, pos=pos, axes=axes.freq)
-    if _grad(x):
-        return _Rotary.apply(x, pos, axes, code)
-    return _turn(x, pos, axes, code, False)
+    return _lib.ops().rotary(x, pos, axes.freq, axes.axis, axes.interleaved)
 
 
 # ---------------------------------------------------------------------------
@@ -312,7 +163,7 @@ class CrossPlan:
     captured graphs.  train=False leaves the backward's lists out."""
 
     __slots__ = ("q_lens", "k_lens", "queries", "keys", "heads", "kv_heads", "head_dim", "dtype",
-                 "device", "train", "_call", "_lists", "_scratch")
+                 "device", "train", "_call", "_lists", "_address")
 
     def __init__(self, q_lens, k_lens, *, heads: int, kv_heads: Optional[int] = None,
                  head_dim: int, dtype: torch.dtype = torch.float32, device="cuda",
@@ -365,72 +216,7 @@ class CrossPlan:
             ps.n_items, ps.n_joins, ps.n_whole = n_items, n_joins, whole
             ps.tile, ps.rows = tile, rows
         self._call = call
-        parts = [s[2] for s in spans]
-        self._scratch = (parts[0], max(parts[1:]) if train else 0)
-
-
-def _cross_call(q, k, v, plan: CrossPlan, mask, scale: float, scratch):
-    c = _lib.CrossCall.from_buffer_copy(plan._call)
-    c.q, c.k, c.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    c.key_mask = None if mask is None else mask.data_ptr()
-    c.ldq, c.ldqh = q.stride(0), q.stride(1)
-    c.ldk, c.ldkh = k.stride(0), k.stride(1)
-    c.ldv, c.ldvh = v.stride(0), v.stride(1)
-    c.scale = scale
-    if scratch is not None:
-        c.scratch, c.scratch_bytes = scratch.data_ptr(), scratch.numel()
-    return c
-
-
-def _scratch(nbytes: int, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _cross_forward(q, k, v, plan: CrossPlan, mask, scale: float, train: bool):
-    q, k, v = _heads(q, 16), _heads(k, 16), _heads(v, 16)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    out32 = lse = None
-    if train:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        if q.dtype != torch.float32:
-            out32 = torch.empty(q.shape, dtype=torch.float32, device=q.device)
-    scratch = _scratch(plan._scratch[0], q.device)
-    c = _cross_call(q, k, v, plan, mask, scale, scratch)
-    _launch(_lib.lib().mignn_cross_attn_forward, "mignn_cross_attn_forward", q.device.index,
-            ctypes.addressof(c), out.data_ptr(), P(out32), P(lse))
-    return out, (out if out32 is None else out32), lse
-
-
-class _CrossAttention(Function):
-    @staticmethod
-    def forward(ctx, q, k, v, plan: CrossPlan, mask, scale: float):
-        out, out32, lse = _cross_forward(q, k, v, plan, mask, scale, True)
-        ctx.plan, ctx.scale = plan, scale
-        # out32 (the fp32 output): <do, o> from the rounded output would leave
-        # the rounding of o in every dS
-        ctx.save_for_backward(q, k, v, mask, out32, lse)
-        return out
-
-    @_first_order
-    def backward(ctx, dout):
-        q, k, v, mask, out32, lse = ctx.saved_tensors
-        plan = ctx.plan
-        q, k, v, dout = _heads(q, 16), _heads(k, 16), _heads(v, 16), _heads(dout, 16)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = dv = None
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        delta = torch.empty_like(lse)
-        scratch = _scratch(plan._scratch[1], q.device)
-        c = _cross_call(q, k, v, plan, mask, ctx.scale, scratch)
-        _launch(_lib.lib().mignn_cross_attn_backward, "mignn_cross_attn_backward",
-                q.device.index, ctypes.addressof(c), dout.data_ptr(), dout.stride(0),
-                dout.stride(1), out32.data_ptr(), lse.data_ptr(), delta.data_ptr(),
-                dq.data_ptr(), P(dk), P(dv))
-        need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None,
-                None, None)
+        self._address = ctypes.addressof(call)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: CrossPlan,
@@ -460,11 +246,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Cro
     _on_device("cross_attention", q, k=k, v=v, key_mask=key_mask, plan=plan._lists)
     if key_mask is not None:
         key_mask = key_mask.contiguous()
-    if _grad(q, k, v):
-        if not plan.train:
-            raise ValueError("cross_attention: gradients need a plan built with train=True")
-        return _CrossAttention.apply(q, k, v, plan, key_mask, scale)
-    return _cross_forward(q, k, v, plan, key_mask, scale, False)[0]
+    if not plan.train and torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
+                                                       or v.requires_grad):
+        raise ValueError("cross_attention: gradients need a plan built with train=True")
+    return _lib.ops().cross_attention(q, k, v, key_mask, plan._lists, plan._address, scale)
 
 
 # ---------------------------------------------------------------------------

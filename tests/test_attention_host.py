@@ -270,3 +270,13 @@ def test_graph_lengths():
     for bad in (torch.tensor([1, 0]), torch.tensor([0])):
         with pytest.raises(ValueError, match="sorted"):
             A.graph_lengths(bad, 2)
+
+
+def test_ops_module_is_bound_to_the_product_library():
+    """_ops.so loads, its table has the entry points that it calls, and a wrong
+    table is an error, not a jump."""
+    ops = _lib.ops()
+    assert ops is _lib.ops()
+    assert all(n in _lib.SIGNATURES for n in _lib.OPS_ENTRIES)
+    with pytest.raises(ValueError, match="entry points"):
+        ops.bind([0])
