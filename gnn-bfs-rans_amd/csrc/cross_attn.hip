@@ -66,52 +66,60 @@ __global__ __launch_bounds__(256) void cross_join_fwd_kernel(CrossArgs a) {
     if (a.lse && c == 0) a.lse[at] = l == 0.f ? INFINITY : base + log2f(l);
 }
 
-// Many parts of few rows: one row a workgroup, its waves take every fourth part.
+// Many parts of few rows: a row a workgroup, 4 columns of a part a thread, so
+// that most parts are in flight at once.
 template <typename T>
 __global__ __launch_bounds__(256) void cross_join_few_kernel(CrossArgs a) {
-    __shared__ float os[4][128];
+    __shared__ float ms[4], ls[4], os[4][128];
     const CrossJoin jn = a.joins[blockIdx.x];
     const int kvh = blockIdx.y, r = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (r >= jn.r1 - jn.r0) return;
+    const int d4 = a.d / 4;
+    int lp = 2;   // lanes of a part
+    while (lp < d4) lp <<= 1;
+    const int groups = 256 / lp, g = threadIdx.x / lp, c = (threadIdx.x & (lp - 1)) * 4;
     const int64_t step = static_cast<int64_t>(a.kv_heads) * a.tile * (a.d + 2);
     const float* src = part_row(a, jn.slot, kvh, r, a.tile, a.d + 2);
     float m = -INFINITY;
-    for (int p = lane; p < jn.parts; p += 64) m = fmaxf(m, src[p * step + a.d]);
-    for (int b = 1; b < 64; b <<= 1) m = fmaxf(m, __shfl_xor(m, b));
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[2] = {0.f, 0.f};
-    const bool two = lane + 64 < a.d, one = lane < a.d;
-    for (int p0 = 0; p0 < jn.parts; p0 += 64) {
-        float f = 0.f;
-        if (p0 + lane < jn.parts) {
-            f = __builtin_amdgcn_exp2f(src[(p0 + lane) * step + a.d] - base);
-            l = fmaf(src[(p0 + lane) * step + a.d + 1], f, l);
-        }
-        const int n = jn.parts - p0 < 64 ? jn.parts - p0 : 64;
-        for (int p = wave; p < n; p += 4) {
-            const float fp = __shfl(f, p);
-            const float* row = src + (p0 + p) * step + lane;
-            if (one) o[0] = fmaf(row[0], fp, o[0]);
-            if (two) o[1] = fmaf(row[64], fp, o[1]);
-        }
-    }
-    for (int b = 1; b < 64; b <<= 1) l += __shfl_xor(l, b);
-    os[wave][lane] = o[0], os[wave][lane + 64] = o[1];
+#pragma unroll 4
+    for (int p = g; p < jn.parts; p += groups) m = fmaxf(m, src[p * step + a.d]);
+    for (int b = lp; b < 64; b <<= 1) m = fmaxf(m, __shfl_xor(m, b));
+    if (lane == 0) ms[wave] = m;
     __syncthreads();
-    if (wave) return;
+    m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = g; p < jn.parts; p += groups) {
+        const float* part = src + p * step;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (c < a.d) load_row(part + c, x);
+        const float f = __builtin_amdgcn_exp2f(part[a.d] - base);
+        l = fmaf(part[a.d + 1], f, l);
 #pragma unroll
-    for (int w = 1; w < 4; ++w) o[0] += os[w][lane], o[1] += os[w][lane + 64];
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+    }
+    for (int b = lp; b < 64; b <<= 1) {
+        l += __shfl_xor(l, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], b);
+    }
+    if (lane < lp) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) os[wave][c + e] = o[e];
+        if (lane == 0) ls[wave] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x >= lp || c >= a.d) return;
+    l = ls[0] + ls[1] + ls[2] + ls[3];
     const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (os[0][c + e] + os[1][c + e] + os[2][c + e] + os[3][c + e]) * inv;
     const int row = jn.r0 + r, t = row / a.group;
     const int64_t at = (jn.begin + static_cast<int64_t>(t)) * a.heads + kvh * a.group + (row - t * a.group);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int c = lane + 64 * i;
-        if (c >= a.d) continue;
-        static_cast<T*>(a.out)[at * a.d + c] = static_cast<T>(o[i] * inv);
-        if (a.o32) a.o32[at * a.d + c] = o[i] * inv;
-    }
-    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : base + log2f(l);
+    store_row(static_cast<T*>(a.out) + at * a.d + c, o);
+    if (a.o32) store_row(a.o32 + at * a.d + c, o);
+    if (a.lse && c == 0) a.lse[at] = l == 0.f ? INFINITY : base + log2f(l);
 }
 
 // Sums the parts of split gradients in slot order, 4 columns of a row a thread:
