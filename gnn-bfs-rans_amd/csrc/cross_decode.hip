@@ -37,6 +37,22 @@ __device__ __forceinline__ float key_sum(float v) {
     return v;
 }
 
+// <a, b> of a lane's 16 bytes: bf16 two at a time, products and sum in fp32
+template <typename T, int V>
+__device__ __forceinline__ float dot(const RowVec<T, V>& a, const RowVec<T, V>& b) {
+    float x = 0.f;
+    if constexpr (__is_same(T, bf16_t)) {
+        typedef T pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < V; i += 2)
+            x = __builtin_amdgcn_fdot2_f32_bf16(pair{a.v[i], a.v[i + 1]}, pair{b.v[i], b.v[i + 1]}, x, false);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x = fmaf(static_cast<float>(a.v[i]), static_cast<float>(b.v[i]), x);
+    }
+    return x;
+}
+
 // One thread's share of UNROLL keys, in flight
 template <typename T, int UNROLL>
 struct KeyLoad {
@@ -56,18 +72,18 @@ __global__ __launch_bounds__(WAVES * 64) void cross_few_kernel(CrossArgs a) {
     const int c0 = sub * V;
     const bool in = c0 < a.d;
     const int rows = it.r1 - it.r0;
-    float q[R][V], o[R][V], m[R], l[R];
+    RowVec<T, V> q[R];
+    float o[R][V], m[R], l[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         m[r] = -INFINITY, l[r] = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) q[r][i] = o[r][i] = 0.f;
+        for (int i = 0; i < V; ++i) o[r][i] = 0.f;
+        q[r] = RowVec<T, V>{};
         if (r < rows && in) {
             const int row = it.r0 + r, t = row / a.group;
-            load_row(static_cast<const T*>(a.q) + (it.q_begin + static_cast<int64_t>(t)) * a.ldq +
-                         (kvh * a.group + row - t * a.group) * a.ldqh + c0, q[r]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) q[r][i] *= a.c;
+            __builtin_memcpy(&q[r], static_cast<const T*>(a.q) + (it.q_begin + static_cast<int64_t>(t)) * a.ldq +
+                                        (kvh * a.group + row - t * a.group) * a.ldqh + c0, 16);
         }
     }
     const T* kb = static_cast<const T*>(a.k) + kvh * a.ldkh + c0;
@@ -94,32 +110,20 @@ __global__ __launch_bounds__(WAVES * 64) void cross_few_kernel(CrossArgs a) {
         bool ok[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) ok[u] = now.ok[u] != 0u && k0 + u * KPW + grp < it.c1;
-        float kf[UNROLL][V], vf[UNROLL][V];
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                kf[u][i] = static_cast<float>(now.k[u].v[i]);
-                vf[u][i] = static_cast<float>(now.v[u].v[i]);
-            }
         float s[R][UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float x = 0.f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) x = fmaf(q[r][i], kf[u][i], x);
-                x = key_sum<LPK>(x);
-                s[r][u] = ok[u] ? x : -INFINITY;
+                const float x = key_sum<LPK>(dot(q[r], now.k[u]));
+                s[r][u] = ok[u] ? x * a.c : -INFINITY;
             }
         // what the mask leaves out may hold anything, and 0 inf is no 0
+        float vf[UNROLL][V];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
-            if (!ok[u]) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) vf[u][i] = 0.f;
-            }
+            for (int i = 0; i < V; ++i) vf[u][i] = ok[u] ? static_cast<float>(now.v[u].v[i]) : 0.f;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float mn = m[r];
