@@ -62,7 +62,7 @@ struct Stage {
     static constexpr int C8 = DP / 8, N = KT * C8 / NT;
     static_assert(KT * C8 % NT == 0, "tile share");
     f32x4 v[N];
-    int off[N];
+    int off[N], lds[N];
     uint32_t bytes;
     __device__ __forceinline__ static int row(int j) { return (threadIdx.x + j * NT) / C8; }
     __device__ __forceinline__ static int chunk(int j) { return (threadIdx.x + j * NT) % C8; }
@@ -73,6 +73,7 @@ struct Stage {
             const int t = row(j) / group, h = row(j) - t * group;
             off[j] = chunk(j) * 8 < d ? static_cast<int>((t * ldt + h * ldh + chunk(j) * 8) * sizeof(T))
                                       : NO_LOAD;
+            lds[j] = TileRow<DP>::at(row(j), chunk(j) * 8);
         }
         // (63 rows' and all heads' strides fit: checked by the host)
         bytes = uniform(static_cast<int>((KT / group * ldt + group * ldh + d) * sizeof(T)));
@@ -87,14 +88,14 @@ struct Stage {
     __device__ __forceinline__ void write(char* tile) const {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            *reinterpret_cast<f32x4*>(tile + row(j) * pitch<DP>() + chunk(j) * 16) = v[j];
+            *reinterpret_cast<f32x4*>(tile + lds[j]) = v[j];
     }
     // rows whose bit is clear as zeros
     __device__ __forceinline__ void write(char* tile, uint64_t keep) const {
         if (keep == ~0ull) return write(tile);
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            *reinterpret_cast<f32x4*>(tile + row(j) * pitch<DP>() + chunk(j) * 16) =
+            *reinterpret_cast<f32x4*>(tile + lds[j]) =
                 (keep >> row(j)) & 1u ? v[j] : f32x4{};
     }
 };
@@ -139,14 +140,14 @@ struct DsScale {
 };
 
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd16_kernel(CrossArgs a) {
-    constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
+__global__ __launch_bounds__(NW * 64, NW > 1 ? (DP <= 64 ? 3 : 2) : DP == 32 ? 2 : 1) void cross_fwd16_kernel(CrossArgs a) {
+    constexpr int TILE = KT * TileRow<DP>::BYTES, NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];   // K, V; twice
     int item, kvh;
     if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int trl = tr_lane<DP>(lane);
+    const TileLane<DP> tl(lane);
     constexpr f32x16 zero = {};
     vec8<T> qf[DP / 16];
     const int row = it.r0 + wave * 32 + col;
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd
         for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                const vec8<T> f = row_frag<T, DP>(kt, 32 * hb, i, col, half);
+                const vec8<T> f = row_frag<T, DP>(kt, tl, 32 * hb, i);
                 s[hb] = mfma16(f, qf[i], i == 0 ? zero : s[hb]);
             }
         if (bits != ~0ull) {
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd
             const vec8<T> rest = NW == 1 ? rest8<T>(s[t >> 1], p, t & 1) : p;
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b) {
-                const vec8<T> f = tr_frag<T, DP>(vt, trl, 16 * t, b);
+                const vec8<T> f = tr_frag<T, DP>(vt, tl, 16 * t, b);
                 if constexpr (NW == 1) o[b] = mfma16(f, rest, o[b]);
                 o[b] = mfma16(f, p, o[b]);
             }
@@ -263,14 +264,14 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_fwd
 }
 
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_dq16_kernel(CrossArgs a) {
-    constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
+__global__ __launch_bounds__(NW * 64, NW > 1 ? (DP <= 64 ? 3 : 2) : DP == 32 ? 2 : 1) void cross_dq16_kernel(CrossArgs a) {
+    constexpr int TILE = KT * TileRow<DP>::BYTES, NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
     int item, kvh;
     if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int trl = tr_lane<DP>(lane);
+    const TileLane<DP> tl(lane);
     constexpr f32x16 zero = {};
     vec8<T> qf[DP / 16], gf[DP / 16];
     const int row = it.r0 + wave * 32 + col;
@@ -335,8 +336,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_dq1
             f32x16 s, dp;
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                const vec8<T> fk = row_frag<T, DP>(kt, 32 * hb, i, col, half);
-                const vec8<T> fv = row_frag<T, DP>(vt, 32 * hb, i, col, half);
+                const vec8<T> fk = row_frag<T, DP>(kt, tl, 32 * hb, i);
+                const vec8<T> fv = row_frag<T, DP>(vt, tl, 32 * hb, i);
                 s = mfma16(fk, qf[i], i == 0 ? zero : s);
                 dp = mfma16(fv, gf[i], i == 0 ? zero : dp);
             }
@@ -357,7 +358,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_dq1
                 const vec8<T> rest = NW == 1 ? rest8<T>(s, p, t) : p;
 #pragma unroll
                 for (int b = 0; b < DP / 32; ++b) {
-                    const vec8<T> f = tr_frag<T, DP>(kt, trl, 32 * hb + 16 * t, b);
+                    const vec8<T> f = tr_frag<T, DP>(kt, tl, 32 * hb + 16 * t, b);
                     if constexpr (NW == 1) acc[b] = mfma16(f, rest, acc[b]);
                     acc[b] = mfma16(f, p, acc[b]);
                 }
@@ -383,14 +384,14 @@ __global__ __launch_bounds__(NW * 64, NW > 1 || DP == 32 ? 2 : 1) void cross_dq1
 
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cross_dkv16_kernel(CrossArgs a) {
-    constexpr int TILE = KT * pitch<DP>(), NT = NW * 64;
+    constexpr int TILE = KT * TileRow<DP>::BYTES, NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];   // lse, delta
     int item, kvh;
     if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int trl = tr_lane<DP>(lane);
+    const TileLane<DP> tl(lane);
     constexpr f32x16 zero = {};
     vec8<T> kf[DP / 16], vf[DP / 16];
     const int key = it.r0 + wave * 32 + col;
@@ -446,8 +447,8 @@ __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cro
             f32x16 s, dp;
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                const vec8<T> fq = row_frag<T, DP>(qt, 32 * rb, i, col, half);
-                const vec8<T> fg = row_frag<T, DP>(gt, 32 * rb, i, col, half);
+                const vec8<T> fq = row_frag<T, DP>(qt, tl, 32 * rb, i);
+                const vec8<T> fg = row_frag<T, DP>(gt, tl, 32 * rb, i);
                 s = mfma16(fq, kf[i], i == 0 ? zero : s);
                 dp = mfma16(fg, vf[i], i == 0 ? zero : dp);
             }
@@ -472,8 +473,8 @@ __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cro
                 const vec8<T> ds_rest = NW == 1 ? rest8<T>(dp, ds, t) : ds;
 #pragma unroll
                 for (int b = 0; b < DP / 32; ++b) {
-                    const vec8<T> fg = tr_frag<T, DP>(gt, trl, 32 * rb + 16 * t, b);
-                    const vec8<T> fq = tr_frag<T, DP>(qt, trl, 32 * rb + 16 * t, b);
+                    const vec8<T> fg = tr_frag<T, DP>(gt, tl, 32 * rb + 16 * t, b);
+                    const vec8<T> fq = tr_frag<T, DP>(qt, tl, 32 * rb + 16 * t, b);
                     if constexpr (NW == 1) {
                         dv[b] = mfma16(fg, p_rest, dv[b]);
                         dk[b] = mfma16(fq, ds_rest, dk[b]);

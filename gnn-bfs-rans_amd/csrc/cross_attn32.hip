@@ -78,10 +78,10 @@ __device__ __forceinline__ Frag3 split_acc(const f32x16& w, int t) {
 // One thread's share of KT rows of fp32, split at the store into three tiles
 template <int DP, int NT>
 struct Stage3 {
-    static constexpr int C4 = DP / 4, N = KT * C4 / NT, TILE = KT * pitch<DP>();
+    static constexpr int C4 = DP / 4, N = KT * C4 / NT, TILE = KT * TileRow<DP>::BYTES;
     static_assert(KT * C4 % NT == 0, "tile share");
     f32x4 v[N];
-    int off[N];
+    int off[N], lds[N];
     uint32_t bytes;
     __device__ __forceinline__ static int row(int j) { return (threadIdx.x + j * NT) / C4; }
     __device__ __forceinline__ static int chunk(int j) { return (threadIdx.x + j * NT) % C4; }
@@ -91,6 +91,7 @@ struct Stage3 {
         for (int j = 0; j < N; ++j) {
             const int t = row(j) / group, h = row(j) - t * group;
             off[j] = chunk(j) * 4 < d ? static_cast<int>((t * ldt + h * ldh + chunk(j) * 4) * 4) : NO_LOAD;
+            lds[j] = TileRow<DP>::at(row(j), chunk(j) * 4);
         }
         bytes = uniform(static_cast<int>((KT / group * ldt + group * ldh + d) * 4));
     }
@@ -108,7 +109,7 @@ struct Stage3 {
             uint2 h, m, l;
             split2(v[j][0], v[j][1], h.x, m.x, l.x);
             split2(v[j][2], v[j][3], h.y, m.y, l.y);
-            char* p = tile + row(j) * pitch<DP>() + chunk(j) * 8;
+            char* p = tile + lds[j];
             *reinterpret_cast<uint2*>(p) = h;
             *reinterpret_cast<uint2*>(p + TILE) = m;
             *reinterpret_cast<uint2*>(p + 2 * TILE) = l;
@@ -117,31 +118,31 @@ struct Stage3 {
 };
 
 template <int DP>
-__device__ __forceinline__ Frag3 row3(const char* tile, int i, int col, int half) {
-    constexpr int TILE = KT * pitch<DP>();
-    return {row_frag<B, DP>(tile, 0, i, col, half), row_frag<B, DP>(tile + TILE, 0, i, col, half),
-            row_frag<B, DP>(tile + 2 * TILE, 0, i, col, half)};
+__device__ __forceinline__ Frag3 row3(const char* tile, const TileLane<DP>& tl, int i) {
+    constexpr int TILE = KT * TileRow<DP>::BYTES;
+    return {row_frag<B, DP>(tile, tl, 0, i), row_frag<B, DP>(tile + TILE, tl, 0, i),
+            row_frag<B, DP>(tile + 2 * TILE, tl, 0, i)};
 }
 template <int DP>
-__device__ __forceinline__ Frag3 tr3(const char* tile, int trl, int row, int b) {
-    constexpr int TILE = KT * pitch<DP>();
-    return {tr_frag<B, DP>(tile, trl, row, b), tr_frag<B, DP>(tile + TILE, trl, row, b),
-            tr_frag<B, DP>(tile + 2 * TILE, trl, row, b)};
+__device__ __forceinline__ Frag3 tr3(const char* tile, const TileLane<DP>& tl, int row, int b) {
+    constexpr int TILE = KT * TileRow<DP>::BYTES;
+    return {tr_frag<B, DP>(tile, tl, row, b), tr_frag<B, DP>(tile + TILE, tl, row, b),
+            tr_frag<B, DP>(tile + 2 * TILE, tl, row, b)};
 }
 
-// (three tiles each of K and V, twice: 37 KB of LDS for heads of 32, 111 KB for
+// (three tiles each of K and V, twice: 25 KB of LDS for heads of 32, 98 KB for
 // 128; 64 keys a tile measured 5 % slower)
 template <int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP <= 32 ? 3 : DP <= 64 ? 2 : 1) void cross_fwd32_kernel(
     CrossArgs a) {
-    constexpr int TILE3 = 3 * KT * pitch<DP>(), NT = NW * 64;
+    constexpr int TILE3 = 3 * KT * TileRow<DP>::BYTES, NT = NW * 64;
     constexpr f32x16 zero = {};
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE3];   // K, V; twice
     int item, kvh;
     if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int trl = tr_lane<DP>(lane);
+    const TileLane<DP> tl(lane);
     const int row = it.r0 + wave * 32 + col;
     const int qt = row / a.group, qh = kvh * a.group + row - qt * a.group;
     const int64_t token = it.q_begin + static_cast<int64_t>(qt);
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP <= 32 ? 3 : DP <= 64 ? 2 
         f32x16 s;
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i)
-            s = mfma3(row3<DP>(kt, i, col, half), qf[i], i == 0 ? zero : s);
+            s = mfma3(row3<DP>(kt, tl, i), qf[i], i == 0 ? zero : s);
         if (bits != ~0u) {
             const uint32_t mine = bits >> (4 * half);
 #pragma unroll
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP <= 32 ? 3 : DP <= 64 ? 2 
         for (int t = 0; t < 2; ++t) {
             const Frag3 p = split_acc(s, t);
 #pragma unroll
-            for (int b = 0; b < DP / 32; ++b) o[b] = mfma3(tr3<DP>(vt, trl, 16 * t, b), p, o[b]);
+            for (int b = 0; b < DP / 32; ++b) o[b] = mfma3(tr3<DP>(vt, tl, 16 * t, b), p, o[b]);
         }
         if (more) write(buf ^ 1);
         __syncthreads();
@@ -236,14 +237,14 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP <= 32 ? 3 : DP <= 64 ? 2 
 
 template <int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq32_kernel(CrossArgs a) {
-    constexpr int TILE3 = 3 * KT * pitch<DP>(), NT = NW * 64;
+    constexpr int TILE3 = 3 * KT * TileRow<DP>::BYTES, NT = NW * 64;
     constexpr f32x16 zero = {};
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE3];   // K, V; twice
     int item, kvh;
     if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int trl = tr_lane<DP>(lane);
+    const TileLane<DP> tl(lane);
     const int row = it.r0 + wave * 32 + col;
     const bool live = row < it.r1;
     const int qt = row / a.group, qh = kvh * a.group + row - qt * a.group;
@@ -302,8 +303,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq3
         f32x16 s, dp;
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            s = mfma3(row3<DP>(kt, i, col, half), qf[i], i == 0 ? zero : s);
-            dp = mfma3(row3<DP>(vt, i, col, half), gf[i], i == 0 ? zero : dp);
+            s = mfma3(row3<DP>(kt, tl, i), qf[i], i == 0 ? zero : s);
+            dp = mfma3(row3<DP>(vt, tl, i), gf[i], i == 0 ? zero : dp);
         }
         const uint32_t mine = bits >> (4 * half);
 #pragma unroll
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq3
         for (int t = 0; t < 2; ++t) {
             const Frag3 p = split_acc(s, t);
 #pragma unroll
-            for (int b = 0; b < DP / 32; ++b) acc[b] = mfma3(tr3<DP>(kt, trl, 16 * t, b), p, acc[b]);
+            for (int b = 0; b < DP / 32; ++b) acc[b] = mfma3(tr3<DP>(kt, tl, 16 * t, b), p, acc[b]);
         }
         if (more) write(buf ^ 1);
         __syncthreads();
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 64 ? 2 : 1) void cross_dq3
 
 template <int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv32_kernel(CrossArgs a) {
-    constexpr int TILE3 = 3 * KT * pitch<DP>(), NT = NW * 64;
+    constexpr int TILE3 = 3 * KT * TileRow<DP>::BYTES, NT = NW * 64;
     constexpr f32x16 zero = {};
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE3];   // q, do; twice
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];    // lse, delta
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv
     if (!cross_work(a, item, kvh)) return;
     const CrossItem it = load_item(a, item);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int trl = tr_lane<DP>(lane);
+    const TileLane<DP> tl(lane);
     const int key = it.r0 + wave * 32 + col;
     const int64_t kt = it.k_begin + static_cast<int64_t>(key);
     const bool live = key < it.r1, keep = live && (!a.mask || a.mask[kt]);
@@ -388,8 +389,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv
         f32x16 s, dp;
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            s = mfma3(row3<DP>(qt, i, col, half), kf[i], i == 0 ? zero : s);
-            dp = mfma3(row3<DP>(gt, i, col, half), vf[i], i == 0 ? zero : dp);
+            s = mfma3(row3<DP>(qt, tl, i), kf[i], i == 0 ? zero : s);
+            dp = mfma3(row3<DP>(gt, tl, i), vf[i], i == 0 ? zero : dp);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -407,8 +408,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && DP <= 32 ? 2 : 1) void cross_dkv
             const Frag3 p = split_acc(s, t), ds = split_acc(dp, t);
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b) {
-                dv[b] = mfma3(tr3<DP>(gt, trl, 16 * t, b), p, dv[b]);
-                dk[b] = mfma3(tr3<DP>(qt, trl, 16 * t, b), ds, dk[b]);
+                dv[b] = mfma3(tr3<DP>(gt, tl, 16 * t, b), p, dv[b]);
+                dk[b] = mfma3(tr3<DP>(qt, tl, 16 * t, b), ds, dk[b]);
             }
         }
         if (more) write(buf ^ 1);

@@ -20,36 +20,63 @@ __device__ __forceinline__ f32x16 mfma16(vec8<f16_t> a, vec8<f16_t> b, f32x16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// Row pitch of a tile in bytes: its width plus 32, so that neither 8 rows'
-// 16-byte reads nor 4 rows' transposed reads meet in a bank
+// LDS tile of rows of DP 16-bit columns: row r at r ROWB, its 16-byte chunk c
+// in place c ^ h(r).  h is chosen so that in any 16 rows (aligned) one chunk of
+// each, and in any 4 rows (aligned) four neighbouring chunks, lie in different
+// banks, whether 128 or 256 bytes go by a cycle: the reads of a product over
+// columns (16 bytes a lane, a lane a row) and the transposed reads (4 rows x 16
+// columns a 16-lane group).  (A pitch of the width plus 32 bytes, without h,
+// spent 40 % of its LDS cycles on conflicts of the former.)
 template <int DP>
-constexpr int pitch() { return DP * 2 + 32; }
+struct TileRow {
+    static constexpr int BYTES = DP == 96 ? 256 : DP * 2;
+    __device__ __forceinline__ static int h(int r) {
+        if constexpr (DP == 32) return (((r >> 1) ^ (r >> 3)) & 1) << 1 | ((r >> 2) & 1);
+        if constexpr (DP == 64) return ((r & 3) << 1 | ((r >> 2) & 1)) ^ ((r >> 3) & 1) << 1;
+        return (r & 3) << 1 | ((r >> 2) & 1) | (((r >> 3) ^ r) & 1) << 3;
+    }
+    // byte of column c (a multiple of 4) in row r
+    __device__ __forceinline__ static int at(int r, int c) {
+        return r * BYTES + (((c >> 3) ^ h(r)) << 4) + 2 * (c & 7);
+    }
+};
 
-// the transposed read's share of a lane: row 4 half + (l % 16) / 4, columns
-// 16 ((l / 16) % 2) + 4 (l % 4) ..+3
+// A lane's byte offsets in a tile
 template <int DP>
-__device__ __forceinline__ int tr_lane(int lane) {
-    return (4 * (lane >> 5) + ((lane & 15) >> 2)) * pitch<DP>() + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
-}
+struct TileLane {
+    int row[DP / 16];        // row l % 32, columns 16 i + 8 (l / 32) ..+7
+    int tr[DP / 32][2];      // rows 4 (l / 32) + (l % 16) / 4 (+ 8), columns 32 b + 16 ((l / 16) % 2) + 4 (l % 4) ..+3
+    __device__ __forceinline__ explicit TileLane(int lane) {
+        const int half = lane >> 5, r = lane & 31, q = 4 * half + ((lane & 15) >> 2);
+        const int c = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) row[i] = TileRow<DP>::at(r, 16 * i + 8 * half);
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) {
+            tr[b][0] = TileRow<DP>::at(q, 32 * b + c);
+            tr[b][1] = TileRow<DP>::at(q + 8, 32 * b + c);
+        }
+    }
+};
 
-// A operand of a product over rows row + (the accumulator's order of 16) of a
-// tile: columns 32 b + l % 32
+// A operand of a product over rows r (a multiple of 16) + (the accumulator's
+// order of 16) of a tile: columns 32 b + l % 32
 template <typename T, int DP>
-__device__ __forceinline__ vec8<T> tr_frag(const char* tile, int trl, int row, int b) {
-    const char* p = tile + trl + row * pitch<DP>() + 64 * b;
+__device__ __forceinline__ vec8<T> tr_frag(const char* tile, const TileLane<DP>& tl, int r, int b) {
+    const char* p = tile + r * TileRow<DP>::BYTES;
     union {
         s16x4 h[2];
         vec8<T> v;
     } u;
-    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * pitch<DP>()));
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + tl.tr[b][0]));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + tl.tr[b][1]));
     return u.v;
 }
 
-// A operand of a product over columns: row r + l % 32, columns 16 i + 8 half ..+7
+// A operand of a product over columns 16 i ..+15: rows r (a multiple of 32) + l % 32
 template <typename T, int DP>
-__device__ __forceinline__ vec8<T> row_frag(const char* tile, int r, int i, int col, int half) {
-    return *reinterpret_cast<const vec8<T>*>(tile + (r + col) * pitch<DP>() + 32 * i + 16 * half);
+__device__ __forceinline__ vec8<T> row_frag(const char* tile, const TileLane<DP>& tl, int r, int i) {
+    return *reinterpret_cast<const vec8<T>*>(tile + r * TileRow<DP>::BYTES + tl.row[i]);
 }
 
 // Which of a tile's keys take part (bit = key), for every lane: the mask's
