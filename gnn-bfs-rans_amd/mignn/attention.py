@@ -227,7 +227,12 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Cro
     h // (heads // kv_heads).  key_mask: bool [keys], False leaves a key out,
     whatever its rows hold.  scale: > 0, default 1 / sqrt(d).  Returns
     [queries, heads, d]; a query without keys gets 0, and no gradient flows
-    through it."""
+    through it.
+
+    fp32 rows are multiplied as three bf16 terms each, to fp32's own rounding;
+    there an infinite key or value makes NaN of the queries that read it.  16-bit
+    rows: the weights are rounded to the rows' type ahead of their product with
+    the values."""
     want_q = (plan.queries, plan.heads, plan.head_dim)
     want_k = (plan.keys, plan.kv_heads, plan.head_dim)
     for name, t, want in (("q", q, want_q), ("k", k, want_k), ("v", v, want_k)):

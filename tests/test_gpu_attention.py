@@ -226,6 +226,7 @@ CROSS = [
     ([129], [129], 2, 2, 40), ([64], [200], 3, 1, 96), ([70, 70], [40, 150], 4, 4, 128),
     ([1] * 9, [1, 2, 3, 15, 16, 17, 63, 64, 900], 8, 1, 72), ([300], [3], 4, 1, 56),
     ([2], [5000], 4, 4, 32), ([2100], [20], 4, 2, 64), ([260], [1111], 2, 2, 104),
+    ([2, 1], [3000, 70], 8, 2, 48), ([7, 90], [100, 40], 32, 1, 32), ([31], [300], 6, 2, 128),
 ]
 
 
@@ -468,6 +469,114 @@ def test_operators_in_captured_graphs():
         for i in (0, 1):
             for a, b in zip(outs[i], step(states[i])):
                 assert torch.equal(a, b)
+
+
+def test_gradients_are_first_order_only():
+    """create_graph gives the gradients; differentiating them again is refused."""
+    x = rnd(6, 32, seed=1).requires_grad_()
+    w = torch.ones(32, device=DEV, requires_grad=True)
+    axes = A.RotaryAxes((8,))
+    plan = A.CrossPlan([6], [6], heads=1, head_dim=32)
+
+    def ops():
+        yield A.rms_norm(x, w)
+        yield A.rms_norm(x, w, residual=x)[0]
+        yield A.rotary(x.view(6, 1, 32), torch.arange(6, device=DEV)[:, None], axes)
+        yield A.cross_attention(*(x.view(6, 1, 32),) * 3, plan)
+    for y in ops():
+        plain, = torch.autograd.grad(y.square().sum(), x, retain_graph=True)
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        assert torch.equal(g.detach(), plain) and g.requires_grad
+        with pytest.raises(RuntimeError, match="first order only"):
+            g.sum().backward(retain_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.parametrize("queries", [1, 40])
+def test_cross_attention_offsets_past_32_bits(queries):
+    """17 million keys of 128 bf16 columns (2^31.02 elements) of which the mask
+    keeps some at both ends: outputs and gradients equal those of the kept keys."""
+    n, d = 17_000_000, 128
+    keep = torch.cat([torch.arange(0, 60), torch.arange(n - 90, n)])
+    k = torch.zeros(n, 1, d, dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros_like(k)
+    ks, vs = rnd(150, 1, d, seed=1, dt=torch.bfloat16), rnd(150, 1, d, seed=2, dt=torch.bfloat16)
+    k[keep.to(DEV)], v[keep.to(DEV)] = ks, vs
+    mask = torch.zeros(n, dtype=torch.bool, device=DEV)
+    mask[keep.to(DEV)] = True
+    q, do = (rnd(queries, 2, d, seed=s, dt=torch.bfloat16) for s in (3, 4))
+    plan = A.CrossPlan([queries], [n], heads=2, kv_heads=1, head_dim=d, dtype=torch.bfloat16)
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = A.cross_attention(q, k, v, plan, key_mask=mask)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+    ref = orc.cross_attention(q, ks, vs, [queries], [150], None, None, do)
+    # (the sums run over 150 weights that are not 0)
+    bound = cross_bounds(ref, torch.bfloat16, d, [150], [queries], 2)
+    close(out, ref["out"], bound["out"], torch.bfloat16, "out")
+    close(dq, ref["dq"], bound["dq"], torch.bfloat16, "dq")
+    close(dk[keep.to(DEV)], ref["dk"], bound["dk"], torch.bfloat16, "dk")
+    close(dv[keep.to(DEV)], ref["dv"], bound["dv"], torch.bfloat16, "dv")
+    assert dk[~mask].count_nonzero() == 0 and dv[~mask].count_nonzero() == 0
+
+
+def test_norm_and_rotary_offsets_past_32_bits():
+    n, h = 17_000_000, 128
+    x = torch.empty(n, h, dtype=torch.bfloat16, device=DEV)
+    x[:] = rnd(1, h, seed=1, dt=torch.bfloat16)
+    x[-300:] = rnd(300, h, seed=2, dt=torch.bfloat16)
+    w = rnd(h, seed=3, dt=torch.bfloat16)
+    y = A.rms_norm(x, w)
+    assert torch.equal(y[-300:], A.rms_norm(x[-300:].clone(), w))
+    assert torch.equal(y[:-300], y[:1].expand(n - 300, h))
+    del y
+    pos = torch.zeros(n, 1, dtype=torch.int64, device=DEV)
+    pos[-300:, 0] = torch.arange(300, device=DEV) * 1000
+    axes = A.RotaryAxes((16,))
+    y = A.rotary(x.view(n, 4, 32), pos, axes)
+    assert torch.equal(y[-300:], A.rotary(x[-300:].clone().view(300, 4, 32), pos[-300:], axes))
+    assert torch.equal(y[:-300], x[:-300].view(-1, 4, 32))
+
+
+def test_cross_attention_from_two_threads_and_streams():
+    """Two threads, each on its own stream, over one plan: every result is the
+    single call's."""
+    import threading
+    ql, kl, d = [300, 5], [900, 4000], 64
+    plan = A.CrossPlan(ql, kl, heads=4, kv_heads=2, head_dim=d, dtype=torch.bfloat16)
+    sets = [cross_inputs(ql, kl, 4, 2, d, torch.bfloat16, seed=30 * i)[:3] for i in (0, 1)]
+    want = [A.cross_attention(*s, plan) for s in sets]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(20):
+                    got[i].append(A.cross_attention(*sets[i], plan))
+            st.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i in (0, 1):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_cross_attention_wide_strides_are_copied():
+    """Rows further apart than the kernels' offsets reach (2^23 elements)."""
+    base = torch.zeros(4, (1 << 23) + 64, device=DEV)
+    base[:, :64] = rnd(4, 64, seed=1)
+    q = base[:, :64].unflatten(1, (2, 32))
+    plan = A.CrossPlan([4], [4], heads=2, head_dim=32)
+    c = q.contiguous()
+    assert torch.equal(A.cross_attention(q, q, q, plan), A.cross_attention(c, c, c, plan))
 
 
 # ---------------------------------------------------------------------------
