@@ -133,7 +133,7 @@ __device__ __forceinline__ Frag3 tr3(const char* tile, const TileLane<DP>& tl, i
 // (three tiles each of K and V, twice: 25 KB of LDS for heads of 32, 98 KB for
 // 128; 64 keys a tile measured 5 % slower)
 template <int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP <= 32 ? 3 : DP <= 64 ? 2 : 1) void cross_fwd32_kernel(
+__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP <= 64 ? 3 : 1) void cross_fwd32_kernel(
     CrossArgs a) {
     constexpr int TILE3 = 3 * KT * TileRow<DP>::BYTES, NT = NW * 64;
     constexpr f32x16 zero = {};
