@@ -194,19 +194,23 @@ __global__ __launch_bounds__(NORM_WAVES * 64) void rms_norm_backward_kernel(Norm
     }
 }
 
-// dw[c] = sum of the blocks' partials, in block order: 8 columns a block, 32
-// threads a column, the threads' sums by a fixed tree
+// dw[c] = sum of the blocks' partials: 8 columns a block, 128 threads a column
+// that take every 128th partial (all in flight), their sums by a fixed tree
 template <typename W>
-__global__ __launch_bounds__(256) void rms_norm_dw_kernel(const float* part, int blocks, int h,
-                                                          W* dw) {
-    __shared__ float acc[256];
+__global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* part, int blocks, int h, W* dw) {
+    __shared__ float acc[1024];
     const int c = blockIdx.x * 8 + (threadIdx.x & 7), k0 = threadIdx.x >> 3;
     float v = 0.f;
-    if (c < h)
-        for (int k = k0; k < blocks; k += 32) v += part[static_cast<int64_t>(k) * h + c];
+    if (c < h) {
+#pragma unroll
+        for (int i = 0; i < NORM_MAX_GRID / 128; ++i) {
+            const int k = k0 + 128 * i;
+            if (k < blocks) v += part[static_cast<int64_t>(k) * h + c];
+        }
+    }
     acc[threadIdx.x] = v;
     __syncthreads();
-    for (int m = 128; m >= 8; m >>= 1) {
+    for (int m = 512; m >= 8; m >>= 1) {
         if (threadIdx.x < m) acc[threadIdx.x] += acc[threadIdx.x + m];
         __syncthreads();
     }
@@ -345,13 +349,13 @@ extern "C" int mignn_rms_norm_backward(const void* x, int64_t ldx, const void* r
     const dim3 grid((h + 7) / 8);
     const int blocks = static_cast<int>(sh.grid);
     if (weight_f32 || dtype == MIGNN_ROW_F32)
-        hipLaunchKernelGGL(rms_norm_dw_kernel<float>, grid, dim3(256), 0, st, a.dw_part, blocks, h,
+        hipLaunchKernelGGL(rms_norm_dw_kernel<float>, grid, dim3(1024), 0, st, a.dw_part, blocks, h,
                            static_cast<float*>(dw));
     else if (dtype == MIGNN_ROW_BF16)
-        hipLaunchKernelGGL(rms_norm_dw_kernel<bf16_t>, grid, dim3(256), 0, st, a.dw_part, blocks, h,
+        hipLaunchKernelGGL(rms_norm_dw_kernel<bf16_t>, grid, dim3(1024), 0, st, a.dw_part, blocks, h,
                            static_cast<bf16_t*>(dw));
     else
-        hipLaunchKernelGGL(rms_norm_dw_kernel<f16_t>, grid, dim3(256), 0, st, a.dw_part, blocks, h,
+        hipLaunchKernelGGL(rms_norm_dw_kernel<f16_t>, grid, dim3(1024), 0, st, a.dw_part, blocks, h,
                            static_cast<f16_t*>(dw));
     return launch_status("rms_norm_dw_kernel");
 }
