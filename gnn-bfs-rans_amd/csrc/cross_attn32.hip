@@ -22,15 +22,18 @@ using B = bf16_t;
 
 constexpr int KT = 32;   // rows of an LDS tile
 
-// (two numbers at a time: one conversion instruction makes a pair)
-__device__ __forceinline__ void split2(float a, float b, uint32_t& h, uint32_t& m, uint32_t& l) {
+// x = h + m + l, two numbers at a time: one instruction converts a pair
+__device__ __forceinline__ uint32_t pair_bits(float a, float b) {
+    typedef float f32pair __attribute__((ext_vector_type(2)));
     typedef B pair __attribute__((ext_vector_type(2)));
-    auto bits = [](pair p) { return __builtin_bit_cast(uint32_t, p); };
-    h = bits(pair{static_cast<B>(a), static_cast<B>(b)});
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32pair{a, b}), pair));
+}
+__device__ __forceinline__ void split2(float a, float b, uint32_t& h, uint32_t& m, uint32_t& l) {
+    h = pair_bits(a, b);
     a -= __uint_as_float(h << 16), b -= __uint_as_float(h & 0xffff0000u);
-    m = bits(pair{static_cast<B>(a), static_cast<B>(b)});
+    m = pair_bits(a, b);
     a -= __uint_as_float(m << 16), b -= __uint_as_float(m & 0xffff0000u);
-    l = bits(pair{static_cast<B>(a), static_cast<B>(b)});
+    l = pair_bits(a, b);
 }
 
 struct Frag3 {
