@@ -342,9 +342,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? (DP <= 64 ? 3 : 2) : DP == 32 ? 2
                 dp = mfma16(fv, gf[i], i == 0 ? zero : dp);
             }
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, sc.up - lse)) *
-                               (dp[r] - delta);
+            for (int r = 0; r < 16; ++r)
+                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, sc.up - lse)) * (dp[r] - delta);
             if (bits != ~0ull) {
                 const uint32_t mine = static_cast<uint32_t>(bits >> (32 * hb + 4 * half));
 #pragma unroll

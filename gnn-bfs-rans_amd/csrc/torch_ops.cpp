@@ -46,6 +46,11 @@ void check(int rc, const char* what) {
 }
 
 void* stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+// A plan's or an axes' table may have been made on another stream than the one
+// that reads it: its memory is not given away before this stream is done
+void reads(const Tensor& t) {
+    t.record_stream(c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device()));
+}
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* out(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 bool is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
@@ -182,6 +187,7 @@ Tensor turn(const Tensor& x_, const Tensor& pos_, const Tensor& freq, const Tens
                          : pos.scalar_type() == at::kInt ? MIGNN_POS_I32 : MIGNN_POS_I64;
     const int64_t n = x.size(0), heads = x.size(1), d = x.size(2);
     Tensor y = at::empty({n, heads, d}, x.options());
+    reads(freq), reads(axis);
     check(lib.rotary(ptr(x), x.stride(0), x.stride(1), n, static_cast<int>(heads), static_cast<int>(d), ptr(pos),
                      pos_type, pos.stride(0), static_cast<const double*>(ptr(freq)),
                      static_cast<const int32_t*>(ptr(axis)), static_cast<int>(freq.numel()), interleaved, inverse,
@@ -237,8 +243,9 @@ struct CrossOut {
 };
 
 CrossOut cross_forward(const mignn_cross_call& plan, const Tensor& q_, const Tensor& k_, const Tensor& v_,
-                       const Tensor& mask, double scale, bool train) {
+                       const Tensor& mask, const Tensor& lists, double scale, bool train) {
     c10::DeviceGuard guard(q_.device());
+    reads(lists);
     const Tensor q = heads_of(q_, 16), k = heads_of(k_, 16), v = heads_of(v_, 16);
     CrossOut o;
     o.out = at::empty(q.sizes(), q.options());
@@ -260,7 +267,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
                           const OptTensor& mask, const Tensor& lists, const std::string& plan, double scale) {
         mignn_cross_call c;
         std::memcpy(&c, plan.data(), sizeof(c));
-        const CrossOut o = cross_forward(c, q, k, v, value(mask), scale, true);
+        const CrossOut o = cross_forward(c, q, k, v, value(mask), lists, scale, true);
         // out32 (the fp32 output): <do, o> from the rounded output would leave
         // the rounding of o in every dS.  lists: the plan's, kept alive
         ctx->save_for_backward({q, k, v, value(mask), o.out32, o.lse, lists});
@@ -302,7 +309,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     if (needs_grad({&q, &k, &v}))
         return CrossAttention::apply(q, k, v, mask, lists,
                                      std::string(reinterpret_cast<const char*>(&c), sizeof(c)), scale);
-    return cross_forward(c, q, k, v, value(mask), scale, false).out;
+    return cross_forward(c, q, k, v, value(mask), lists, scale, false).out;
 }
 
 }  // namespace

@@ -160,7 +160,8 @@ class CrossPlan:
     k_lens[b] keys, the sequences' rows back to back (one int: a single
     sequence).  Lengths of 0 are allowed.  Holds the launches' work lists on
     `device`; immutable, so it may serve any number of calls, streams and
-    captured graphs.  train=False leaves the backward's lists out."""
+    captured graphs (which need it for as long as they are replayed).
+    train=False leaves the backward's lists out."""
 
     __slots__ = ("q_lens", "k_lens", "queries", "keys", "heads", "kv_heads", "head_dim", "dtype",
                  "device", "train", "_call", "_lists", "_address")
@@ -315,11 +316,12 @@ class CrossAttention(nn.Module):
                          head_dim=self.head_dim, device=device, train=train)
 
     def _rotary_axes(self, device) -> RotaryAxes:
-        if self._axes is None or self._axes.device != device:
+        scales = (float(self.position_scale),) * self.axes
+        if self._axes is None or self._axes.device != device \
+                or (self._axes.base, self._axes.scales) != (self.base, scales):
             half = self.head_dim // 2
             pairs = [half // self.axes + (a < half % self.axes) for a in range(self.axes)]
-            self._axes = RotaryAxes(pairs, base=self.base,
-                                    scales=(self.position_scale,) * self.axes, device=device)
+            self._axes = RotaryAxes(pairs, base=self.base, scales=scales, device=device)
         return self._axes
 
     def keys_values(self, context: torch.Tensor, context_pos: torch.Tensor):

@@ -280,3 +280,14 @@ def test_ops_module_is_bound_to_the_product_library():
     assert all(n in _lib.SIGNATURES for n in _lib.OPS_ENTRIES)
     with pytest.raises(ValueError, match="entry points"):
         ops.bind([0])
+
+
+def test_block_axes_follow_its_settings():
+    blk = A.CrossAttention(64, 4)
+    cpu = torch.device("cpu")
+    first = blk._rotary_axes(cpu)
+    assert blk._rotary_axes(cpu) is first
+    blk.position_scale = 8.0
+    assert blk._rotary_axes(cpu).scales == (8.0,) * 3
+    blk.base = 50.0
+    assert blk._rotary_axes(cpu).base == 50.0

@@ -706,3 +706,34 @@ def test_surrogate_batch_of_graphs_reads_its_own_context():
                          blk.plan([n], [k]))
             assert (one - y[a0:a0 + n]).abs().max() <= 2.0 ** -12 * y.abs().max()
             a0, c0 = a0 + n, c0 + k
+
+
+def test_plan_and_axes_dropped_while_another_stream_reads_them():
+    """A plan and axes made on one stream, read by another and dropped: their
+    memory is not handed out again before the reader is done."""
+    x = rnd(3000, 3000, seed=1)
+    q = rnd(300, 2, 32, seed=2)
+    pos = torch.arange(300, device=DEV)[:, None]
+    plan = A.CrossPlan([300], [300], heads=2, head_dim=32)
+    axes = A.RotaryAxes((16,))
+    sizes = [plan._lists.numel(), 8 * axes.freq.numel(), 4 * axes.axis.numel()]
+    held = {t.data_ptr() for t in (plan._lists, axes.freq, axes.axis)}
+    want = A.cross_attention(q, q, q, plan), A.rotary(q, pos, axes)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(40):
+            x @ x
+        got = A.cross_attention(q, q, q, plan), A.rotary(q, pos, axes)
+    del plan, axes
+    new = {torch.empty(n, dtype=torch.uint8, device=DEV).data_ptr() for n in sizes}
+    busy = not side.query()
+    side.synchronize()
+    assert not busy or not held & new
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_out_of_memory_is_torch_s_error():
+    x, pos = torch.zeros(1, 1, 64, device=DEV), torch.zeros(1, 1, device=DEV)
+    with pytest.raises(torch.OutOfMemoryError):
+        A.rotary(x.expand(1 << 33, 1, 64), pos.expand(1 << 33, 1), A.RotaryAxes((32,)))
