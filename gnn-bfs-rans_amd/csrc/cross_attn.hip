@@ -8,6 +8,9 @@
 //   delta_i = <do_i, o_i>;  dS_ij = P_ij (<do_i, v_j> - delta_i)
 //   dq_i = scale sum_j dS_ij k_j;  dk_j = scale sum_i dS_ij q_i;  dv_j = sum_i P_ij do_i
 //
+// (scores and P are made again in each of the two gradient kernels, seven
+// products where four are new: dq's own kernel needs no atomics)
+//
 // One pass over the keys with the running maximum and sum of the softmax;
 // scores and P stay in registers: S^T = K Q^T puts a query in a lane's column,
 // so the maximum and the sum are in-lane but for one exchange between the
@@ -160,7 +163,9 @@ struct PassShape {
     int64_t tile;     // rows of a tile
     int64_t longest;  // of the r side
     int64_t slots;    // workgroups that the card holds at a time
-    int64_t least;    // shortest chunk: below it a part's join costs what the split gains
+    int64_t least;    // shortest chunk
+    int64_t rest;     // the same for what whole tiles leave over
+    double start, join, part;   // a workgroup's start, a join and each of its parts, in rows of the c side
     int64_t unit;     // chunks are a multiple of it
 };
 struct PassPlan {
@@ -180,7 +185,7 @@ int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 // dv 108 us in tiles of 32, 61 in tiles of 128.)
 PassShape pass_shape(const Sequence* seq, int64_t batch, int pass, int d, int dtype, int group) {
     const bool dkv = pass == MIGNN_CROSS_DKV;
-    PassShape s{128, 0, 512, 256, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
+    PassShape s{128, 0, 512, 128, 128, 64.0, 0.0, 0.0, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
     int64_t results = 0;   // of one kv head
     for (int64_t b = 0; b < batch; ++b) {
         s.longest = seq[b].rn > s.longest ? seq[b].rn : s.longest;
@@ -191,8 +196,21 @@ PassShape pass_shape(const Sequence* seq, int64_t batch, int pass, int d, int dt
     // registers and LDS: two workgroups of four waves a CU, one where the heads
     // are wide and much is held in fp32; eight small ones
     const bool wide = dtype == MIGNN_ROW_F32 ? d > 64 || (dkv && d > 32) : dkv && d > 96;
-    if (s.tile != 128) s.slots = 2048, s.least = 128;
-    else if (wide) s.slots = 256;
+    if (s.tile != 128) {
+        s.slots = 2048;
+        return s;
+    }
+    if (wide) s.slots = 256;
+    // 4 us to start a workgroup (its rows and first tile), 5 for a join's
+    // launch, 0.15 for each part it goes through, against the time of a row of
+    // the c side.  (A least chunk of 256 and no price on parts: 20
+    // sequences of up to 419 rows, 529 keys, 2 heads of 128, fp32 57 us, now 36; a least
+    // of 64 without the prices, 2 of 27 rows, 17025 keys, fp32: 45 -> 56.)
+    const double ns = (d + 31) / 32 * 32 * (dtype == MIGNN_ROW_F32 ? 0.55 : 0.12) *
+                      (pass == MIGNN_CROSS_FORWARD ? 1.0 : pass == MIGNN_CROSS_DQ ? 1.5 : 2.0);
+    s.start = 4000.0 / ns, s.join = 5000.0 / ns, s.part = 150.0 / ns;
+    if (dtype == MIGNN_ROW_F32) s.least = 64;
+    s.rest = 256;   // (128: 49181 rows x 4096 keys bf16, trained, 1038 -> 1046 us)
     return s;
 }
 
@@ -212,7 +230,8 @@ int64_t pick_chunk(const PassShape& s, const Sequence* seq, int64_t batch, int k
                 items += static_cast<double>((seq[b].rn + s.tile - 1) / s.tile) *
                          static_cast<double>((seq[b].cn + len - 1) / len);
         const int64_t rounds = (static_cast<int64_t>(items) * kv_heads + s.slots - 1) / s.slots;
-        const double cost = static_cast<double>(rounds) * static_cast<double>(len + s.least / 2);
+        const double cost = static_cast<double>(rounds) * (static_cast<double>(len) + s.start) +
+                            (parts > 1 ? s.join + s.part * static_cast<double>(parts) : 0.0);
         if (best_cost < 0.0 || cost < best_cost) best = len, best_cost = cost;
     }
     return best;
@@ -238,7 +257,8 @@ PassPlan plan_pass(const PassShape& s, const Sequence* seq, int64_t batch, int k
             int64_t parts = 1;
             if (t >= whole && cn > 0) {
                 parts = whole == 0 ? (cn + chunk - 1) / chunk : split;
-                if (parts > cn / s.least) parts = cn / s.least;
+                const int64_t least = whole == 0 ? s.least : s.rest;
+                if (parts > cn / least) parts = cn / least;
                 if (parts < 1) parts = 1;
             }
             // equal parts, each a multiple of the unit but the last
