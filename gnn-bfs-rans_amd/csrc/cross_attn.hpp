@@ -1,5 +1,5 @@
-// Shared by the cross-attention sources (cross_attn.hip: plan, exact fp32
-// kernels, joins; cross_attn16.hip: 16-bit kernels;
+// Shared by the cross-attention sources (cross_attn.hip: plan, joins, entry
+// points; cross_attn16.hip: 16-bit rows; cross_attn32.hip: fp32 rows;
 // cross_decode.hip: few rows).
 #pragma once
 

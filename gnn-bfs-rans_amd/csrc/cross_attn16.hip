@@ -1,8 +1,9 @@
 // Cross attention of bf16 and fp16 rows on the 16-bit matrix instructions
 // (formulas and pass structure: cross_attn.hip).
 //
-// A wave owns 32 rows (forward, dq) or keys (dk / dv) as MFMA columns.  The other side comes in LDS tiles of 64, double buffered through
-// registers: while a tile is worked on, the next one's rows are in flight.
+// A wave owns 32 rows (forward, dq) or keys (dk / dv) as MFMA columns.  The
+// other side comes in LDS tiles of 64, double buffered through registers:
+// while a tile is worked on, the next one's rows are in flight.
 //   S^T (keys x rows)   A = key rows, 16 bytes a lane;  B = q, in registers
 //   O^T (d x rows)      A = V^T, read transposed from the row-major tile
 //                       (ds_read_b64_tr_b16: 4 rows x 16 columns a 16-lane
@@ -15,10 +16,21 @@
 // matrix instruction takes both operands in one type), which adds to a result
 // about what its own rounding does; statistics, sums and accumulators are fp32.
 // Tiles of 32 (few rows or few results: bound by latency, not by the matrix
-// unit) carry the roundings' remainders through a second product instead.  bf16 has fp32's range.  fp16 has not: a weight of
-// 1 / 5000 is already subnormal there, so P is carried up by a constant power
-// of two and dS by one that each row (dq) or key (dk) lowers when its values
-// would not fit (DsScale); the results are brought back in fp32.
+// unit) carry the roundings' remainders through a second product instead.
+// bf16 has fp32's range.  fp16 has not: a weight of 1 / 5000 is already
+// subnormal there, so P is carried up by a constant power of two and dS by one
+// that each row (dq) or key (dk) lowers when its values would not fit
+// (DsScale); the results are brought back in fp32.
+//
+// Bound by issue: the matrix and the vector unit (exponentials, maxima,
+// roundings) are each busy about 44 % of the time and take turns within a
+// wave, so it is other waves that fill the gaps.  Measured (a plain product of
+// 8192^3 reaches 1203 TFLOP/s in bf16, 1150 in fp16): 49181 rows x 4096 keys x 4
+// heads over 2 of 64, bf16: forward 270 us (763 TFLOP/s), dq 340 (909), dk / dv
+// 460 (897); 2 x 16384^2 x 8 x 128, fp16: forward 2370 (928; 2105 us with the
+// softmax left out).  Heads to 64 run forward and dq at three waves a SIMD (dk
+// / dv, and all of 128 columns, spill there: 2790 us).  Tiles of 32 keys cost
+// 270 -> 296 us, reads of LDS ahead of time by fences of the scheduler 350 -> 404.
 #include "mfma16.hpp"
 
 namespace mignn {

