@@ -2,13 +2,16 @@
 // module (mignn/_ops.so) owns memory and the autograd graph, the arithmetic is
 // libmignn's C ABI.  In C++ because a call of a probe's size is a few
 // microseconds of work: a Python autograd function costs 60 us more a training
-// step, most of it in the engine's thread.  The arguments' checks are Python's
-// (mignn/attention.py); nothing here is called with unchecked shapes or types.
+// step, most of it in the engine's thread, and the arguments' checks 1.5 us a
+// call.
 #include <torch/extension.h>
 
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <array>
+#include <cmath>
 #include <cstring>
 #include <stdexcept>
 #include <string>
@@ -49,7 +52,9 @@ void* stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().
 // A plan's or an axes' table may have been made on another stream than the one
 // that reads it: its memory is not given away before this stream is done
 void reads(const Tensor& t) {
-    t.record_stream(c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device()));
+    if (t.is_cuda())
+        c10::hip::HIPCachingAllocator::recordStream(t.storage().data_ptr(),
+                                                    c10::hip::getCurrentHIPStream(t.device().index()));
 }
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* out(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -64,6 +69,32 @@ bool needs_grad(std::initializer_list<const Tensor*> ts) {
     for (const Tensor* t : ts)
         if (t->defined() && t->requires_grad()) return true;
     return false;
+}
+
+// ---------------------------------------------------------------------------
+// Refusals
+
+std::string shape(at::IntArrayRef sizes) {
+    std::string s = "(";
+    for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);
+    return s + (sizes.size() == 1 ? ",)" : ")");
+}
+std::string shape(const Tensor& t) { return shape(t.sizes()); }
+std::string dtype(const Tensor& t) { return py::str(py::cast(t).attr("dtype")); }
+std::string number(double v) { return py::str(py::float_(v)); }
+bool is_row(const Tensor& t) {
+    return is_f32(t) || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf;
+}
+void check_rows(const char* what, const Tensor& t) {
+    if (!is_row(t))
+        throw py::type_error(std::string(what) + ": rows must be float32, bfloat16 or float16, got " + dtype(t));
+}
+void on_device(const char* what, const Tensor& ref, std::initializer_list<std::pair<const char*, const Tensor*>> others) {
+    if (!ref.is_cuda()) throw std::runtime_error(std::string("mignn ") + what + " runs on ROCm devices only (no CPU path)");
+    for (const auto& [name, t] : others)
+        if (t->defined() && t->device() != ref.device())
+            throw std::runtime_error(std::string("mignn ") + what + ": " + name + " is on " + t->device().str() +
+                                     ", not on " + ref.device().str());
 }
 
 // Gradients that autograd cannot differentiate again: under create_graph they
@@ -151,6 +182,22 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
 };
 
 py::object rms_norm(const Tensor& x, const Tensor& w, const OptTensor& r, double eps) {
+    if (x.dim() != 2) throw py::value_error("rms_norm: x must be [N, H], got " + shape(x));
+    check_rows("rms_norm", x);
+    const int64_t h = x.size(1);
+    if (h < 1 || h > MIGNN_RMS_NORM_MAX_H)
+        throw py::value_error("rms_norm: width " + std::to_string(h) + " is not in 1.." +
+                              std::to_string(MIGNN_RMS_NORM_MAX_H));
+    if (w.dim() != 1 || w.size(0) != h)
+        throw py::value_error("rms_norm: weight must be [" + std::to_string(h) + "], got " + shape(w));
+    if (!is_f32(w) && w.scalar_type() != x.scalar_type())
+        throw py::type_error("rms_norm: weight must be float32 or " + dtype(x) + ", got " + dtype(w));
+    if (r.has_value() && (r->sizes() != x.sizes() || r->scalar_type() != x.scalar_type()))
+        throw py::value_error("rms_norm: residual must be " + shape(x) + " " + dtype(x) + ", got " + shape(*r) + " " +
+                              dtype(*r));
+    if (!(eps >= 0.0)) throw py::value_error("rms_norm: eps must not be negative, got " + number(eps));
+    const Tensor res = value(r);
+    on_device("rms_norm", x, {{"weight", &w}, {"residual", &res}});
     if (needs_grad({&x, &w}) || (r.has_value() && needs_grad({&*r}))) {
         variable_list o = RMSNorm::apply(x, w, r, eps);
         if (o.size() == 1) return py::cast(o[0]);
@@ -211,7 +258,24 @@ struct Rotary : torch::autograd::Function<Rotary> {
     }
 };
 
-Tensor rotary(const Tensor& x, const Tensor& pos, const Tensor& freq, const Tensor& axis, bool interleaved) {
+Tensor rotary(const Tensor& x, const Tensor& pos, const Tensor& freq, const Tensor& axis, int64_t axes,
+              bool interleaved) {
+    if (x.dim() != 3) throw py::value_error("rotary: x must be [N, heads, d], got " + shape(x));
+    check_rows("rotary", x);
+    if (pos.dim() != 2 || pos.size(0) != x.size(0) || pos.size(1) != axes)
+        throw py::value_error("rotary: pos must be [" + std::to_string(x.size(0)) + ", " + std::to_string(axes) +
+                              "], got " + shape(pos));
+    const auto pt = pos.scalar_type();
+    if (pt != at::kFloat && pt != at::kDouble && pt != at::kInt && pt != at::kLong)
+        throw py::type_error("rotary: pos must be float32, float64, int32 or int64, got " + dtype(pos));
+    if (2 * freq.numel() > x.size(2))
+        throw py::value_error("rotary: " + std::to_string(freq.numel()) + " pairs do not fit heads of width " +
+                              std::to_string(x.size(2)));
+    if (needs_grad({&pos})) {
+        PyErr_SetString(PyExc_NotImplementedError, "rotary: positions get no gradient (pass pos.detach())");
+        throw py::error_already_set();
+    }
+    on_device("rotary", x, {{"pos", &pos}, {"axes", &freq}});
     if (needs_grad({&x})) return Rotary::apply(x, pos, freq, axis, interleaved);
     return turn(x, pos, freq, axis, interleaved, false);
 }
@@ -303,13 +367,36 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     }
 };
 
-Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask,
-                       const Tensor& lists, uint64_t plan, double scale) {
+Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& key_mask,
+                       const c10::optional<double>& scale_, const Tensor& lists, uint64_t plan, int64_t queries,
+                       bool train) {
     const auto& c = *reinterpret_cast<const mignn_cross_call*>(plan);
-    if (needs_grad({&q, &k, &v}))
-        return CrossAttention::apply(q, k, v, mask, lists,
+    const std::array<int64_t, 3> want_q{queries, c.heads, c.d}, want_k{c.n_keys, c.kv_heads, c.d};
+    const auto type = c.dtype == MIGNN_ROW_F32 ? at::kFloat : c.dtype == MIGNN_ROW_BF16 ? at::kBFloat16 : at::kHalf;
+    auto check_like = [&](const char* name, const Tensor& t, const std::array<int64_t, 3>& want) {
+        if (t.sizes() != at::IntArrayRef(want))
+            throw py::value_error(std::string("cross_attention: the plan's ") + name + " is " + shape(want) +
+                                  ", got " + shape(t));
+        if (t.scalar_type() != type)
+            throw py::type_error(std::string("cross_attention: the plan's rows are ") +
+                                 dtype(at::empty({0}, type)) + ", " + name + " is " + dtype(t));
+    };
+    check_like("q", q, want_q), check_like("k", k, want_k), check_like("v", v, want_k);
+    Tensor mask = value(key_mask);
+    if (mask.defined() && (mask.scalar_type() != at::kBool || mask.dim() != 1 || mask.size(0) != c.n_keys))
+        throw py::value_error("cross_attention: key_mask must be bool [" + std::to_string(c.n_keys) + "], got " +
+                              dtype(mask) + " " + shape(mask));
+    const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt(static_cast<double>(c.d));
+    if (!(scale > 0.0 && scale < 1e30))
+        throw py::value_error("cross_attention: scale must be positive and finite, got " + number(scale));
+    on_device("cross_attention", q, {{"k", &k}, {"v", &v}, {"key_mask", &mask}, {"plan", &lists}});
+    if (mask.defined()) mask = mask.contiguous();
+    const bool grad = needs_grad({&q, &k, &v});
+    if (grad && !train) throw py::value_error("cross_attention: gradients need a plan built with train=True");
+    if (grad)
+        return CrossAttention::apply(q, k, v, mask.defined() ? OptTensor(mask) : OptTensor(), lists,
                                      std::string(reinterpret_cast<const char*>(&c), sizeof(c)), scale);
-    return cross_forward(c, q, k, v, value(mask), lists, scale, false).out;
+    return cross_forward(c, q, k, v, mask, lists, scale, false).out;
 }
 
 }  // namespace

@@ -8,10 +8,11 @@ over another graph of another size.
 
 Rows are fp32, bf16 or fp16; sums, softmax statistics and norms are fp32 and
 each output is rounded once.  All three run and differentiate in HIP kernels
-of libmignn.so (through _ops.so, csrc/torch_ops.cpp) on the tensors' device and
-its current stream; there is no CPU path.  Outputs and scratch come from PyTorch's allocator at every call, so
-calls on several streams, or captured into several graphs, share nothing but
-the read-only `RotaryAxes` / `CrossPlan`.  Gradients are first order only.
+of libmignn.so (through _ops.so, csrc/torch_ops.cpp, which also checks the
+arguments) on the tensors' device and its current stream; there is no CPU path.
+Outputs and scratch come from PyTorch's allocator at every call, so calls on
+several streams, or captured into several graphs, share nothing but the
+read-only `RotaryAxes` / `CrossPlan`.  Gradients are first order only.
 
 A graph batch is a list of lengths (one sequence a graph), rows back to back.
 """
@@ -20,7 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence
 
 import numpy as np
 import torch
@@ -30,12 +31,6 @@ from . import _lib
 from . import train_ops as T
 
 _ROW = {torch.float32: _lib.ROW_F32, torch.bfloat16: _lib.ROW_BF16, torch.float16: _lib.ROW_F16}
-_POS = (torch.float32, torch.float64, torch.int32, torch.int64)
-
-
-def _row_type(what: str, t: torch.Tensor):
-    if t.dtype not in _ROW:
-        raise TypeError(f"{what}: rows must be float32, bfloat16 or float16, got {t.dtype}")
 
 
 def _on_device(what: str, ref: torch.Tensor, **others):
@@ -58,22 +53,6 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     s = x + residual and (y, s) is returned, s being the stream that the next
     residual adds to.  y is formed from the unrounded s.  weight: [H], float32
     or x's type.  H <= 2048."""
-    if x.dim() != 2:
-        raise ValueError(f"rms_norm: x must be [N, H], got {tuple(x.shape)}")
-    _row_type("rms_norm", x)
-    h = x.shape[1]
-    if not 1 <= h <= _lib.RMS_NORM_MAX_H:
-        raise ValueError(f"rms_norm: width {h} is not in 1..{_lib.RMS_NORM_MAX_H}")
-    if weight.dim() != 1 or weight.shape[0] != h:
-        raise ValueError(f"rms_norm: weight must be [{h}], got {tuple(weight.shape)}")
-    if weight.dtype != torch.float32 and weight.dtype != x.dtype:
-        raise TypeError(f"rms_norm: weight must be float32 or {x.dtype}, got {weight.dtype}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError(f"rms_norm: residual must be {tuple(x.shape)} {x.dtype}, got "
-                         f"{tuple(residual.shape)} {residual.dtype}")
-    if not eps >= 0.0:
-        raise ValueError(f"rms_norm: eps must not be negative, got {eps}")
-    _on_device("rms_norm", x, weight=weight, residual=residual)
     return _lib.ops().rms_norm(x, weight, residual, eps)
 
 
@@ -119,21 +98,7 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, axes: RotaryAxes) -> torch.Tensor
     """x [N, heads, d] with the pairs of every head turned by the row's
     position pos [N, len(axes.pairs)] (float32 / float64 coordinates or int32 /
     int64 indices; angles are formed in float64).  Positions get no gradient."""
-    if x.dim() != 3:
-        raise ValueError(f"rotary: x must be [N, heads, d], got {tuple(x.shape)}")
-    _row_type("rotary", x)
-    if pos.dim() != 2 or pos.shape[0] != x.shape[0] or pos.shape[1] != len(axes.pairs):
-        raise ValueError(f"rotary: pos must be [{x.shape[0]}, {len(axes.pairs)}], got "
-                         f"{tuple(pos.shape)}")
-    if pos.dtype not in _POS:
-        raise TypeError("rotary: pos must be float32, float64, int32 or int64, got "
-                        f"{pos.dtype}")
-    if 2 * axes.total > x.shape[2]:
-        raise ValueError(f"rotary: {axes.total} pairs do not fit heads of width {x.shape[2]}")
-    if torch.is_grad_enabled() and pos.requires_grad:
-        raise NotImplementedError("rotary: positions get no gradient (pass pos.detach())")
-    _on_device("rotary", x, pos=pos, axes=axes.freq)
-    return _lib.ops().rotary(x, pos, axes.freq, axes.axis, axes.interleaved)
+    return _lib.ops().rotary(x, pos, axes.freq, axes.axis, len(axes.pairs), axes.interleaved)
 
 
 # ---------------------------------------------------------------------------
@@ -234,28 +199,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Cro
     there an infinite key or value makes NaN of the queries that read it.  16-bit
     rows: the weights are rounded to the rows' type ahead of their product with
     the values."""
-    want_q = (plan.queries, plan.heads, plan.head_dim)
-    want_k = (plan.keys, plan.kv_heads, plan.head_dim)
-    for name, t, want in (("q", q, want_q), ("k", k, want_k), ("v", v, want_k)):
-        if tuple(t.shape) != want:
-            raise ValueError(f"cross_attention: the plan's {name} is {want}, got {tuple(t.shape)}")
-        if t.dtype != plan.dtype:
-            raise TypeError(f"cross_attention: the plan's rows are {plan.dtype}, {name} is "
-                            f"{t.dtype}")
-    if key_mask is not None:
-        if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (plan.keys,):
-            raise ValueError(f"cross_attention: key_mask must be bool [{plan.keys}], got "
-                             f"{key_mask.dtype} {tuple(key_mask.shape)}")
-    scale = 1.0 / math.sqrt(plan.head_dim) if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"cross_attention: scale must be positive and finite, got {scale}")
-    _on_device("cross_attention", q, k=k, v=v, key_mask=key_mask, plan=plan._lists)
-    if key_mask is not None:
-        key_mask = key_mask.contiguous()
-    if not plan.train and torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
-                                                       or v.requires_grad):
-        raise ValueError("cross_attention: gradients need a plan built with train=True")
-    return _lib.ops().cross_attention(q, k, v, key_mask, plan._lists, plan._address, scale)
+    return _lib.ops().cross_attention(q, k, v, key_mask, scale, plan._lists, plan._address,
+                                      plan.queries, plan.train)
 
 
 # ---------------------------------------------------------------------------
