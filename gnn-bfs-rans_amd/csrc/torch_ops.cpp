@@ -169,7 +169,7 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
             if (want_w) {
                 dw = at::empty(w.sizes(), w.options());
                 bytes = lib.rms_norm_backward_scratch_bytes(n, static_cast<int>(h), row_type(x));
-                scratch = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+                if (bytes > 0) scratch = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
             }
             check(lib.rms_norm_backward(ptr(x), row_stride(x), ptr(r), row_stride(r), ptr(w), is_f32(w), n,
                                         static_cast<int>(h), static_cast<float>(ctx->saved_data["eps"].toDouble()),

@@ -741,7 +741,8 @@ int mignn_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr
                    const void* weight, int weight_f32, int64_t n, int h, float eps, int dtype,
                    void* y, int64_t ldy, void* s, int64_t lds, void* stream);
 /* Gradients: dx (the residual's is the same) from dy and, when given, ds (the
- * gradient of s); dw in the weight's type, or NULL.  Scratch is needed for dw. */
+ * gradient of s); dw in the weight's type, or NULL.  Scratch (0 bytes: none) is
+ * needed for dw. */
 size_t mignn_rms_norm_backward_scratch_bytes(int64_t n, int h, int dtype);
 int mignn_rms_norm_backward(const void* x, int64_t ldx, const void* residual, int64_t ldr,
                             const void* weight, int weight_f32, int64_t n, int h, float eps,

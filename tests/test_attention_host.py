@@ -168,10 +168,15 @@ def test_c_entry_points_check_arguments():
                     ({"n": -1}, "n = -1"), ({"x": None}, "null"), ({"ldx": 7}, "stride"),
                     ({"eps": -1.0}, "eps"), ({"ldy": 7}, "output")]:
         assert norm(**kw) == 1 and msg in _lib.last_error(), (kw, _lib.last_error())
-    need = L.mignn_rms_norm_backward_scratch_bytes(100, 8, 0)
+    need = L.mignn_rms_norm_backward_scratch_bytes(1000, 8, 0)
     assert need > 0 and L.mignn_rms_norm_backward_scratch_bytes(-1, 8, 0) == 0
-    assert L.mignn_rms_norm_backward(p, 8, None, 0, p, 1, 100, 8, 1e-6, 0, p, 8, None, 0, p, 8, p,
-                                     p, need - 1, None) == 4
+    assert L.mignn_rms_norm_backward_scratch_bytes(100, 8, 0) == 0     # one block's
+
+    def norm_backward(n, w, nbytes):
+        return L.mignn_rms_norm_backward(p, 8, None, 0, w, 1, n, 8, 1e-6, 0, p, 8, None, 0, p, 8, p,
+                                         p, nbytes, None)
+    assert norm_backward(1000, p, need - 1) == 4
+    assert norm_backward(0, None, need) == 1 and "null" in _lib.last_error()
 
     def rot(n=1, heads=1, d=8, pos_type=0, pairs=4, dtype=0, freq=p):
         return L.mignn_rotary(p, 8, 8, n, heads, d, p, pos_type, 1, freq, p, pairs, 0, 0, dtype, p,

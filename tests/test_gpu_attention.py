@@ -737,3 +737,21 @@ def test_out_of_memory_is_torch_s_error():
     x, pos = torch.zeros(1, 1, 64, device=DEV), torch.zeros(1, 1, device=DEV)
     with pytest.raises(torch.OutOfMemoryError):
         A.rotary(x.expand(1 << 33, 1, 64), pos.expand(1 << 33, 1), A.RotaryAxes((32,)))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("h", [8, 128, 257, 2048])
+def test_rms_norm_weight_gradient_around_one_block(dt, h):
+    """Rows on both sides of where one block takes all of them."""
+    vec = 4 if dt == torch.float32 else 8
+    lanes = 1
+    while lanes < 64 and lanes < -(-h // vec):
+        lanes *= 2
+    edge = 4 * 4 * (64 // lanes)
+    for n in (1, 2, edge - 1, edge, edge + 1, 2 * edge + 3):
+        for wt in {dt, torch.float32}:
+            x, dy = rnd(n, h, seed=n, dt=dt), rnd(n, h, seed=n + 1, dt=dt)
+            w = rnd(h, seed=3, dt=wt).requires_grad_()
+            gw, = torch.autograd.grad(A.rms_norm(x, w), w, dy)
+            _, rw, _, mw = orc.rms_norm_grads(x, w.detach(), None, 1e-6, dy)
+            close(gw, rw, (n + 128) * U * mw, wt, f"dw of {n} rows")
