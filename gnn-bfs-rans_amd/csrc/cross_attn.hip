@@ -389,8 +389,9 @@ extern "C" int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, in
     const PassPlan p = plan_pass(sh, seq, batch, kv_heads, dkv, static_cast<CrossItem*>(items),
                                  static_cast<CrossJoin*>(joins));
     free(seq);
-    MIGNN_REQUIRE(p.items * kv_heads <= INT32_MAX / 2 && p.joins <= INT32_MAX,
-                  "cross_plan: too many tiles");
+    // (a launch's threads are counted in 32 bits)
+    MIGNN_REQUIRE(p.items * kv_heads <= UINT32_MAX / 256 - 16, "cross_plan: too many tiles (%lld of %d key heads)",
+                  static_cast<long long>(p.items), kv_heads);
     info[0] = p.items;
     info[1] = p.joins;
     info[2] = p.slots * kv_heads * sh.tile * part_width(pass, d) * static_cast<int64_t>(sizeof(float));

@@ -140,7 +140,8 @@ int launch_rotary(RotArgs a, bool interleaved, hipStream_t st) {
     if (rows > 2048 / a.pairs) rows = 2048 / a.pairs;
     a.rows = rows < 1 ? 1 : static_cast<int>(rows);
     const int64_t blocks = (a.n + a.rows - 1) / a.rows;
-    MIGNN_REQUIRE(blocks <= INT32_MAX && per_row <= INT32_MAX / 4096, "rotary: too many rows or heads");
+    // (a launch's threads are counted in 32 bits)
+    MIGNN_REQUIRE(blocks <= UINT32_MAX / 256 && per_row <= INT32_MAX / 4096, "rotary: too many rows or heads");
     const unsigned grid = static_cast<unsigned>(blocks);
     const size_t lds = static_cast<size_t>(a.rows) * a.pairs * 2 * sizeof(float);
 #define MIGNN_ROT(VV, I) \

@@ -296,3 +296,26 @@ def test_block_axes_follow_its_settings():
     assert blk._rotary_axes(cpu).scales == (8.0,) * 3
     blk.base = 50.0
     assert blk._rotary_axes(cpu).base == 50.0
+
+
+def test_more_blocks_than_a_launch_holds_are_refused():
+    n = 2 ** 22
+    with pytest.raises(_lib.MignnError, match="too many tiles"):
+        A.CrossPlan(np.ones(n, np.int64), np.ones(n, np.int64), heads=4, head_dim=8, device="cpu",
+                    train=False)
+    L = _lib.lib()
+    buf = (ctypes.c_float * 64)()
+    p = (ctypes.addressof(buf) + 15) & ~15      # never dereferenced
+    assert L.mignn_rotary(p, 8192, 8192, 1 << 24, 1, 8192, p, 0, 1, p, p, 4096, 0, 0, 1, p, 8192, 8192,
+                          None) == 1 and "too many rows" in _lib.last_error()
+
+
+def test_block_and_axes_copy_and_pickle():
+    import copy
+    import pickle
+    blk = A.CrossAttention(64, 4)
+    axes = blk._rotary_axes(torch.device("cpu"))
+    for other in (copy.deepcopy(blk), pickle.loads(pickle.dumps(blk))):
+        assert other._axes.pairs == axes.pairs and torch.equal(other._axes.freq, axes.freq)
+        assert all(torch.equal(a, b) for a, b in zip(blk.state_dict().values(),
+                                                     other.state_dict().values()))
