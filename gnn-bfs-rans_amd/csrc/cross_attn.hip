@@ -221,9 +221,12 @@ int64_t pick_chunk(const PassShape& s, const Sequence* seq, int64_t batch, int k
     for (int64_t b = 0; b < batch; ++b) longest = seq[b].cn > longest ? seq[b].cn : longest;
     int64_t best = up(longest > 0 ? longest : 1, s.unit);
     double best_cost = -1.0;
+    int64_t last = 0;
     for (int64_t parts = 1; parts <= 256; ++parts) {
         const int64_t len = up((longest + parts - 1) / parts, s.unit);
         if (parts > 1 && len < s.least) break;
+        if (len == last) continue;
+        last = len;
         double items = 0.0;
         for (int64_t b = 0; b < batch; ++b)
             if (seq[b].cn > 0)

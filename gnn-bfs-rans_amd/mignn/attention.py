@@ -152,21 +152,21 @@ class CrossPlan:
         self.dtype, self.train = dtype, bool(train)
         self.queries, self.keys = int(ql.sum()), int(kl.sum())
         L = _lib.lib()
-        info = np.zeros(8, np.int64)
+        info = (ctypes.c_int64 * 8)()
+        lengths = ql.ctypes.data, kl.ctypes.data
         lists, spans, at = [], [], 0
         size = _lib.CROSS_ITEM_BYTES
         for kind in range(3 if train else 1):
             def plan(items, joins):
                 _lib.check(L.mignn_cross_plan(
-                    ql.ctypes.data, kl.ctypes.data, ql.size, self.heads, self.kv_heads,
-                    self.head_dim, _ROW[dtype], kind, items, joins, info.ctypes.data),
-                    "mignn_cross_plan")
+                    *lengths, ql.size, self.heads, self.kv_heads, self.head_dim, _ROW[dtype],
+                    kind, items, joins, info), "mignn_cross_plan")
             plan(None, None)
-            n_items, n_joins, part = (int(v) for v in info[:3])
-            buf = np.zeros((n_items + n_joins) * size, np.uint8)
-            plan(buf.ctypes.data, buf.ctypes.data + n_items * size)
-            spans.append((at, at + n_items * size, part, n_items, n_joins) +
-                         tuple(int(v) for v in info[5:]))
+            n_items, n_joins, part = info[:3]
+            buf = np.empty((n_items + n_joins) * size, np.uint8)
+            base = buf.ctypes.data
+            plan(base, base + n_items * size)
+            spans.append((at, at + n_items * size, part, n_items, n_joins) + tuple(info[5:]))
             lists.append(buf)
             at += buf.size
         host = torch.from_numpy(np.concatenate(lists))
