@@ -283,6 +283,16 @@ Tensor rotary(const Tensor& x, const Tensor& pos, const Tensor& freq, const Tens
 // ---------------------------------------------------------------------------
 // Cross attention
 
+// A plan's call moved from its lists at `from` to the same bytes at `to`
+mignn_cross_call moved(mignn_cross_call c, const void* from, const void* to) {
+    const uintptr_t by = reinterpret_cast<uintptr_t>(to) - reinterpret_cast<uintptr_t>(from);
+    for (mignn_cross_pass& p : c.pass) {
+        p.items = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(p.items) + by);
+        p.joins = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(p.joins) + by);
+    }
+    return c;
+}
+
 // a plan's call, with the tensors of one use filled in
 mignn_cross_call call_of(const mignn_cross_call& plan, const Tensor& q, const Tensor& k, const Tensor& v,
                          const Tensor& mask, double scale, const Tensor& scratch) {
@@ -328,14 +338,18 @@ CrossOut cross_forward(const mignn_cross_call& plan, const Tensor& q_, const Ten
 
 struct CrossAttention : torch::autograd::Function<CrossAttention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
-                          const OptTensor& mask, const Tensor& lists, const std::string& plan, double scale) {
-        mignn_cross_call c;
-        std::memcpy(&c, plan.data(), sizeof(c));
+                          const OptTensor& mask, const Tensor& lists, uint64_t plan, double scale) {
+        const auto& c = *reinterpret_cast<const mignn_cross_call*>(plan);
         const CrossOut o = cross_forward(c, q, k, v, value(mask), lists, scale, true);
         // out32 (the fp32 output): <do, o> from the rounded output would leave
-        // the rounding of o in every dS.  lists: the plan's, kept alive
-        ctx->save_for_backward({q, k, v, value(mask), o.out32, o.lse, lists});
-        ctx->saved_data["plan"] = plan;
+        // the rounding of o in every dS
+        ctx->save_for_backward({q, k, v, value(mask), o.out32, o.lse});
+        // The plan may be gone by the backward, and saved tensors may come back as
+        // others (saved-tensor hooks, checkpointing): the lists are held here,
+        // out of the hooks' reach, and the call holds distances into them
+        const mignn_cross_call placed = moved(c, ptr(lists), nullptr);
+        ctx->saved_data["lists"] = lists;
+        ctx->saved_data["plan"] = std::string(reinterpret_cast<const char*>(&placed), sizeof(placed));
         ctx->saved_data["scale"] = scale;
         return o.out;
     }
@@ -343,9 +357,12 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
         const auto saved = ctx->get_saved_variables();
         mignn_cross_call plan;
         std::memcpy(&plan, ctx->saved_data["plan"].toStringRef().data(), sizeof(plan));
+        const Tensor lists = ctx->saved_data["lists"].toTensor();
+        plan = moved(plan, nullptr, ptr(lists));
         const Tensor q = heads_of(saved[0], 16), k = heads_of(saved[1], 16), v = heads_of(saved[2], 16);
         const Tensor dout = heads_of(grads[0], 16), &mask = saved[3], &out32 = saved[4], &lse = saved[5];
         c10::DeviceGuard guard(q.device());
+        reads(lists);
         Tensor dq = at::empty(q.sizes(), q.options()), dk, dv;
         const bool keys = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
         if (keys) {
@@ -394,9 +411,20 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     const bool grad = needs_grad({&q, &k, &v});
     if (grad && !train) throw py::value_error("cross_attention: gradients need a plan built with train=True");
     if (grad)
-        return CrossAttention::apply(q, k, v, mask.defined() ? OptTensor(mask) : OptTensor(), lists,
-                                     std::string(reinterpret_cast<const char*>(&c), sizeof(c)), scale);
+        return CrossAttention::apply(q, k, v, mask.defined() ? OptTensor(mask) : OptTensor(), lists, plan,
+                                     scale);
     return cross_forward(c, q, k, v, mask, lists, scale, false).out;
+}
+
+// The addresses of a plan's lists (each pass's items and joins), as a backward
+// forms them that finds the lists at `at`
+std::vector<uint64_t> plan_places(uint64_t plan, const Tensor& lists, const Tensor& at) {
+    const mignn_cross_call c = moved(
+        moved(*reinterpret_cast<const mignn_cross_call*>(plan), ptr(lists), nullptr), nullptr, ptr(at));
+    std::vector<uint64_t> places;
+    for (const mignn_cross_pass& p : c.pass)
+        for (const void* a : {p.items, p.joins}) places.push_back(reinterpret_cast<uint64_t>(a));
+    return places;
 }
 
 }  // namespace
@@ -407,4 +435,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("rms_norm", &rms_norm);
     m.def("rotary", &rotary);
     m.def("cross_attention", &cross_attention);
+    m.def("plan_places", &plan_places);
 }

@@ -319,3 +319,19 @@ def test_block_and_axes_copy_and_pickle():
         assert other._axes.pairs == axes.pairs and torch.equal(other._axes.freq, axes.freq)
         assert all(torch.equal(a, b) for a, b in zip(blk.state_dict().values(),
                                                      other.state_dict().values()))
+
+
+@pytest.mark.parametrize("ql,kl", [([1], [20000]), ([300, 5], [900, 4000]), ([0], [9])])
+def test_backward_s_work_lists_follow_the_lists_it_holds(ql, kl):
+    """The backward forms the addresses of its work lists from the list tensor
+    in its hands, not from where the forward found the plan's."""
+    plan = A.CrossPlan(ql, kl, heads=4, kv_heads=2, head_dim=32, device="cpu")
+    other = plan._lists.clone()
+    assert other.data_ptr() != plan._lists.data_ptr()
+
+    def places(at):
+        return _lib.ops().plan_places(plan._address, plan._lists, at)
+    own = [p or 0 for ps in plan._call.passes for p in (ps.items, ps.joins)]
+    assert places(plan._lists) == own
+    assert [p - other.data_ptr() for p in places(other)] == \
+        [p - plan._lists.data_ptr() for p in own]
