@@ -97,6 +97,18 @@ void on_device(const char* what, const Tensor& ref, std::initializer_list<std::p
                                      ", not on " + ref.device().str());
 }
 
+// What saved-tensor hooks gave back for a saved tensor: the kernels read it by
+// the gradient's device and the forward's type and shape
+const Tensor& returned(const char* what, const char* name, const Tensor& t, const Tensor& grad, bool type_ok,
+                       at::IntArrayRef sizes) {
+    if (t.device() != grad.device() || !type_ok || t.sizes() != sizes)
+        throw std::runtime_error(std::string(what) + " backward: saved " + name + " came back as " +
+                                 c10::toString(t.scalar_type()) + " " + shape(t) + " on " + t.device().str() +
+                                 " (expected " + shape(sizes) + ", the type that was saved, on " +
+                                 grad.device().str() + ")");
+    return t;
+}
+
 // Gradients that autograd cannot differentiate again: under create_graph they
 // refuse it when asked.
 variable_list first_order(variable_list grads) {
@@ -154,15 +166,20 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
         const auto saved = ctx->get_saved_variables();
         const bool residual = ctx->saved_data["residual"].toBool();
         const bool want_w = ctx->needs_input_grad(1);
-        const Tensor x = matrix(saved[0]), w = saved[1].contiguous(), r = matrix(saved[2]);
         const Tensor dy = matrix(grads[0]), ds = residual ? matrix(grads[1]) : Tensor();
-        c10::DeviceGuard guard(x.device());
         Tensor dx, dw;
         if (!dy.defined()) {
             dx = ds;
-            if (want_w) dw = at::zeros_like(w);
+            if (want_w) dw = at::zeros_like(saved[1]);
         } else {
-            const int64_t n = x.size(0), h = x.size(1);
+            const int64_t n = dy.size(0), h = dy.size(1);
+            auto like_dy = [&](const Tensor& t) { return t.scalar_type() == dy.scalar_type(); };
+            for (int i : {0, 2})
+                if (saved[i].defined())
+                    returned("rms_norm", "rows", saved[i], dy, like_dy(saved[i]), dy.sizes());
+            returned("rms_norm", "weight", saved[1], dy, is_f32(saved[1]) || like_dy(saved[1]), {h});
+            const Tensor x = matrix(saved[0]), w = saved[1].contiguous(), r = matrix(saved[2]);
+            c10::DeviceGuard guard(dy.device());
             dx = at::empty({n, h}, x.options());
             Tensor scratch;
             size_t bytes = 0;
@@ -246,14 +263,22 @@ Tensor turn(const Tensor& x_, const Tensor& pos_, const Tensor& freq, const Tens
 struct Rotary : torch::autograd::Function<Rotary> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& pos, const Tensor& freq,
                           const Tensor& axis, bool interleaved) {
-        ctx->save_for_backward({pos, freq, axis});
+        ctx->save_for_backward({pos});
+        // the axes' tables: out of the hooks' reach
+        ctx->saved_data["freq"] = freq;
+        ctx->saved_data["axis"] = axis;
+        ctx->saved_data["axes"] = pos.size(1);
+        ctx->saved_data["pos_type"] = static_cast<int64_t>(pos.scalar_type());
         ctx->saved_data["interleaved"] = interleaved;
         return turn(x, pos, freq, axis, interleaved, false);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const auto saved = ctx->get_saved_variables();
-        return first_order({turn(grads[0], saved[0], saved[1], saved[2],
-                                 ctx->saved_data["interleaved"].toBool(), true),
+        const Tensor pos = ctx->get_saved_variables()[0];
+        returned("rotary", "pos", pos, grads[0],
+                 static_cast<int64_t>(pos.scalar_type()) == ctx->saved_data["pos_type"].toInt(),
+                 {grads[0].size(0), ctx->saved_data["axes"].toInt()});
+        return first_order({turn(grads[0], pos, ctx->saved_data["freq"].toTensor(),
+                                 ctx->saved_data["axis"].toTensor(), ctx->saved_data["interleaved"].toBool(), true),
                             Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
@@ -359,9 +384,22 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
         std::memcpy(&plan, ctx->saved_data["plan"].toStringRef().data(), sizeof(plan));
         const Tensor lists = ctx->saved_data["lists"].toTensor();
         plan = moved(plan, nullptr, ptr(lists));
-        const Tensor q = heads_of(saved[0], 16), k = heads_of(saved[1], 16), v = heads_of(saved[2], 16);
-        const Tensor dout = heads_of(grads[0], 16), &mask = saved[3], &out32 = saved[4], &lse = saved[5];
-        c10::DeviceGuard guard(q.device());
+        const Tensor& g = grads[0];
+        auto rows = [&](int i, const char* name, at::IntArrayRef sizes) {
+            const bool type_ok = saved[i].scalar_type() == g.scalar_type();
+            return heads_of(returned("cross_attention", name, saved[i], g, type_ok, sizes), 16);
+        };
+        auto flat = [&](int i, const char* name, at::ScalarType type, at::IntArrayRef sizes) {
+            const bool type_ok = saved[i].scalar_type() == type;
+            return returned("cross_attention", name, saved[i], g, type_ok, sizes).contiguous();
+        };
+        const std::array<int64_t, 3> key_rows{plan.n_keys, plan.kv_heads, plan.d};
+        c10::DeviceGuard guard(g.device());
+        const Tensor q = rows(0, "q", g.sizes()), k = rows(1, "k", key_rows), v = rows(2, "v", key_rows);
+        const Tensor mask = saved[3].defined() ? flat(3, "key_mask", at::kBool, {plan.n_keys}) : Tensor();
+        const Tensor out32 = flat(4, "output", at::kFloat, g.sizes());
+        const Tensor lse = flat(5, "statistics", at::kFloat, {g.size(0), g.size(1)});
+        const Tensor dout = heads_of(g, 16);
         reads(lists);
         Tensor dq = at::empty(q.sizes(), q.options()), dk, dv;
         const bool keys = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);

@@ -99,3 +99,40 @@ def test_surrogate_that_makes_its_own_plan(way):
     want = step("plain")
     assert same(step("plain"), want)
     assert same(step(way), want)
+
+
+@pytest.mark.parametrize("spoil", ["host", "type", "rows"])
+def test_hooks_that_give_back_other_tensors_are_refused(spoil):
+    """Each saved tensor in turn comes back on the host, in another type or a row
+    short: an error by name ahead of any launch."""
+    x, w = rnd(20, 64, seed=1).requires_grad_(), rnd(64, seed=2).requires_grad_()
+    q, k = rnd(20, 4, 32, seed=3).requires_grad_(), rnd(90, 2, 32, seed=4).requires_grad_()
+    mask = torch.ones(90, dtype=torch.bool, device=DEV)
+    pos = torch.rand(20, 2, device=DEV)
+    axes = A.RotaryAxes((4, 4))
+    plan = A.CrossPlan([20], [90], heads=4, kv_heads=2, head_dim=32)
+    change = {"host": lambda t: t.cpu(), "type": lambda t: t.to(torch.float64),
+              "rows": lambda t: t[:-1]}[spoil]
+    for what, f, leaf in [
+            ("rms_norm", lambda: A.rms_norm(x, w), x),
+            ("rms_norm", lambda: A.rms_norm(x, w, residual=x)[0], w),
+            ("rms_norm", lambda: A.rms_norm(x.half(), w, residual=x.half())[0], x),
+            ("rotary", lambda: A.rotary(q, pos, axes), q),
+            ("cross_attention", lambda: A.cross_attention(q, k, k, plan, key_mask=mask), k)]:
+        turn, kept = 0, [1]
+        while turn < kept[0]:
+            kept[0] = 0
+
+            def pack(t):
+                kept[0] += 1
+                return kept[0] - 1, t
+
+            def unpack(p):
+                return change(p[1]) if p[0] == turn else p[1]
+            with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+                y = f()
+            with pytest.raises(RuntimeError, match=f"{what} backward: saved"):
+                torch.autograd.grad(y.float().square().sum(), leaf)
+            turn += 1
+        assert turn == {"rms_norm": 3 if y.dtype == torch.float16 else 2, "rotary": 1,
+                        "cross_attention": 6}[what]
