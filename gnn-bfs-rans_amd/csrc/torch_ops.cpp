@@ -74,6 +74,18 @@ bool needs_grad(std::initializer_list<const Tensor*> ts) {
 // ---------------------------------------------------------------------------
 // Refusals
 
+[[noreturn]] void not_implemented(const std::string& message) {
+    PyErr_SetString(PyExc_NotImplementedError, message.c_str());
+    throw py::error_already_set();
+}
+// Dual tensors (forward-mode derivatives): their tangents would be dropped
+void no_tangents(const char* what, std::initializer_list<std::pair<const char*, const Tensor*>> inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const auto& [name, t] : inputs)
+        if (t->defined() && t->_fw_grad(0).defined())
+            not_implemented(std::string(what) + ": " + name + " carries a tangent (no forward-mode derivatives)");
+}
+
 std::string shape(at::IntArrayRef sizes) {
     std::string s = "(";
     for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);
@@ -214,6 +226,7 @@ py::object rms_norm(const Tensor& x, const Tensor& w, const OptTensor& r, double
                               dtype(*r));
     if (!(eps >= 0.0)) throw py::value_error("rms_norm: eps must not be negative, got " + number(eps));
     const Tensor res = value(r);
+    no_tangents("rms_norm", {{"x", &x}, {"weight", &w}, {"residual", &res}});
     on_device("rms_norm", x, {{"weight", &w}, {"residual", &res}});
     if (needs_grad({&x, &w}) || (r.has_value() && needs_grad({&*r}))) {
         variable_list o = RMSNorm::apply(x, w, r, eps);
@@ -296,10 +309,8 @@ Tensor rotary(const Tensor& x, const Tensor& pos, const Tensor& freq, const Tens
     if (2 * freq.numel() > x.size(2))
         throw py::value_error("rotary: " + std::to_string(freq.numel()) + " pairs do not fit heads of width " +
                               std::to_string(x.size(2)));
-    if (needs_grad({&pos})) {
-        PyErr_SetString(PyExc_NotImplementedError, "rotary: positions get no gradient (pass pos.detach())");
-        throw py::error_already_set();
-    }
+    if (needs_grad({&pos})) not_implemented("rotary: positions get no gradient (pass pos.detach())");
+    no_tangents("rotary", {{"x", &x}, {"pos", &pos}});
     on_device("rotary", x, {{"pos", &pos}, {"axes", &freq}});
     if (needs_grad({&x})) return Rotary::apply(x, pos, freq, axis, interleaved);
     return turn(x, pos, freq, axis, interleaved, false);
@@ -444,6 +455,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt(static_cast<double>(c.d));
     if (!(scale > 0.0 && scale < 1e30))
         throw py::value_error("cross_attention: scale must be positive and finite, got " + number(scale));
+    no_tangents("cross_attention", {{"q", &q}, {"k", &k}, {"v", &v}});
     on_device("cross_attention", q, {{"k", &k}, {"v", &v}, {"key_mask", &mask}, {"plan", &lists}});
     if (mask.defined()) mask = mask.contiguous();
     const bool grad = needs_grad({&q, &k, &v});

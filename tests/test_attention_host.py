@@ -335,3 +335,36 @@ def test_backward_s_work_lists_follow_the_lists_it_holds(ql, kl):
     assert places(plan._lists) == own
     assert [p - other.data_ptr() for p in places(other)] == \
         [p - plan._lists.data_ptr() for p in own]
+
+
+def test_forward_mode_tangents_are_refused_by_name():
+    """A dual tensor, with or without requires_grad: no output without its tangent."""
+    import torch.autograd.forward_ad as fwd
+    w, axes, pos = torch.ones(16), A.RotaryAxes((3, 3, 2), device="cpu"), torch.zeros(5, 3)
+    plan = A.CrossPlan([5], [5], heads=2, head_dim=16, device="cpu")
+    h = torch.zeros(5, 2, 16)
+    calls = {
+        "rms_norm: x": lambda d: A.rms_norm(d(torch.zeros(4, 16)), w),
+        "rms_norm: weight": lambda d: A.rms_norm(torch.zeros(4, 16), d(w)),
+        "rms_norm: residual": lambda d: A.rms_norm(torch.zeros(4, 16), w, d(torch.zeros(4, 16))),
+        "rotary: x": lambda d: A.rotary(d(h), pos, axes),
+        "rotary: pos": lambda d: A.rotary(h, d(pos), axes),
+        "cross_attention: q": lambda d: A.cross_attention(d(h), h, h, plan),
+        "cross_attention: k": lambda d: A.cross_attention(h, d(h), h, plan),
+        "cross_attention: v": lambda d: A.cross_attention(h, h, d(h), plan)}
+    for name, call in calls.items():
+        for leaf in (False, True):
+            with fwd.dual_level():
+                def dual(t):
+                    return fwd.make_dual(t.clone().requires_grad_(leaf and name != "rotary: pos"),
+                                         torch.ones_like(t))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), \
+                            pytest.raises(NotImplementedError, match=name + " carries a tangent"):
+                        call(dual)
+                # forward mode switched off, or the primal alone: an ordinary call
+                with fwd._set_fwd_grad_enabled(False), \
+                        pytest.raises(RuntimeError, match="ROCm devices only"):
+                    call(dual)
+                with pytest.raises(RuntimeError, match="ROCm devices only"):
+                    call(lambda t: fwd.unpack_dual(dual(t)).primal)
