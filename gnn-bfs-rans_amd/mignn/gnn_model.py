@@ -1362,6 +1362,11 @@ class FlowGNNSurrogate(nn.Module):
         self.cross = CrossAttention(hidden_dim, cross_heads, axes=min(3, input_dim)) \
             if cross_heads else None
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "cross" not in self._modules:    # a model pickled before there was one
+            self.__dict__.setdefault("cross", None)
+
     def forward(self, x, edge_index, edge_attr=None, boundary_conditions=None, context=None,
                 batch=None, plan=None):
         """context (only with cross_heads > 0, and then required): the second

@@ -368,3 +368,21 @@ def test_forward_mode_tangents_are_refused_by_name():
                     call(dual)
                 with pytest.raises(RuntimeError, match="ROCm devices only"):
                     call(lambda t: fwd.unpack_dual(dual(t)).primal)
+
+
+def test_surrogate_pickled_before_cross_attention_still_runs():
+    """A model saved whole when FlowGNNSurrogate had no `cross`, and one with it."""
+    import pickle
+    from mignn import Data, FlowGNNSurrogate
+    x, ei = torch.zeros(2, 3), torch.zeros(2, 0, dtype=torch.long)
+    m = FlowGNNSurrogate(hidden_dim=32, num_layers=2)
+    del m.__dict__["cross"]
+    old = pickle.loads(pickle.dumps(m))
+    assert old.cross is None and list(old.state_dict()) == list(FlowGNNSurrogate(
+        hidden_dim=32, num_layers=2).state_dict())
+    with pytest.raises(RuntimeError, match="ROCm devices only"):
+        old(x, ei)
+    with pytest.raises(ValueError, match="context is for"):
+        old(x, ei, context=Data(x=x, edge_index=ei))
+    new = pickle.loads(pickle.dumps(FlowGNNSurrogate(hidden_dim=32, num_layers=2, cross_heads=2)))
+    assert isinstance(new.cross, A.CrossAttention) and "cross" not in new.__dict__
