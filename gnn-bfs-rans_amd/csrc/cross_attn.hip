@@ -161,8 +161,9 @@ __global__ __launch_bounds__(256) void cross_join_grad_kernel(CrossArgs a, bool 
 // Tiles of the "r" side (rows or keys) times chunks of the "c" side.
 struct PassShape {
     int64_t tile;     // rows of a tile
+    bool exact;       // carries the remainders of P's and dS's rounding (16-bit rows; in tiles of 32 always)
     int64_t longest;  // of the r side
-    int64_t slots;    // workgroups that the card holds at a time
+    int64_t slots;    // workgroups that chunks are made for
     int64_t least;    // shortest chunk
     int64_t rest;     // the same for what whole tiles leave over
     double start, join, part;   // a workgroup's start, a join and each of its parts, in rows of the c side
@@ -178,23 +179,50 @@ struct Sequence {
 int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 
 // Tile: 8 rows where no sequence has more (forward: cross_few), 32 (one wave)
-// where none has more than 32 or there are few results of 16 bits (those tiles
-// are the exacter ones), else 128, four waves that share the staging of the
-// other side.  (32 for longer sequences saves padding but not time: LDS
+// where none has more than 32, else 128, four waves that share the staging of
+// the other side.  (32 for longer sequences saves padding but not time: LDS
 // holds few such workgroups; keys of three sequences of 78, 134 and 167: dk /
 // dv 108 us in tiles of 32, 61 in tiles of 128.)
+//
+// Few results of 16 bits (a kv head's output is below 32 KB) carry the
+// remainders of P's and dS's rounding: their error against 64 bits is then the
+// output's own rounding (bf16 1.7e-3 for 2.4e-3 without, fp16 2.1e-4 for
+// 2.9e-4).  A launch of few results seldom is bound by the matrix unit (127
+// rows of 128, 262144 keys, 4 heads, tiles of 128: forward 162 -> 187 us, dq 202 ->
+// 197, dk / dv 243 -> 283); one of many is (49181 x 4096 x 4 heads over 2 of 64,
+// trained, 1013 -> 1425; 2 x 16384^2 x 8 x 128 2313 -> 3197).
+// They take tiles of 32 as long as that is the faster: those spread over more
+// CUs, but each stages its own copy of the other side.  bf16, 4 heads, rows x
+// other side x columns, us in tiles of 32 / 128:
+//   forward  128 x 4096 x 64  14 / 18   40 x 32768 x 32  22 / 40    250 x 32768 x 64  51 / 51
+//            40 x 262144 x 64 97 / 135  127 x 4096 x 128 20 / 24    128 x 262144 x 64 171 / 134
+//            40 x 32768 x 128 60 / 52   127 x 32768 x 128 83 / 56   250 x 262144 x 64 288 / 176
+//   dq       128 x 4096 x 64  13 / 15   40 x 32768 x 32  30 / 25    8 of 40 x 32768 x 32 52 / 60
+//            250 x 4096 x 64  18 / 19   128 x 262144 x 32 147 / 74  127 x 32768 x 128 93 / 44
+//   dk / dv  128 x 4096 x 64  18 / 19   40 x 32768 x 32  34 / 28    8 of 40 x 32768 x 32 57 / 86
+//            250 x 4096 x 64  27 / 16   128 x 262144 x 32 161 / 101 127 x 32768 x 128 133 / 50
 PassShape pass_shape(const Sequence* seq, int64_t batch, int pass, int d, int dtype, int group) {
     const bool dkv = pass == MIGNN_CROSS_DKV;
-    PassShape s{128, 0, 512, 128, 128, 64.0, 0.0, 0.0, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
+    PassShape s{128, false, 0, 512, 128, 128, 64.0, 0.0, 0.0, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
     int64_t results = 0;   // of one kv head
+    double work = 0.0;     // products of one kv head and form
     for (int64_t b = 0; b < batch; ++b) {
         s.longest = seq[b].rn > s.longest ? seq[b].rn : s.longest;
         results += seq[b].rn * d;
+        work += static_cast<double>(seq[b].rn) * static_cast<double>(seq[b].cn) * d;
     }
+    const double limit = pass == MIGNN_CROSS_FORWARD ? (d <= 64 ? 0x1p30 : 0x1p27) : d <= 32 ? 0x1p29 : 0x1p25;
+    const bool few = dtype != MIGNN_ROW_F32 && results < 16384;
     if (pass == MIGNN_CROSS_FORWARD && s.longest <= CROSS_FEW) s.tile = CROSS_FEW;
-    else if (s.longest <= CROSS_ROWS || (dtype != MIGNN_ROW_F32 && results < 16384)) s.tile = CROSS_ROWS;
-    // registers and LDS: two workgroups of four waves a CU, one where the heads
-    // are wide and much is held in fp32; eight small ones
+    else if (s.longest <= CROSS_ROWS || (few && work <= limit)) s.tile = CROSS_ROWS;
+    s.exact = few && s.tile == 128;
+    // Workgroups that chunks are made for.  Four waves: two a CU (a forward or
+    // dq of narrow heads holds three; made for 768, 12225^2 fp32 took 475 -> 489
+    // us), one where the heads are wide and much is held in fp32.  One wave:
+    // eight a CU, more than LDS holds of wide heads (16 bits: five of 64
+    // columns, two of 128; fp32 one of 128), and joins are not priced there.
+    // (4096: the same; 1024: the same, or less: 16 of 20 rows x 4096 keys of 64,
+    // bf16, forward 27 -> 23 us.)
     const bool wide = dtype == MIGNN_ROW_F32 ? d > 64 || (dkv && d > 32) : dkv && d > 96;
     if (s.tile != 128) {
         s.slots = 2048;
@@ -311,7 +339,8 @@ void launch_join(const CrossArgs& a, int pass, hipStream_t st) {
 int run_pass(CrossArgs a, const mignn_cross_pass& ps, int pass, int dtype, hipStream_t st) {
     a.items = static_cast<const CrossItem*>(ps.items);
     a.joins = static_cast<const CrossJoin*>(ps.joins);
-    a.n_items = ps.n_items, a.n_joins = ps.n_joins, a.n_whole = ps.n_whole, a.tile = ps.tile, a.rows = ps.rows;
+    a.n_items = ps.n_items, a.n_joins = ps.n_joins, a.n_whole = ps.n_whole, a.rows = ps.rows;
+    a.tile = ps.tile & ~MIGNN_CROSS_EXACT, a.exact = (ps.tile & MIGNN_CROSS_EXACT) != 0;
     if (a.n_items > 0) {
         int rc;
         if (a.tile == CROSS_FEW) rc = cross_few(a, dtype, st);
@@ -400,7 +429,7 @@ extern "C" int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, in
     info[2] = p.slots * kv_heads * sh.tile * part_width(pass, d) * static_cast<int64_t>(sizeof(float));
     info[3] = queries;
     info[4] = keys;
-    info[5] = sh.tile;
+    info[5] = sh.tile | (sh.exact ? MIGNN_CROSS_EXACT : 0);
     info[6] = sh.longest;
     info[7] = p.whole;
     return MIGNN_OK;

@@ -48,6 +48,7 @@ struct CrossArgs {
     int64_t ldq, ldqh, ldk, ldkh, ldv, ldvh, lddo, lddoh;
     int32_t n_items, n_whole, n_joins, heads, kv_heads, group, d;
     int32_t tile, rows;          // of the pass: rows (keys) of a tile, of the longest sequence
+    int32_t exact;               // 16-bit rows: the roundings' remainders are carried
     float scale, c;              // c = scale log2(e)
 };
 

@@ -15,8 +15,8 @@
 // P and dS are rounded to the rows' type ahead of their second product (the
 // matrix instruction takes both operands in one type), which adds to a result
 // about what its own rounding does; statistics, sums and accumulators are fp32.
-// Tiles of 32 (few rows or few results: bound by latency, not by the matrix
-// unit) carry the roundings' remainders through a second product instead.
+// Where rows or results are few (the plan's rule) the roundings' remainders go
+// through a second product (REST), and only the output's rounding is left.
 // bf16 has fp32's range.  fp16 has not: a weight of 1 / 5000 is already
 // subnormal there, so P is carried up by a constant power of two and dS by one
 // that each row (dq) or key (dk) lowers when its values would not fit
@@ -151,7 +151,7 @@ struct DsScale {
     __device__ __forceinline__ float back() const { return NARROW<T> ? __builtin_amdgcn_exp2f(-up) : 1.f; }
 };
 
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool REST>
 __global__ __launch_bounds__(NW * 64, NW > 1 ? (DP <= 64 ? 3 : 2) : DP == 32 ? 2 : 1) void cross_fwd16_kernel(CrossArgs a) {
     constexpr int TILE = KT * TileRow<DP>::BYTES, NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];   // K, V; twice
@@ -241,11 +241,11 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? (DP <= 64 ? 3 : 2) : DP == 32 ? 2
 #pragma unroll
         for (int t = 0; t < KT / 16; ++t) {
             const vec8<T> p = pack8<T>(s[t >> 1], t & 1);
-            const vec8<T> rest = NW == 1 ? rest8<T>(s[t >> 1], p, t & 1) : p;
+            const vec8<T> rest = REST ? rest8<T>(s[t >> 1], p, t & 1) : p;
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b) {
                 const vec8<T> f = tr_frag<T, DP>(vt, tl, 16 * t, b);
-                if constexpr (NW == 1) o[b] = mfma16(f, rest, o[b]);
+                if constexpr (REST) o[b] = mfma16(f, rest, o[b]);
                 o[b] = mfma16(f, p, o[b]);
             }
         }
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? (DP <= 64 ? 3 : 2) : DP == 32 ? 2
     if (a.lse && half == 0) a.lse[at] = sum == 0.f ? INFINITY : m2 + log2f(sum);
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool REST>
 __global__ __launch_bounds__(NW * 64, NW > 1 ? (DP <= 64 ? 3 : 2) : DP == 32 ? 2 : 1) void cross_dq16_kernel(CrossArgs a) {
     constexpr int TILE = KT * TileRow<DP>::BYTES, NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
@@ -366,11 +366,11 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? (DP <= 64 ? 3 : 2) : DP == 32 ? 2
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const vec8<T> p = pack8<T>(s, t);
-                const vec8<T> rest = NW == 1 ? rest8<T>(s, p, t) : p;
+                const vec8<T> rest = REST ? rest8<T>(s, p, t) : p;
 #pragma unroll
                 for (int b = 0; b < DP / 32; ++b) {
                     const vec8<T> f = tr_frag<T, DP>(kt, tl, 32 * hb + 16 * t, b);
-                    if constexpr (NW == 1) acc[b] = mfma16(f, rest, acc[b]);
+                    if constexpr (REST) acc[b] = mfma16(f, rest, acc[b]);
                     acc[b] = mfma16(f, p, acc[b]);
                 }
             }
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 ? (DP <= 64 ? 3 : 2) : DP == 32 ? 2
         store_acc<T, DP>(static_cast<T*>(a.out) + at * a.d, acc, f, a.d, half);
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool REST>
 __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cross_dkv16_kernel(CrossArgs a) {
     constexpr int TILE = KT * TileRow<DP>::BYTES, NT = NW * 64;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
@@ -480,13 +480,13 @@ __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cro
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const vec8<T> p = pack8<T>(s, t), ds = pack8<T>(dp, t);
-                const vec8<T> p_rest = NW == 1 ? rest8<T>(s, p, t) : p;
-                const vec8<T> ds_rest = NW == 1 ? rest8<T>(dp, ds, t) : ds;
+                const vec8<T> p_rest = REST ? rest8<T>(s, p, t) : p;
+                const vec8<T> ds_rest = REST ? rest8<T>(dp, ds, t) : ds;
 #pragma unroll
                 for (int b = 0; b < DP / 32; ++b) {
                     const vec8<T> fg = tr_frag<T, DP>(gt, tl, 32 * rb + 16 * t, b);
                     const vec8<T> fq = tr_frag<T, DP>(qt, tl, 32 * rb + 16 * t, b);
-                    if constexpr (NW == 1) {
+                    if constexpr (REST) {
                         dv[b] = mfma16(fg, p_rest, dv[b]);
                         dk[b] = mfma16(fq, ds_rest, dk[b]);
                     }
@@ -518,21 +518,22 @@ __global__ __launch_bounds__(NW * 64, DP <= (NW > 1 ? 96 : 32) ? 2 : 1) void cro
     }
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool REST>
 void launch16_tile(const CrossArgs& a, int pass, hipStream_t st) {
     const dim3 grid(cross_grid(a)), block(NW * 64);
     if (pass == MIGNN_CROSS_FORWARD)
-        hipLaunchKernelGGL((cross_fwd16_kernel<T, DP, NW>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((cross_fwd16_kernel<T, DP, NW, REST>), grid, block, 0, st, a);
     else if (pass == MIGNN_CROSS_DQ)
-        hipLaunchKernelGGL((cross_dq16_kernel<T, DP, NW>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((cross_dq16_kernel<T, DP, NW, REST>), grid, block, 0, st, a);
     else
-        hipLaunchKernelGGL((cross_dkv16_kernel<T, DP, NW>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((cross_dkv16_kernel<T, DP, NW, REST>), grid, block, 0, st, a);
 }
 
 template <typename T, int DP>
 void launch16(const CrossArgs& a, int pass, hipStream_t st) {
-    if (a.tile == CROSS_ROWS) launch16_tile<T, DP, 1>(a, pass, st);
-    else launch16_tile<T, DP, 4>(a, pass, st);
+    if (a.tile == CROSS_ROWS) launch16_tile<T, DP, 1, true>(a, pass, st);
+    else if (a.exact) launch16_tile<T, DP, 4, true>(a, pass, st);
+    else launch16_tile<T, DP, 4, false>(a, pass, st);
 }
 
 template <typename T>

@@ -774,6 +774,7 @@ int mignn_rotary(const void* x, int64_t ldt, int64_t ldh, int64_t n, int heads, 
 #define MIGNN_CROSS_MAX_GROUP 32          /* query heads a key head */
 #define MIGNN_CROSS_MAX_STRIDE (1 << 23)  /* of rows and heads, elements */
 #define MIGNN_CROSS_ITEM_BYTES 32
+#define MIGNN_CROSS_EXACT (1 << 16)       /* in a pass's tile: 16-bit rows carry the remainders of roundings */
 enum { MIGNN_CROSS_FORWARD = 0, MIGNN_CROSS_DQ = 1, MIGNN_CROSS_DKV = 2 };
 int mignn_cross_plan(const int64_t* q_lens, const int64_t* k_lens, int64_t batch, int heads,
                      int kv_heads, int d, int dtype, int pass, void* items, void* joins,
@@ -783,7 +784,7 @@ typedef struct {
     const void* joins;      /* device */
     int64_t part_bytes;
     int32_t n_items, n_joins;
-    int32_t tile, rows;     /* rows (keys) of a tile; of the longest sequence */
+    int32_t tile, rows;     /* rows (keys) of a tile (as the plan gives it); of the longest sequence */
     int32_t n_whole;        /* items ahead of the split ones */
     int32_t reserved;
 } mignn_cross_pass;
