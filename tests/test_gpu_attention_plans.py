@@ -92,3 +92,18 @@ def test_few_results_of_long_passes_carry_the_remainders(ql, kl, heads, kv, d, k
     for kind, name in enumerate("fqk"):
         if name in kinds:
             assert plan._call.passes[kind].tile == 128 | EXACT, name
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ql,kl,heads,kv,d,kinds", [
+    ([33000, 70], [600, 50], 4, 2, 32, "fq"), ([600], [66000], 4, 2, 32, "k"),
+    ([17000], [600], 4, 4, 64, "fq"), ([260], [66000], 4, 2, 64, "k"),
+    ([16512], [600], 4, 4, 128, "fq")])
+def test_whole_and_split_tiles_in_one_pass(ql, kl, heads, kv, d, kinds, dt):
+    """More tiles than the card holds at a time, the last round's split and
+    joined: both ranges of a launch's workgroups, joins of some tiles only."""
+    plan = check(ql, kl, heads, kv, d, dt, masked=True)
+    for kind, name in enumerate("fqk"):
+        p = plan._call.passes[kind]
+        if name in kinds:
+            assert p.tile == 128 and 0 < p.n_whole < p.n_items and p.n_joins > 0, name
