@@ -184,16 +184,28 @@ int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 // holds few such workgroups; keys of three sequences of 78, 134 and 167: dk /
 // dv 108 us in tiles of 32, 61 in tiles of 128.)
 //
-// Few results of 16 bits (a kv head's output is below 32 KB) carry the
-// remainders of P's and dS's rounding: their error against 64 bits is then the
-// output's own rounding (bf16 1.7e-3 for 2.4e-3 without, fp16 2.1e-4 for
-// 2.9e-4).  A launch of few results seldom is bound by the matrix unit (127
-// rows of 128, 262144 keys, 4 heads, tiles of 128: forward 162 -> 187 us, dq 202 ->
-// 197, dk / dv 243 -> 283); one of many is (49181 x 4096 x 4 heads over 2 of 64,
-// trained, 1013 -> 1425; 2 x 16384^2 x 8 x 128 2313 -> 3197).
-// They take tiles of 32 as long as that is the faster: those spread over more
-// CUs, but each stages its own copy of the other side.  bf16, 4 heads, rows x
-// other side x columns, us in tiles of 32 / 128:
+// The remainders of P's and dS's rounding to 16 bits are carried where that
+// costs little or where their loss shows most.  Errors against 64 bits, in units
+// of what the output's own rounding leaves (bf16 1.7e-3, fp16 2.1e-4): 1.0 with
+// the remainders, 1.4 without.  They are half the matrix work again: 49181 x
+// 4096 x 4 heads over 2 of 64, trained, would take 1425 for 1013 us, 2 x 16384^2 x 8
+// x 128 3197 for 2313.  They are carried
+//   for few results (a kv head's output is below 32 KB): such a launch seldom is
+//     bound by the matrix unit (127 rows of 128, 262144 keys, 4 heads: forward 162
+//     -> 187 us, dq 202 -> 197, dk / dv 243 -> 283);
+//   where the other side is one LDS tile: bound by memory, and a few large weights'
+//     errors are most of a result's (dv of 35 sequences of one row, 2606 keys, 2
+//     heads of 24, fp16: 1.54 without).  36675 rows or keys x 64 x 4 heads over 2 of
+//     64: forward 16.0 -> 16.0 us, dq 25.0 -> 25.3, dk / dv 21.3 -> 24.6; 4 of 128:
+//     28 -> 30, 58 -> 54, 63 -> 67;
+//   in dq of heads to 16 columns: a row's dS sum to 0, which takes the keys' common
+//     part out of dq but not out of the roundings, and in few columns that is much
+//     of a key (16 columns 1.50 -> 1.03; without them 24 columns 1.48, 32 1.46, 64
+//     1.43).  Up to 8 of 12077 x 13392 x 2 heads of 16, trained, 916 -> 1025 us.
+//
+// Few results take tiles of 32 as long as that is the faster: those spread over
+// more CUs, but each stages its own copy of the other side.  bf16, 4 heads,
+// rows x other side x columns, us in tiles of 32 / 128:
 //   forward  128 x 4096 x 64  14 / 18   40 x 32768 x 32  22 / 40    250 x 32768 x 64  51 / 51
 //            40 x 262144 x 64 97 / 135  127 x 4096 x 128 20 / 24    128 x 262144 x 64 171 / 134
 //            40 x 32768 x 128 60 / 52   127 x 32768 x 128 83 / 56   250 x 262144 x 64 288 / 176
@@ -206,8 +218,10 @@ PassShape pass_shape(const Sequence* seq, int64_t batch, int pass, int d, int dt
     PassShape s{128, false, 0, 512, 128, 128, 64.0, 0.0, 0.0, dkv ? CROSS_STAGE / group * group : CROSS_STAGE};
     int64_t results = 0;   // of one kv head
     double work = 0.0;     // products of one kv head and form
+    int64_t other = 0;     // longest of the c side
     for (int64_t b = 0; b < batch; ++b) {
         s.longest = seq[b].rn > s.longest ? seq[b].rn : s.longest;
+        other = seq[b].cn > other ? seq[b].cn : other;
         results += seq[b].rn * d;
         work += static_cast<double>(seq[b].rn) * static_cast<double>(seq[b].cn) * d;
     }
@@ -215,7 +229,8 @@ PassShape pass_shape(const Sequence* seq, int64_t batch, int pass, int d, int dt
     const bool few = dtype != MIGNN_ROW_F32 && results < 16384;
     if (pass == MIGNN_CROSS_FORWARD && s.longest <= CROSS_FEW) s.tile = CROSS_FEW;
     else if (s.longest <= CROSS_ROWS || (few && work <= limit)) s.tile = CROSS_ROWS;
-    s.exact = few && s.tile == 128;
+    const bool narrow = pass == MIGNN_CROSS_DQ && d <= 16;
+    s.exact = s.tile == 128 && dtype != MIGNN_ROW_F32 && (few || other <= CROSS_STAGE || narrow);
     // Workgroups that chunks are made for.  Four waves: two a CU (a forward or
     // dq of narrow heads holds three; made for 768, 12225^2 fp32 took 475 -> 489
     // us), one where the heads are wide and much is held in fp32.  One wave:

@@ -85,8 +85,10 @@ def check(ql, kl, heads, kv, d, dt, masked=False):
     ([70, 55], [34000, 33700], 2, 1, 64, "q"), ([2500], [230], 2, 2, 64, "k"),
     ([33, 260], [11, 65000], 2, 2, 32, "q"), ([3000, 5], [400, 90], 3, 1, 32, ""),
     ([250], [68000], 1, 1, 64, "fq"), ([505], [67000], 1, 1, 32, "fq"),
-    ([20000, 40], [500, 1], 2, 1, 32, "k")])
-def test_few_results_of_long_passes_carry_the_remainders(ql, kl, heads, kv, d, kinds, dt):
+    ([20000, 40], [500, 1], 2, 1, 32, "k"),
+    ([1] * 35, [75 * i for i in range(35)], 2, 2, 24, "k"), ([9, 16], [3000, 1], 8, 2, 64, "k"),
+    ([700, 300], [64, 1], 4, 2, 128, "fq"), ([2000], [63], 2, 1, 96, "fq")])
+def test_few_results_and_short_passes_carry_the_remainders(ql, kl, heads, kv, d, kinds, dt):
     """128-row tiles with the remainders, at every width, ragged and grouped."""
     plan = check(ql, kl, heads, kv, d, dt, masked=True)
     for kind, name in enumerate("fqk"):
@@ -107,3 +109,10 @@ def test_whole_and_split_tiles_in_one_pass(ql, kl, heads, kv, d, kinds, dt):
         p = plan._call.passes[kind]
         if name in kinds:
             assert p.tile == 128 and 0 < p.n_whole < p.n_items and p.n_joins > 0, name
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [8, 16, 24])
+def test_dq_of_narrow_heads_carries_the_remainders(d, dt):
+    plan = check([2100, 300], [700, 1234], 4, 2, d, dt, masked=True)
+    assert plan._call.passes[1].tile == (128 | EXACT if d <= 16 else 128)
