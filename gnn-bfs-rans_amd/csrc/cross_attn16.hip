@@ -22,9 +22,10 @@
 // that each row (dq) or key (dk) lowers when its values would not fit
 // (DsScale); the results are brought back in fp32.
 //
-// Bound by issue: the matrix and the vector unit (exponentials, maxima,
-// roundings) are each busy about 44 % of the time and take turns within a
-// wave, so it is other waves that fill the gaps.  Measured (a plain product of
+// Bound by issue: the vector unit (exponentials, maxima, roundings) and the
+// matrix unit take turns within a wave, so it is other waves that fill the gaps
+// (busy, of 128 columns: 45 % each; of 64: 62 / 36 % in the forward, 58 / 46 in dq,
+// 47 / 43 in dk / dv).  Measured (a plain product of
 // 8192^3 reaches 1203 TFLOP/s in bf16, 1150 in fp16): 49181 rows x 4096 keys x 4
 // heads over 2 of 64, bf16: forward 270 us (763 TFLOP/s), dq 340 (909), dk / dv
 // 460 (897); 2 x 16384^2 x 8 x 128, fp16: forward 2370 (928; 2105 us with the

@@ -13,8 +13,8 @@
 // instruction takes 512 (which measured, at 12225 x 12225 x 4 x 32: 840 us
 // against 468, 163 TFLOP/s; a plain fp32 product of 8192^3 reaches 153).  The
 // tiles are split once a workgroup, on their way into LDS; what a wave owns at
-// the start; P and dS in registers, in place.  Bound by the vector unit (81 %
-// busy, most of it the splits; the matrix unit 45 %).  Trained, 19488 rows
+// the start; P and dS in registers, in place.  Bound by the vector unit (80 %
+// busy, most of it the splits; the matrix unit 47 %).  Trained, 19488 rows
 // against 379 keys in three sequences, 4 heads of 64: forward 27 us, dq 44, dk
 // / dv 62.
 #include "mfma16.hpp"
