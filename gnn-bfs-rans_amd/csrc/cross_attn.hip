@@ -193,14 +193,15 @@ int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 //   for few results (a kv head's output is below 32 KB): such a launch seldom is
 //     bound by the matrix unit (127 rows of 128, 262144 keys, 4 heads: forward 162
 //     -> 187 us, dq 202 -> 197, dk / dv 243 -> 283);
-//   where the other side is one LDS tile: bound by memory, and a few large weights'
-//     errors are most of a result's (dv of 35 sequences of one row, 2606 keys, 2
-//     heads of 24, fp16: 1.54 without).  36675 rows or keys x 64 x 4 heads over 2 of
-//     64: forward 16.0 -> 16.0 us, dq 25.0 -> 25.3, dk / dv 21.3 -> 24.6; 4 of 128:
-//     28 -> 30, 58 -> 54, 63 -> 67;
-//   in dq of heads to 16 columns: a row's dS sum to 0, which takes the keys' common
-//     part out of dq but not out of the roundings, and in few columns that is much
-//     of a key (16 columns 1.50 -> 1.03; without them 24 columns 1.48, 32 1.46, 64
+//   in gradients that go through one LDS tile: bound by memory, and a few large
+//     weights' errors are most of a result's (dv of 35 sequences of one row, 2606
+//     keys, 2 heads of 24, fp16: 1.54 without), while a row's dS sum to 0, which
+//     takes the keys' common part out of dq but not out of the roundings (2 x 5742
+//     x up to 5 keys, 8 heads over 2 of 24, bf16: 1.65).  36675 rows or keys x 64 x 4
+//     heads over 2 of 64: dq 25.0 -> 25.3 us, dk / dv 21.3 -> 24.6; 4 of 128: 58 -> 54,
+//     63 -> 67.  (The forward stays below 1.42 without.);
+//   in dq of heads to 16 columns, where the common part is much of a key at any
+//     length (16 columns 1.50 -> 1.03; without them 24 columns 1.48, 32 1.46, 64
 //     1.43).  Up to 8 of 12077 x 13392 x 2 heads of 16, trained, 916 -> 1025 us.
 //
 // Few results take tiles of 32 as long as that is the faster: those spread over
@@ -229,8 +230,8 @@ PassShape pass_shape(const Sequence* seq, int64_t batch, int pass, int d, int dt
     const bool few = dtype != MIGNN_ROW_F32 && results < 16384;
     if (pass == MIGNN_CROSS_FORWARD && s.longest <= CROSS_FEW) s.tile = CROSS_FEW;
     else if (s.longest <= CROSS_ROWS || (few && work <= limit)) s.tile = CROSS_ROWS;
-    const bool narrow = pass == MIGNN_CROSS_DQ && d <= 16;
-    s.exact = s.tile == 128 && dtype != MIGNN_ROW_F32 && (few || other <= CROSS_STAGE || narrow);
+    const bool lossy = pass != MIGNN_CROSS_FORWARD && (other <= CROSS_STAGE || (!dkv && d <= 16));
+    s.exact = s.tile == 128 && dtype != MIGNN_ROW_F32 && (few || lossy);
     // Workgroups that chunks are made for.  Four waves: two a CU (a forward or
     // dq of narrow heads holds three; made for 768, 12225^2 fp32 took 475 -> 489
     // us), one where the heads are wide and much is held in fp32.  One wave:

@@ -198,11 +198,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Cro
     fp32 rows are multiplied as three bf16 terms each, to fp32's own rounding;
     there an infinite key or value makes NaN of the queries that read it.  16-bit
     rows: the weights (and, in the backward, the scores' gradients) are rounded
-    to the rows' type ahead of their product with the values, but for passes of
-    few results (a key head's output, or its keys' gradient, of less than 16384
-    numbers, or no sequence above 32 rows) over at most 64 rows, and dq of
-    heads to 16 columns, which keep the remainders: what a row's last bits are depends on the plan that it is
-    part of."""
+    to the rows' type ahead of their product with the values, but for
+    passes of few results (a key head's output, or its keys' gradient, of less
+    than 16384 numbers, or no sequence above 32 rows), gradients over at most 64
+    keys or rows, and queries' gradients of heads to 16 columns, which keep the
+    remainders: what a row's last bits are depends on the plan that it is part of."""
     return _lib.ops().cross_attention(q, k, v, key_mask, scale, plan._lists, plan._address,
                                       plan.queries, plan.train)
 

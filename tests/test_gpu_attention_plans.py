@@ -87,8 +87,8 @@ def check(ql, kl, heads, kv, d, dt, masked=False):
     ([250], [68000], 1, 1, 64, "fq"), ([505], [67000], 1, 1, 32, "fq"),
     ([20000, 40], [500, 1], 2, 1, 32, "k"),
     ([1] * 35, [75 * i for i in range(35)], 2, 2, 24, "k"), ([9, 16], [3000, 1], 8, 2, 64, "k"),
-    ([700, 300], [64, 1], 4, 2, 128, "fq"), ([2000], [63], 2, 1, 96, "fq")])
-def test_few_results_and_short_passes_carry_the_remainders(ql, kl, heads, kv, d, kinds, dt):
+    ([700, 300], [64, 1], 4, 2, 128, "q"), ([32], [2000], 2, 1, 96, "k")])
+def test_few_results_and_short_gradients_carry_the_remainders(ql, kl, heads, kv, d, kinds, dt):
     """128-row tiles with the remainders, at every width, ragged and grouped."""
     plan = check(ql, kl, heads, kv, d, dt, masked=True)
     for kind, name in enumerate("fqk"):
