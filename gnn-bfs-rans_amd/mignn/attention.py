@@ -12,7 +12,7 @@ of libmignn.so (through _ops.so, csrc/torch_ops.cpp, which also checks the
 arguments) on the tensors' device and its current stream; there is no CPU path.
 Outputs and scratch come from PyTorch's allocator at every call, so calls on
 several streams, or captured into several graphs, share nothing but the
-read-only `RotaryAxes` / `CrossPlan`.  Gradients are first order only.
+read-only `RotaryAxes` / `CrossPlan`.  Gradients are first order and reverse mode only.
 
 A graph batch is a list of lengths (one sequence a graph), rows back to back.
 """
